@@ -312,6 +312,44 @@ LQ_API int lq_i8_gemm_i32_ws(const int8_t* a, const int8_t* b, int32_t* c, int M
 LQ_API int lq_i8_gemm_scaled_ws(const int8_t* a, const int8_t* b, const float* a_scale, const float* b_scale, void* y,
                          int out_dtype, int M, int N, int K, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- mixture-of-experts layers (no counterpart in the reference, whose plugin leaves such layers unquantised) ----
+ *
+ * Router: chooses `topk` of E experts for each of T tokens.  Scores are softmax(logits) (scoring 0) or sigmoid(logits) (1)
+ * of logits [T, E] (logits_dtype: LQ_DT_*).  Experts are chosen by score + bias[E] (bias may be null: by score), the
+ * largest first, the lowest index among equals.  n_group > 1: the experts form n_group groups of E / n_group neighbours, and
+ * only those of the topk_group best groups can be chosen; a group ranks by its largest key (group_score 0) or by the sum of
+ * its two largest (1), the lowest index among equals.  weights [T, topk] are the chosen scores (without bias), divided by their sum
+ * with `renormalize`, times `scale`.  A logit of -inf or NaN takes its expert out of the choice (and adds nothing to the softmax);
+ * where fewer than topk experts are left the remaining slots hold id -1 and weight 0.
+ * E <= 512, topk <= 32, E % n_group == 0, topk <= topk_group * (E / n_group). */
+LQ_API int lq_moe_route(const void* logits, int logits_dtype, const float* bias, float* weights, int32_t* ids, int T,
+                        int E, int topk, int scoring, int n_group, int topk_group, int group_score, int renormalize,
+                        float scale, void* stream);
+
+/* Grouped W4A8 / INT8 product: for token t and slot j with expert e = ids[t, j],
+ *   y[t, j, :] = (out type)((float)(xq . q[e, n, :]) * ascale * s1[e, n]),
+ * exact int32 sums, two float32 multiplies, one rounding: what lq_w4a8_gemm_fused / lq_i8_gemm_scaled compute for one matrix.
+ * An id outside [0, E) is no expert: its row is zero.  x: [T, K], or [T, topk, K] with x_per_pair; x_dtype LQ_DT_* (each row is
+ * quantised as by lq_quant_per_token) or 3 = INT8 with one scale per row in x_scale (null otherwise).  w_kind 0: E tile blobs one
+ * behind the other (lq_tile_blob_bytes(N, K) each), 1: INT8 [E, N, K].  s1 [E, N].  y [T, topk, N].
+ * K % 128 == 0, E <= 512, topk <= 32, T * topk <= 2^24; x, w and scratch 16-byte aligned.
+ * `scratch`: lq_experts_linear_scratch_bytes() bytes, any content (0 from that function: sizes out of range). */
+LQ_API size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K);
+LQ_API int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_per_pair, const int32_t* ids,
+                             const void* w, int w_kind, const float* s1, void* y, int out_dtype, int T, int topk, int E,
+                             int N, int K, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Gated MLP of the chosen experts, y [T, H] in out_dtype:
+ *   h = silu(gate) * up  (float32) of the product of x with w13[e], quantised to INT8 with one scale per (token, slot),
+ *   y[t] = sum_j weights[t, j] * (product of h with w2[e])  in float32, slot by slot, rounded once.
+ * w13 [E, 2 I, H] holds gate channel c in row 2 c and up channel c in row 2 c + 1; w2 [E, H, I]; both in the form of
+ * w_kind.  weights [T, topk] float32; an id outside [0, E) adds nothing.  H % 128 == 0 and I % 128 == 0, the other limits as
+ * above; s13 and s2 16-byte aligned. */
+LQ_API size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I);
+LQ_API int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32_t* ids, const void* w13,
+                          const float* s13, const void* w2, const float* s2, int w_kind, void* y, int out_dtype, int T,
+                          int topk, int E, int H, int I, void* scratch, size_t scratch_bytes, void* stream);
+
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,456 @@
+// Grouped W4A8 / INT8 product of a mixture-of-experts layer: for every tile of up to BN sorted activation rows of one
+// expert, out = rows x weights(expert)^T in exact int32, then one of three epilogues (see OutMode).
+//
+// The kernel is the two-CTAs-per-SM tile kernel of the dense linear (lq_gemm_tile.cu) made persistent: the number of tiles is
+// known on the device only (it depends on how the tokens chose), so CTA b takes work items b, b + grid, ... of the plan's
+// tiles x channel blocks x k-ranges and its rings run on from one item to the next: the copies and the unpacking of the next
+// item start while the sums of the last one are read out.  Item order: channel blocks fastest, so that the
+// CTAs at work at one time share a few row tiles, and the row tiles of one expert follow each other and find its weights in L2.
+//
+// A tile's width is what its rows need: the rows come in boxes of kBox rows, as many as cover the tile, and the MMA's N is
+// that many rows.  A box may reach past the last row of its expert: it then holds rows of the next expert (or, past the
+// end, zeros), whose sums are not stored.
+//
+// Per CTA: warp 0 = copies (8704-byte bulk copy of a blob tile, or a 128 x 128 box of INT8 weights; boxes of rows), warp 1 =
+// tensor-memory allocation and MMA issue, warps 2..5 and 6..9 = two sets that unpack alternate k-steps into tensor memory
+// (4-bit weights) and share every epilogue.  The stage counts are even wherever two sets take turns, so that a set
+// sees every use of its stages.  All waits are bounded; status codes 161-166.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "lq_experts.cuh"
+#include "lq_sched.cuh"
+#include "lq_tc_ptx.cuh"
+
+namespace lq {
+
+int make_byte_matrix_map(CUtensorMap* map, const void* ptr, long rows, long row_bytes, int box_rows,
+                         int box_bytes);  // lq_gemm_tc.cu
+
+namespace experts {
+
+constexpr int kBlobTile = 8704;
+constexpr int kSets = 2;
+constexpr int kThreads = 64 + 128 * kSets;
+constexpr int kNT = 4;                      // operand stages in tensor memory (4-bit weights)
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+
+struct Args {
+  const uint8_t* blob;
+  const float* s1;
+  const float* ascale;
+  const int* counts;
+  const int4* tiles;
+  const int* pair_of_pos;
+  void* out;
+  unsigned* amax;
+  int* status;
+  long rows;
+  int out_mode, out_dtype;
+  int N, kt_total, n_tiles, splits;
+};
+
+template <int BN, int NS, bool W4>
+struct Cfg {
+  static constexpr int kBox = BN >= 64 ? 32 : 16;
+  static constexpr int kXStage = BN * 128;
+  static constexpr int kWStage = W4 ? kBlobTile : 128 * 128;
+  static constexpr int kAcc = BN <= 64 || !W4 ? 2 : 1;        // accumulators
+  static constexpr int kCols = kAcc * BN + (W4 ? 32 * kNT : 0);
+  static constexpr int kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
+  static constexpr int kNumBars = 2 * NS + 2 * kNT + 2 * kAcc;
+  static constexpr int kSmemBytes = 1024 /* alignment slack */ + NS * (kXStage + kWStage) + kNumBars * 8 + 16;
+  static_assert(kCols <= 256, "two CTAs per SM share 512 columns");
+  static_assert(!W4 || NS % kSets == 0, "a set must see every use of its stages");
+  static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
+};
+
+// One work item: k-steps [kb, ke) of channel block nt for the rows [row0, row0 + rows) of an expert.
+struct Item {
+  int expert, row0, rows, nt, s, kb, ke;
+};
+__device__ __forceinline__ Item item_at(const Args& a, int i) {
+  Item it;
+  const int per_tile = a.n_tiles * a.splits;
+  const int t = i / per_tile;
+  const int in = i - t * per_tile;
+  it.s = in / a.n_tiles;
+  it.nt = in - it.s * a.n_tiles;
+  const int4 tile = __ldcg(a.tiles + t);
+  it.expert = tile.x;
+  it.row0 = tile.y;
+  it.rows = tile.z;
+  it.kb = (it.s * a.kt_total) / a.splits;
+  it.ke = ((it.s + 1) * a.kt_total) / a.splits;
+  return it;
+}
+
+// silu(g) * u.  expf and a correctly rounded division: the hidden rows are quantised next, which turns an error of d counts
+// into a wrong code with probability d, so nothing is gained with fewer bits here.
+__device__ __forceinline__ float gated(float g, float u) { return __fmul_rn(__fdiv_rn(g, 1.0f + expf(-g)), u); }
+
+// Sixteen rows of one channel (see OutMode).  `full`: all 128 channels of the block exist.
+__device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c0, const int (&v)[16], int n, bool n_ok, float w_scale) {
+  const int lane = threadIdx.x & 31;
+  const int valid = it.rows - c0;
+  const long p0 = (long)it.row0 + c0;
+  if (a.out_mode == kOutPlanes) {
+    if (n_ok) {
+      int32_t* o = static_cast<int32_t*>(a.out) + ((size_t)it.s * a.rows + p0) * a.N + n;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < valid) o[(size_t)j * a.N] = v[j];
+    }
+    return;
+  }
+  // lane j < 16 fetches the scale (and the destination) of row j; the others get them by shuffle
+  const float my_scale = lane < 16 && lane < valid ? a.ascale[p0 + lane] : 0.f;
+  if (a.out_mode == kOutPairs) {
+    const int my_pair = lane < 16 && lane < valid ? a.pair_of_pos[p0 + lane] : 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float sc = __shfl_sync(0xffffffffu, my_scale, j);
+      const int pair = __shfl_sync(0xffffffffu, my_pair, j);
+      if (n_ok && j < valid) store_out(a.out, (size_t)pair * a.N + n, lqq_scale(v[j], sc, w_scale), a.out_dtype);
+    }
+    return;
+  }
+  // Gated: an even lane holds the gate and the odd one beside it the up value of the same hidden channel.  The even lane
+  // takes rows 0..7 and the odd one rows 8..15, each handing over what the other needs.
+  const bool odd = lane & 1;
+  float h[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float lo = lqq_scale(v[j], __shfl_sync(0xffffffffu, my_scale, j), w_scale);
+    const float hi = lqq_scale(v[j + 8], __shfl_sync(0xffffffffu, my_scale, j + 8), w_scale);
+    const float other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
+    h[j] = odd ? gated(other, hi) : gated(lo, other);
+  }
+  const int first = odd ? 8 : 0;
+  float* o = static_cast<float*>(a.out) + (size_t)(p0 + first) * (a.N / 2) + (n >> 1);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (first + j < valid) o[(size_t)j * (a.N / 2)] = h[j];
+  // the rows' largest magnitudes over the warp's 16 hidden channels: after three halving steps every lane holds one row
+  float m[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m[j] = fabsf(h[j]);
+#pragma unroll
+  for (int w = 4; w >= 1; w >>= 1) {
+    const bool up = lane & (2 * (4 / w));   // lane bits 1, 2, 3
+#pragma unroll
+    for (int j = 0; j < w; ++j) {
+      const float keep = up ? m[j + w] : m[j], give = up ? m[j] : m[j + w];
+      m[j] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, 2 * (4 / w)));
+    }
+  }
+  m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], 16));
+  const int row = first + ((lane & 2) ? 4 : 0) + ((lane & 4) ? 2 : 0) + ((lane & 8) ? 1 : 0);
+  // magnitudes compare like their bits; the order of the atomics does not matter to a maximum
+  if (lane < 16 && row < valid) atomicMax(a.amax + p0 + row, __float_as_uint(m[0]));
+}
+
+template <int BN, int NS, bool W4>
+__global__ void __launch_bounds__(kThreads, 2)
+experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Args args) {
+  using C = Cfg<BN, NS, W4>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+
+  const uint32_t xs = base;                                   // NS row stages (1024-aligned, 128-byte swizzle)
+  const uint32_t ws = xs + NS * C::kXStage;                   // NS weight stages (1024-aligned for INT8: swizzled too)
+  const uint32_t bars = ws + NS * C::kWStage;
+  const uint32_t bar_full = bars;                             // [NS] copies landed
+  const uint32_t bar_empty = bar_full + NS * 8;               // [NS] stage may be overwritten
+  const uint32_t bar_aready = bar_empty + NS * 8;             // [kNT] operand in tensor memory
+  const uint32_t bar_afree = bar_aready + kNT * 8;            // [kNT] MMAs that read the operand are done
+  const uint32_t bar_accfull = bar_afree + kNT * 8;           // [kAcc] sums final
+  const uint32_t bar_accfree = bar_accfull + C::kAcc * 8;     // [kAcc] sums read out
+  const uint32_t tmem_slot = bar_accfree + C::kAcc * 8;
+  volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, W4 ? 129 : 1);
+    }
+    for (int t = 0; t < kNT; ++t) {
+      ptx::mbar_init(bar_aready + 8 * t, 128);
+      ptx::mbar_init(bar_afree + 8 * t, 1);
+    }
+    for (int b = 0; b < C::kAcc; ++b) {
+      ptx::mbar_init(bar_accfull + 8 * b, 1);
+      ptx::mbar_init(bar_accfree + 8 * b, 4 * kSets);   // one arrival per epilogue warp
+    }
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmap_x);
+    if (!W4) ptx::prefetch_tensormap(&tmap_w);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, C::kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  allow_dependents();
+  dependency_wait();   // the plan, the rows and the buffers written here belong to earlier kernels until now
+  const uint32_t tmem_acc = *tmem_slot_p;
+  const uint32_t tmem_a = tmem_acc + C::kAcc * BN;
+  const int items = __ldcg(args.counts) * args.n_tiles * args.splits;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ copies
+    if (lane == 0) {
+      Ring<NS> ring;
+      int issued = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+        const Item it = item_at(args, i);
+        const int boxes = (it.rows + C::kBox - 1) / C::kBox;
+        const uint32_t tx = (uint32_t)(boxes * C::kBox * 128 + C::kWStage);
+        const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;
+        const int wrow = W4 ? 0 : it.expert * args.N + it.nt * 128;
+        for (int kt = it.kb; kt < it.ke; ++kt) {
+          if (!ptx::mbar_wait_bounded(bar_empty + 8 * ring.s, ring.ph ^ 1u, kWaitLimitNs)) {
+            atomicExch(args.status, 161);
+            ok = false;
+            break;
+          }
+          const uint32_t full = bar_full + 8 * ring.s;
+          ptx::mbar_expect_tx(full, tx);
+          if (W4) {
+            ptx::bulk_load(ws + ring.s * C::kWStage, src, kBlobTile, full);
+            src += kBlobTile;
+          } else {
+            ptx::tensor_load_2d(ws + ring.s * C::kWStage, &tmap_w, kt * 128, wrow, full);
+          }
+          for (int b = 0; b < boxes; ++b)
+            ptx::tensor_load_2d(xs + ring.s * C::kXStage + b * C::kBox * 128, &tmap_x, kt * 128, it.row0 + b * C::kBox, full);
+          ring.advance();
+          ++issued;
+        }
+      }
+      if (!ok) {
+        // copies already issued still write shared memory: let them land before the CTA exits
+        for (int q = issued > NS ? issued - NS : 0; q < issued; ++q)
+          ptx::mbar_wait_bounded(bar_full + 8 * (q % NS), (uint32_t)(q / NS) & 1u, kWaitLimitNs);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issue
+    // The whole warp walks the loop; one elected lane issues (see ptx::elect_one).
+    const bool leader = ptx::elect_one();
+    Ring<NS> ring;
+    Ring<kNT> tring;
+    Ring<C::kAcc> accring;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      const Item it = item_at(args, i);
+      const uint32_t idesc = ptx::idesc_i8((it.rows + C::kBox - 1) / C::kBox * C::kBox);
+      ok = ptx::mbar_wait_bounded(bar_accfree + 8 * accring.s, accring.ph ^ 1u, kWaitLimitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (leader) atomicExch(args.status, 162);
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t acc = tmem_acc + accring.s * BN;
+      for (int kt = it.kb; kt < it.ke; ++kt) {
+        ok = ptx::mbar_wait_bounded(bar_full + 8 * ring.s, ring.ph, kWaitLimitNs);
+        if (ok && W4) ok = ptx::mbar_wait_bounded(bar_aready + 8 * tring.s, tring.ph, kWaitLimitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (leader) atomicExch(args.status, 163);
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t xb = xs + ring.s * C::kXStage;
+        const uint32_t wb = ws + ring.s * C::kWStage;
+        const uint32_t ab = tmem_a + tring.s * 32;
+        if (leader) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint64_t bdesc = ptx::smem_desc_sw128(xb + j * 32);
+            const uint32_t accumulate = (kt > it.kb || j > 0) ? 1u : 0u;
+            if (W4) ptx::mma_i8_ts(acc, ab + j * 8, bdesc, idesc, accumulate);
+            else ptx::mma_i8_ss(acc, ptx::smem_desc_sw128(wb + j * 32), bdesc, idesc, accumulate);
+          }
+          ptx::tc_commit(bar_empty + 8 * ring.s);
+          if (W4) ptx::tc_commit(bar_afree + 8 * tring.s);
+        }
+        ring.advance();
+        tring.advance();
+      }
+      if (ok && leader) ptx::tc_commit(bar_accfull + 8 * accring.s);
+      accring.advance();
+    }
+  } else {
+    // ------------------------------------------------------------------ unpacking and epilogue
+    const int quad = warp & 3;               // TMEM lane quadrant this warp may access
+    const int row = quad * 32 + lane;        // channel inside the block == TMEM lane
+    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+    const int set = (threadIdx.x - 64) >> 7;
+    Ring<NS> ring;
+    Ring<kNT> tring;
+    Ring<C::kAcc> accring;
+    int turn = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      const Item it = item_at(args, i);
+      if (W4) {
+        for (int kt = it.kb; kt < it.ke; ++kt) {
+          const bool mine = turn == set;
+          turn ^= 1;
+          if (!mine) {
+            ring.advance();
+            tring.advance();
+            continue;
+          }
+          if (!ptx::mbar_wait_bounded(bar_full + 8 * ring.s, ring.ph, kWaitLimitNs)) {
+            atomicExch(args.status, 164);
+            ok = false;
+            break;
+          }
+          const uint8_t* wst = smem + (ws - base) + ring.s * C::kWStage;
+          uint4 ch[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ch[c] = *reinterpret_cast<const uint4*>(wst + (c * 128 + row) * 16);
+          const uint32_t meta = *reinterpret_cast<const uint32_t*>(wst + 8192 + row * 4);
+          ptx::mbar_arrive(bar_empty + 8 * ring.s);
+          const uint32_t step0 = meta & 0xffu, a0 = ((meta >> 8) & 0xffu) * 0x01010101u;
+          const uint32_t step1 = (meta >> 16) & 0xffu, a1 = (meta >> 24) * 0x01010101u;
+          uint32_t v[4][8];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t step = c < 2 ? step0 : step1;
+            const uint32_t ab = c < 2 ? a0 : a1;
+            const uint32_t pk[4] = {ch[c].x, ch[c].y, ch[c].z, ch[c].w};
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              v[c][2 * h] = lqq_dequant4(pk[h] & 0x0F0F0F0Fu, step, ab);
+              v[c][2 * h + 1] = lqq_dequant4((pk[h] >> 4) & 0x0F0F0F0Fu, step, ab);
+            }
+          }
+          if (!ptx::mbar_wait_bounded(bar_afree + 8 * tring.s, tring.ph ^ 1u, kWaitLimitNs)) {
+            atomicExch(args.status, 165);
+            ok = false;
+            break;
+          }
+          __syncwarp();   // lanes leave the poll loops one by one; tcgen05.st / wait::st need the warp converged
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ptx::tmem_st8(tmem_a + lane_addr + tring.s * 32 + c * 8, v[c]);
+          ptx::tc_wait_st();
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(bar_aready + 8 * tring.s);
+          ring.advance();
+          tring.advance();
+        }
+        if (!ok) break;
+      }
+      if (!ptx::mbar_wait_bounded(bar_accfull + 8 * accring.s, accring.ph, kWaitLimitNs)) {
+        atomicExch(args.status, 166);
+        ok = false;
+      }
+      // the warp reads tensor memory and shuffles as one: it goes on as one or not at all
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const int n = it.nt * 128 + row;
+      const bool n_ok = n < args.N;
+      const float w_scale = n_ok && args.out_mode != kOutPlanes ? args.s1[(size_t)it.expert * args.N + n] : 0.f;
+      const uint32_t acc = tmem_acc + accring.s * BN + lane_addr;
+#pragma unroll 1
+      for (int c0 = 16 * set; c0 < it.rows; c0 += 16 * kSets) {
+        int v[16];
+        ptx::tmem_ld16(acc + c0, v);
+        ptx::tc_wait_ld();
+        store_chunk(args, it, c0, v, n, n_ok, w_scale);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_accfree + 8 * accring.s);
+      accring.advance();
+    }
+  }
+
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_acc, C::kTmemCols);
+  }
+}
+
+template <int BN, int NS, bool W4>
+static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
+  using C = Cfg<BN, NS, W4>;
+  auto kern = &experts_kernel<BN, NS, W4>;
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t attr_err = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() {
+    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  });
+  if (attr_err != cudaSuccess) {
+    record_cuda_error(attr_err, "cudaFuncSetAttribute(experts_kernel)");
+    return LQ_ERR_CUDA;
+  }
+  CUtensorMap tx, tw;
+  if (int rc = make_byte_matrix_map(&tx, p.x, p.rows, p.K, C::kBox, 128)) return rc;
+  if (W4) tw = tx;
+  else if (int rc = make_byte_matrix_map(&tw, p.w, (long)p.E * p.N, p.K, 128, 128)) return rc;
+  Args a;
+  a.blob = static_cast<const uint8_t*>(p.w);
+  a.s1 = p.s1;
+  a.ascale = p.ascale;
+  a.counts = plan.counts;
+  a.tiles = plan.tiles;
+  a.pair_of_pos = plan.pair_of_pos;
+  a.out = p.out;
+  a.amax = p.amax;
+  a.status = status_word();
+  a.rows = p.rows;
+  a.out_mode = p.out_mode;
+  a.out_dtype = p.out_dtype;
+  a.N = p.N;
+  a.kt_total = p.K / 128;
+  a.n_tiles = (p.N + 127) / 128;
+  a.splits = p.splits;
+  if (!a.status) return LQ_ERR_CUDA;
+  const long items = max_tiles(p.rows, p.E, plan.bn) * a.n_tiles * a.splits;
+  const long slots = 2L * sm_count();
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(kThreads),
+                                          (size_t)C::kSmemBytes, st, tx, tw, a);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "experts_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("experts_kernel");
+}
+
+int run_product(const Product& p, const Plan& plan, cudaStream_t st) {
+  if (p.w_kind == kBlob) {
+    switch (plan.bn) {
+      case 32: return launch_product<32, 8, true>(p, plan, st);
+      case 64: return launch_product<64, 6, true>(p, plan, st);
+      default: return launch_product<128, 4, true>(p, plan, st);
+    }
+  }
+  switch (plan.bn) {
+    case 32: return launch_product<32, 5, false>(p, plan, st);
+    case 64: return launch_product<64, 4, false>(p, plan, st);
+    default: return launch_product<128, 3, false>(p, plan, st);
+  }
+}
+
+}  // namespace experts
+}  // namespace lq

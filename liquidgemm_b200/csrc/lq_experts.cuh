@@ -1,0 +1,56 @@
+// What the kernels of the mixture-of-experts path share: the plan that sorts (token, expert) pairs by expert, and the
+// grouped product over it.
+#pragma once
+
+#include <stdint.h>
+
+#include "lq_common.cuh"
+
+namespace lq {
+namespace experts {
+
+constexpr int kMaxExperts = 512;
+constexpr int kMaxTopk = 32;
+
+// Weights of a grouped product: tile blobs of the 4-bit weights, one behind the other, or INT8 rows [E * N, K].
+enum WeightKind { kBlob = 0, kInt8 = 1 };
+
+// A stable counting sort of the T * topk pairs by expert: pair i (token i / topk) gets row pos_of_pair[i] of the sorted
+// activations, the pair at row p is pair_of_pos[p].  Pairs whose id is no expert get no row (-1).  The rows of an expert
+// are cut into tiles of at most `bn` rows; tiles[i] = (expert, first row, rows, 0).
+struct Plan {
+  int* counts;        // [4]: tiles, rows
+  int4* tiles;        // [max_tiles]
+  int* pos_of_pair;   // [pairs]
+  int* pair_of_pos;   // [pairs]
+  int bn;
+};
+inline long max_tiles(long pairs, int E, int bn) {
+  const long by_rows = pairs / bn + E;
+  return by_rows < pairs ? by_rows : pairs;
+}
+
+// Outputs of a grouped product, for the sorted row p and output channel n of its expert:
+enum OutMode {
+  kOutPlanes = 0,   // int32 sums out[s][p][n] of k-range s
+  kOutPairs = 1,    // scaled, in `out_dtype`, out[pair_of_pos[p]][n]
+  kOutGated = 2     // channels 2c, 2c + 1 = gate, up of hidden channel c: out[p][c] = silu(gate) * up in float32, and the
+                    // largest magnitude of each row as the bits of a float in amax[p] (zero before)
+};
+struct Product {
+  const void* w;
+  int w_kind;
+  const float* s1;         // [E, N]
+  const int8_t* x;         // [rows, K], sorted
+  const float* ascale;     // [rows]
+  long rows;               // rows of `x`: at least as many as the plan has
+  int E, N, K;
+  int splits;              // k-ranges (kOutPlanes; 1 otherwise)
+  int out_mode, out_dtype;
+  void* out;
+  unsigned* amax;
+};
+int run_product(const Product& p, const Plan& plan, cudaStream_t st);   // lq_experts.cu
+
+}  // namespace experts
+}  // namespace lq

@@ -1,0 +1,928 @@
+// Mixture-of-experts layer: the router, the plan that sorts (token, expert) pairs by expert, and what stands around the
+// grouped products (lq_experts.cu): quantising the rows into their sorted places, the gated activation's quantiser and
+// the weighted sum over a token's experts.
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "lq_experts.cuh"
+
+namespace lq {
+namespace experts {
+
+// ---------------------------------------------------------------------------------------------
+// router
+// ---------------------------------------------------------------------------------------------
+// One warp per token, expert e = lane + 32 i in register i of its lane.  Score s = softmax(l) over the token's experts or
+// sigmoid(l).  Key: the logit itself without a bias (scores rise with it, and it is exact), else s + bias.  Groups of E / G
+// neighbouring experts are ranked by their largest key or by the sum of their two largest keys (without a bias: scores), and
+// only experts of the best groups stay.  Then `topk` times the largest key, the lowest index among equals.
+// Where scores decide what is chosen (keys with a bias, sums of two) they are worked out in float64: neighbouring keys may
+// lie closer than a float32 exponential's error, and a choice is a whole number.  The part has a float64 rate of half its
+// float32 rate, and the kernel is bound by its shuffles and reductions all the same.
+// A logit of -inf or NaN, or a bias that makes a key so, takes its expert out.
+
+// Orders numbers like unsigned integers; every number's image is above 0, which stands for "not to be chosen".
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);   // -0 becomes 0: equal keys are equal bits
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long ordered(double v) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+  return u ^ ((u >> 63) ? 0xffffffffffffffffull : 0x8000000000000000ull);
+}
+__device__ __forceinline__ double from_ordered(unsigned long long k) {
+  return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : 0xffffffffffffffffull)));
+}
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return ((unsigned long long)hi << 32) | lo;
+}
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;
+  float* weights;
+  int* ids;
+  int T, E, topk, n_group, topk_group;
+  float scale;
+  bool sigmoid, top2, renormalize;
+};
+
+template <typename Key> struct KeyOf;
+template <> struct KeyOf<float> { using type = uint32_t; };
+template <> struct KeyOf<double> { using type = unsigned long long; };
+
+// S: the type of the scores (and with a bias of the keys).
+template <typename T, int PER, typename S>
+__global__ void __launch_bounds__(128)
+route_kernel(const RouteArgs a) {
+  using Key = typename KeyOf<S>::type;
+  allow_dependents();
+  dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const long t = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  const T* row = static_cast<const T*>(a.logits) + t * a.E;
+  const float none = -INFINITY;
+  float l[PER];
+  float top = none;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    l[i] = e < a.E ? to_f32<T>(row[e]) : none;
+    if (!(l[i] > none)) l[i] = none;   // NaN too
+    top = fmaxf(top, l[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+
+  S s[PER];
+  S sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool can = l[i] > none;
+    if (a.sigmoid) {
+      s[i] = can ? (S)1 / ((S)1 + exp(-(S)l[i])) : (S)0;
+    } else {
+      s[i] = !can ? (S)0 : l[i] == top ? (S)1 : exp((S)l[i] - (S)top);   // (equal to the largest: also where that is infinite)
+      sum += s[i];
+    }
+  }
+  if (!a.sigmoid) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const S d = sum > 0 ? sum : (S)1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = s[i] / d;
+  }
+
+  const bool by_score = a.bias != nullptr;
+  Key key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = 0;
+    if (l[i] > none) {
+      const S v = by_score ? s[i] + (S)a.bias[e] : (S)l[i];
+      if (v > (S)none) key[i] = ordered(v);
+    }
+  }
+
+  if (a.n_group > 1) {
+    // lane g (and, above 32 groups, its further registers) keeps the rank key of group g
+    const int size = a.E / a.n_group;
+    Key rank[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) rank[i] = 0;
+    for (int g = 0; g < a.n_group; ++g) {
+      const int first = g * size, last = first + size;
+      Key best = 0;
+      Key mine = 0;
+      int at = -1;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = lane + 32 * i;
+        if (e >= first && e < last && key[i] > mine) mine = key[i], at = i;
+      }
+      best = warp_max(mine);
+      if (a.top2 && best != 0) {
+        // by_score: the keys' sum; else the scores of the two experts with the largest keys
+        const unsigned owner = __ballot_sync(0xffffffffu, mine == best && at >= 0);
+        const int first_lane = __ffs(owner) - 1;
+        Key second = 0;
+        int at2 = -1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int e = lane + 32 * i;
+          if (e >= first && e < last && key[i] > second && !(lane == first_lane && i == at)) second = key[i], at2 = i;
+        }
+        const Key next = warp_max(second);
+        const unsigned owner2 = __ballot_sync(0xffffffffu, second == next && at2 >= 0);
+        S v1 = 0, v2 = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const S v = by_score ? s[i] + (S)a.bias[min(lane + 32 * i, a.E - 1)] : s[i];
+          if (i == at) v1 = v;
+          if (i == at2) v2 = v;
+        }
+        v1 = __shfl_sync(0xffffffffu, v1, first_lane);
+        v2 = __shfl_sync(0xffffffffu, v2, owner2 ? __ffs(owner2) - 1 : 0);
+        best = ordered(owner2 ? v1 + v2 : v1);
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (g == lane + 32 * i) rank[i] = best;
+    }
+    unsigned kept[PER];   // bit of lane: group lane + 32 i stays
+#pragma unroll
+    for (int i = 0; i < PER; ++i) kept[i] = 0;
+    for (int q = 0; q < a.topk_group; ++q) {
+      Key mine = 0;
+      int g = 1 << 20;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (rank[i] > mine) mine = rank[i], g = lane + 32 * i;
+      const Key best = warp_max(mine);
+      if (best == 0) break;   // no group with an expert is left
+      const int win = (int)__reduce_min_sync(0xffffffffu, mine == best ? (unsigned)g : 1u << 20);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (win >> 5 == i) kept[i] |= 1u << (win & 31);
+        if (win == lane + 32 * i) rank[i] = 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int g = (lane + 32 * i) / size;
+      unsigned word = 0;
+#pragma unroll
+      for (int w = 0; w < PER; ++w)
+        if (g >> 5 == w) word = kept[w];
+      if (!((word >> (g & 31)) & 1u)) key[i] = 0;
+    }
+  }
+
+  // lane j ends up with choice j
+  int my_id = -1;
+  S my_w = 0;
+  for (int j = 0; j < a.topk; ++j) {
+    Key mine = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > mine) mine = key[i], at = i;
+    const Key best = warp_max(mine);
+    if (best == 0) break;
+    const int win = (int)__reduce_min_sync(0xffffffffu, mine == best ? (unsigned)(lane + 32 * at) : 1u << 20);
+    S w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (win == lane + 32 * i) {
+        key[i] = 0;
+        w = s[i];
+      }
+    }
+    w = __shfl_sync(0xffffffffu, w, win & 31);
+    if (lane == j) my_id = win, my_w = w;
+  }
+  if (a.renormalize) {
+    S total = my_w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (total > 0) my_w = my_w / total;
+  }
+  if (lane < a.topk) {
+    a.weights[t * a.topk + lane] = (float)(my_w * (S)a.scale);
+    a.ids[t * a.topk + lane] = my_id;
+  }
+}
+
+template <typename T, typename S>
+static int launch_route(const RouteArgs& a, cudaStream_t st) {
+  const int per = (a.E + 31) / 32;
+  void (*kern)(RouteArgs) = per <= 1   ? route_kernel<T, 1, S>
+                            : per <= 2 ? route_kernel<T, 2, S>
+                            : per <= 4 ? route_kernel<T, 4, S>
+                            : per <= 8 ? route_kernel<T, 8, S>
+                                       : route_kernel<T, 16, S>;
+  const cudaError_t e = launch_overlapped(kern, dim3((a.T + 3) / 4), dim3(128), 0, st, a);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "route_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("route_kernel");
+}
+
+// ---------------------------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------------------------
+// One CTA of 32 warps.  Warp w counts the pairs of its contiguous share per expert, the counts are summed over warps and
+// experts, and in a second pass every pair's row is the running count of its (warp, expert): a stable sort, the same
+// on every run.
+constexpr int kPlanWarps = 32;
+__global__ void __launch_bounds__(32 * kPlanWarps)
+plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
+  extern __shared__ int hist[];   // [kPlanWarps][E]
+  __shared__ int sums[2][kPlanWarps];
+  allow_dependents();
+  dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kPlanWarps * E; i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  const long share = ((pairs + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
+  const long begin = warp * share, end = begin + share < pairs ? begin + share : pairs;
+  for (long i = begin + lane; i < end; i += 32) {
+    const int e = ids[i];
+    if (e >= 0 && e < E) atomicAdd(&hist[warp * E + e], 1);
+  }
+  __syncthreads();
+  // thread e: the pairs of expert e, and how many of them lie before each warp's share
+  const int e = threadIdx.x;
+  int n = 0, tiles = 0;
+  if (e < E) {
+    for (int w = 0; w < kPlanWarps; ++w) {
+      const int c = hist[w * E + e];
+      hist[w * E + e] = n;
+      n += c;
+    }
+    tiles = (n + plan.bn - 1) / plan.bn;
+  }
+  // exclusive sums over the experts of both counts
+  int a = n, b = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int pa = __shfl_up_sync(0xffffffffu, a, o), pb = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += pa, b += pb;
+  }
+  if (lane == 31) sums[0][warp] = a, sums[1][warp] = b;
+  __syncthreads();
+  int ra = 0, rb = 0;
+  for (int w = 0; w < warp; ++w) ra += sums[0][w], rb += sums[1][w];
+  const int row0 = ra + a - n, tile0 = rb + b - tiles;
+  if (e < E) {
+    for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] += row0;
+    for (int i = 0; i < tiles; ++i) {
+      const int left = n - i * plan.bn;
+      plan.tiles[tile0 + i] = make_int4(e, row0 + i * plan.bn, left < plan.bn ? left : plan.bn, 0);
+    }
+  }
+  if (threadIdx.x == blockDim.x - 1) {
+    plan.counts[0] = rb + b;
+    plan.counts[1] = ra + a;
+  }
+  __syncthreads();
+  for (long i0 = begin; i0 < end; i0 += 32) {
+    const long i = i0 + lane;
+    int e2 = i < end ? ids[i] : -1;
+    if (e2 < 0 || e2 >= E) e2 = -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e2);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    int base = 0;
+    if (e2 >= 0) base = hist[warp * E + e2];
+    __syncwarp();
+    if (e2 >= 0 && before == 0) hist[warp * E + e2] = base + __popc(same);
+    __syncwarp();
+    if (i < end) {
+      plan.pos_of_pair[i] = e2 >= 0 ? base + before : -1;
+      if (e2 >= 0) plan.pair_of_pos[base + before] = (int)i;
+    }
+  }
+}
+
+static int run_plan(const int* ids, long pairs, int E, const Plan& plan, cudaStream_t st) {
+  const size_t smem = (size_t)kPlanWarps * E * sizeof(int);
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::call_once(once[dev & 63], [&]() {
+    cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanWarps * kMaxExperts * (int)sizeof(int));
+  });
+  const cudaError_t e = launch_overlapped(plan_kernel, dim3(1), dim3(32 * kPlanWarps), smem, st, ids, pairs, E, plan);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "plan_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("plan_kernel");
+}
+
+// ---------------------------------------------------------------------------------------------
+// rows into their sorted places
+// ---------------------------------------------------------------------------------------------
+// One CTA per row of x (one per token, or one per pair): quantised as by quant_row_kernel of the dense linear, bit for bit,
+// and written to the places of its pairs.  NV 16-byte vectors per thread in registers; NV = 0: a row too long for that is read
+// twice.  Where the outputs are one row per pair, the rows of pairs without an expert are set to zero here.
+struct PlaceArgs {
+  const void* x;
+  const float* x_scale;    // scales of INT8 rows
+  int8_t* xq;
+  float* ascale;
+  const int* pos_of_pair;
+  unsigned* amax;          // set to zero for the rows placed, or null
+  void* y;                 // [pairs, N] whose rows without an expert are cleared, or null
+  int y_size;              // bytes of an element of y
+  int per_row;             // pairs of a row of x
+  int K, N;
+};
+
+__device__ __forceinline__ void clear_output_row(const PlaceArgs& a, long pair) {
+  if (a.y_size == 2) {
+    uint16_t* y = static_cast<uint16_t*>(a.y) + pair * a.N;
+    for (int n = threadIdx.x; n < a.N; n += blockDim.x) y[n] = 0;
+  } else {
+    uint32_t* y = static_cast<uint32_t*>(a.y) + pair * a.N;
+    for (int n = threadIdx.x; n < a.N; n += blockDim.x) y[n] = 0;
+  }
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024)
+place_rows_kernel(const PlaceArgs a) {
+  __shared__ float red[32];
+  constexpr int VEC = 16 / sizeof(T);
+  allow_dependents();
+  dependency_wait();
+  const long m = blockIdx.x;
+  const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + m * a.K);
+  const int nvec = a.K / VEC;
+  uint4 raw[NV > 0 ? NV : 1];
+  RowMax<T> rm;
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      raw[i] = v < nvec ? xr[v] : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) rm.take(raw[i]);
+  } else {
+    for (int v = threadIdx.x; v < nvec; v += blockDim.x) rm.take(xr[v]);
+  }
+  const float amax = block_max(rm.value(), red);
+  const float scale = __fdiv_rn(fmaxf(amax, 1e-12f), 127.0f);
+  const float inv = __fdiv_rn(1.0f, scale);
+  for (int j = 0; j < a.per_row; ++j) {
+    const long pair = m * a.per_row + j;
+    const int p = a.pos_of_pair[pair];
+    if (p < 0) {
+      if (a.y) clear_output_row(a, pair);
+      continue;
+    }
+    if (threadIdx.x == 0) {
+      a.ascale[p] = scale;
+      if (a.amax) a.amax[p] = 0u;
+    }
+    int8_t* qr = a.xq + (long)p * a.K;
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v >= nvec) break;
+        uint32_t out[4 / sizeof(T)];
+        quant_vec<T>(raw[i], scale, inv, out);
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(qr)[v] = out[0];
+        else reinterpret_cast<uint2*>(qr)[v] = make_uint2(out[0], out[1]);
+      }
+    } else {
+      for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+        uint32_t out[4 / sizeof(T)];
+        quant_vec<T>(xr[v], scale, inv, out);
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(qr)[v] = out[0];
+        else reinterpret_cast<uint2*>(qr)[v] = make_uint2(out[0], out[1]);
+      }
+    }
+  }
+}
+
+// Rows that come in INT8 with their scales.
+__global__ void __launch_bounds__(256)
+place_i8_kernel(const PlaceArgs a) {
+  allow_dependents();
+  dependency_wait();
+  const long m = blockIdx.x;
+  const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const int8_t*>(a.x) + m * a.K);
+  const float scale = a.x_scale[m];
+  for (int j = 0; j < a.per_row; ++j) {
+    const long pair = m * a.per_row + j;
+    const int p = a.pos_of_pair[pair];
+    if (p < 0) {
+      if (a.y) clear_output_row(a, pair);
+      continue;
+    }
+    if (threadIdx.x == 0) a.ascale[p] = scale;
+    uint4* qr = reinterpret_cast<uint4*>(a.xq + (long)p * a.K);
+    for (int v = threadIdx.x; v < a.K / 16; v += blockDim.x) qr[v] = xr[v];
+  }
+}
+
+template <typename T>
+static int launch_place(const PlaceArgs& a, long rows, cudaStream_t st) {
+  int threads = 0;
+  const int nv = row_units_per_thread(rows, a.K / (16 / (int)sizeof(T)), 8, 128, 1024, &threads);
+  void (*kern)(PlaceArgs) = nv == 1   ? place_rows_kernel<T, 1>
+                            : nv == 2 ? place_rows_kernel<T, 2>
+                            : nv == 4 ? place_rows_kernel<T, 4>
+                            : nv == 8 ? place_rows_kernel<T, 8>
+                                      : place_rows_kernel<T, 0>;
+  if (nv == 0) threads = 1024;
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)rows), dim3(threads), 0, st, a);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "place_rows_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("place_rows_kernel");
+}
+
+static int run_place(const PlaceArgs& a, int x_dtype, long rows, cudaStream_t st) {
+  if (x_dtype == LQ_DT_BF16) return launch_place<__nv_bfloat16>(a, rows, st);
+  if (x_dtype == LQ_DT_F16) return launch_place<__half>(a, rows, st);
+  if (x_dtype == LQ_DT_F32) return launch_place<float>(a, rows, st);
+  const cudaError_t e = launch_overlapped(place_i8_kernel, dim3((unsigned)rows), dim3(256), 0, st, a);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "place_i8_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("place_i8_kernel");
+}
+
+// ---------------------------------------------------------------------------------------------
+// hidden rows: activation (where the product left its sums) and quantisation
+// ---------------------------------------------------------------------------------------------
+struct HiddenArgs {
+  const int32_t* planes;     // [splits][rows][2 * I] sums of the gate and up channels, interleaved; or null
+  const float* h;            // [rows][I] hidden values, with amax
+  const unsigned* amax;
+  const float* ascale;       // [rows] scales of the product's rows
+  const float* s1;           // [E][2 * I]
+  const int* ids;            // [pairs]
+  const int* counts;
+  const int* pair_of_pos;
+  int8_t* hq;                // [rows][I]
+  float* hscale;             // [rows]
+  long rows;
+  int I, splits;
+};
+
+__device__ __forceinline__ float gated_hidden(float g, float u) { return __fmul_rn(__fdiv_rn(g, 1.0f + expf(-g)), u); }
+
+// Four hidden values of row p from the planes.
+__device__ __forceinline__ void hidden4(const HiddenArgs& a, long p, const float* s1, float as, int c, float (&h)[4]) {
+  int4 g0 = make_int4(0, 0, 0, 0), g1 = g0;
+  for (int s = 0; s < a.splits; ++s) {
+    const int4* src = reinterpret_cast<const int4*>(a.planes + ((size_t)s * a.rows + p) * 2 * a.I + 2 * c);
+    const int4 v0 = src[0], v1 = src[1];
+    g0.x += v0.x; g0.y += v0.y; g0.z += v0.z; g0.w += v0.w;
+    g1.x += v1.x; g1.y += v1.y; g1.z += v1.z; g1.w += v1.w;
+  }
+  const float4 f0 = *reinterpret_cast<const float4*>(s1 + 2 * c), f1 = *reinterpret_cast<const float4*>(s1 + 2 * c + 4);
+  h[0] = gated_hidden(lqq_scale(g0.x, as, f0.x), lqq_scale(g0.y, as, f0.y));
+  h[1] = gated_hidden(lqq_scale(g0.z, as, f0.z), lqq_scale(g0.w, as, f0.w));
+  h[2] = gated_hidden(lqq_scale(g1.x, as, f1.x), lqq_scale(g1.y, as, f1.y));
+  h[3] = gated_hidden(lqq_scale(g1.z, as, f1.z), lqq_scale(g1.w, as, f1.w));
+}
+
+__device__ __forceinline__ uint32_t quant4(const float (&h)[4], float scale, float inv) {
+  uint32_t out[1];
+  quant_vec<float>(make_uint4(__float_as_uint(h[0]), __float_as_uint(h[1]), __float_as_uint(h[2]), __float_as_uint(h[3])), scale,
+                   inv, out);
+  return out[0];
+}
+
+// One CTA per row: the largest magnitude first, then the codes; the row's values are worked out twice, from sums that the
+// second pass finds in L2.
+__global__ void __launch_bounds__(512)
+hidden_planes_kernel(const HiddenArgs a) {
+  __shared__ float red[32];
+  allow_dependents();
+  dependency_wait();
+  const long p = blockIdx.x;
+  if (p >= a.counts[1]) return;
+  const int e = a.ids[a.pair_of_pos[p]];
+  const float* s1 = a.s1 + (size_t)e * 2 * a.I;
+  const float as = a.ascale[p];
+  float m = 0.f;
+  for (int c = threadIdx.x * 4; c < a.I; c += blockDim.x * 4) {
+    float h[4];
+    hidden4(a, p, s1, as, c, h);
+    m = fmaxf(fmaxf(m, fmaxf(fabsf(h[0]), fabsf(h[1]))), fmaxf(fabsf(h[2]), fabsf(h[3])));
+  }
+  m = block_max(m, red);
+  const float scale = __fdiv_rn(fmaxf(m, 1e-12f), 127.0f);
+  const float inv = __fdiv_rn(1.0f, scale);
+  if (threadIdx.x == 0) a.hscale[p] = scale;
+  for (int c = threadIdx.x * 4; c < a.I; c += blockDim.x * 4) {
+    float h[4];
+    hidden4(a, p, s1, as, c, h);
+    *reinterpret_cast<uint32_t*>(a.hq + p * a.I + c) = quant4(h, scale, inv);
+  }
+}
+
+// The hidden values and their rows' maxima are there: codes only.
+__global__ void __launch_bounds__(256)
+hidden_quant_kernel(const HiddenArgs a) {
+  allow_dependents();
+  dependency_wait();
+  const long p = blockIdx.x;
+  if (p >= a.counts[1]) return;
+  const float scale = __fdiv_rn(fmaxf(__uint_as_float(a.amax[p]), 1e-12f), 127.0f);
+  const float inv = __fdiv_rn(1.0f, scale);
+  if (threadIdx.x == 0) a.hscale[p] = scale;
+  const uint4* src = reinterpret_cast<const uint4*>(a.h + p * a.I);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.hq + p * a.I);
+  for (int v = threadIdx.x; v < a.I / 4; v += blockDim.x) {
+    uint32_t out[1];
+    quant_vec<float>(ld_stream_v4(src + v), scale, inv, out);
+    dst[v] = out[0];
+  }
+}
+
+static int run_hidden(const HiddenArgs& a, cudaStream_t st) {
+  const cudaError_t e = a.planes ? launch_overlapped(hidden_planes_kernel, dim3((unsigned)a.rows), dim3(512), 0, st, a)
+                                 : launch_overlapped(hidden_quant_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "hidden rows launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("hidden rows");
+}
+
+// ---------------------------------------------------------------------------------------------
+// outputs from planes
+// ---------------------------------------------------------------------------------------------
+struct CombineArgs {
+  const int32_t* planes;     // [splits][rows][N]
+  const float* ascale;       // [rows]
+  const float* s1;           // [E][N]
+  const float* weights;      // [T][topk], or null: one output row per pair, unweighted
+  const int* ids;            // [T][topk]
+  const int* pos_of_pair;
+  void* y;                   // [T][N] or [T * topk][N]
+  long rows, outs;           // rows of a plane, rows of y
+  int N, topk, splits, out_dtype;
+};
+
+// A thread makes VEC neighbouring channels of one output row: y = sum_j weight_j * (sums * row scale * channel scale), the
+// experts of a token in the order of their slots, in float32, rounded once.
+template <int VEC>
+__global__ void __launch_bounds__(256)
+combine_kernel(const CombineArgs a) {
+  allow_dependents();
+  dependency_wait();
+  const int per = (a.N / VEC + blockDim.x - 1) / blockDim.x;
+  const long m = blockIdx.x / per;
+  const int c = ((int)(blockIdx.x - m * per) * blockDim.x + threadIdx.x) * VEC;
+  if (c >= a.N) return;
+  const int slots = a.weights ? a.topk : 1;
+  float sum[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+  for (int j = 0; j < slots; ++j) {
+    const long pair = m * slots + j;
+    const int p = a.pos_of_pair[pair];
+    if (p < 0) continue;
+    int v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = 0;
+    for (int s = 0; s < a.splits; ++s) {
+      const int32_t* src = a.planes + ((size_t)s * a.rows + p) * a.N + c;
+      if constexpr (VEC == 4) {
+        const int4 q = *reinterpret_cast<const int4*>(src);
+        v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+      } else {
+        v[0] += src[0];
+      }
+    }
+    const float as = a.ascale[p];
+    const float w = a.weights ? a.weights[pair] : 1.0f;
+    const float* s1 = a.s1 + (size_t)a.ids[pair] * a.N + c;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float o = lqq_scale(v[i], as, s1[i]);
+      sum[i] = a.weights ? __fmaf_rn(w, o, sum[i]) : o;
+    }
+  }
+  const size_t at = (size_t)m * a.N + c;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) store_out(a.y, at + i, sum[i], a.out_dtype);
+}
+
+static int run_combine(const CombineArgs& a, cudaStream_t st) {
+  const bool vec = a.N % 4 == 0;
+  const int per = ((vec ? a.N / 4 : a.N) + 255) / 256;
+  const cudaError_t e = vec ? launch_overlapped(combine_kernel<4>, dim3((unsigned)(a.outs * per)), dim3(256), 0, st, a)
+                            : launch_overlapped(combine_kernel<1>, dim3((unsigned)(a.outs * per)), dim3(256), 0, st, a);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "combine_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("combine_kernel");
+}
+
+// ---------------------------------------------------------------------------------------------
+// sizes
+// ---------------------------------------------------------------------------------------------
+// Rows of a tile: what an expert gets on average, with room for the uneven choice of a router.
+static int pick_bn(long pairs, int E) {
+  const long mean = pairs / E;
+  return mean <= 12 ? 32 : mean <= 40 ? 64 : 128;
+}
+
+// K-ranges of a product: only where the tiles of the experts that can be reached leave half of the CTA slots free, and with four
+// k-steps a range at least.
+static int pick_splits(long pairs, int E, int bn, int N, int K) {
+  const long reached = pairs < E ? pairs : E;
+  const long tiles = reached * ((pairs / reached + bn - 1) / bn) * ((N + 127) / 128);
+  const long slots = 2L * sm_count();
+  int S = (int)(slots / tiles);
+  if (S > K / 512) S = K / 512;
+  if (S > 16) S = 16;
+  return S < 1 ? 1 : S;
+}
+
+static size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+// Takes pieces off a scratch buffer (or, with a null buffer, only counts them).
+struct Carver {
+  uint8_t* base;
+  size_t used = 0;
+  explicit Carver(void* p) : base(static_cast<uint8_t*>(p)) {}
+  template <class T> T* take(size_t count) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += aligned(count * sizeof(T));
+    return p;
+  }
+};
+
+static Plan carve_plan(Carver& c, long pairs, int E) {
+  Plan p;
+  p.bn = pick_bn(pairs, E);
+  p.counts = c.take<int>(4);
+  p.tiles = c.take<int4>((size_t)max_tiles(pairs, E, p.bn));
+  p.pos_of_pair = c.take<int>((size_t)pairs);
+  p.pair_of_pos = c.take<int>((size_t)pairs);
+  return p;
+}
+
+struct LinearBuffers {
+  Plan plan;
+  int8_t* xq;
+  float* ascale;
+  int32_t* planes;
+  int splits;
+};
+static LinearBuffers carve_linear(Carver& c, long pairs, int E, int N, int K) {
+  LinearBuffers b;
+  b.plan = carve_plan(c, pairs, E);
+  b.splits = pick_splits(pairs, E, b.plan.bn, N, K);
+  b.xq = c.take<int8_t>((size_t)pairs * K);
+  b.ascale = c.take<float>((size_t)pairs);
+  b.planes = b.splits > 1 ? c.take<int32_t>((size_t)b.splits * pairs * N) : nullptr;
+  return b;
+}
+
+struct MlpBuffers {
+  Plan plan;
+  int8_t *xq, *hq;
+  float *ascale, *hscale, *h;
+  unsigned* amax;
+  int32_t *planes1, *planes2;
+  int splits1, splits2;
+};
+static MlpBuffers carve_mlp(Carver& c, long pairs, int E, int H, int I) {
+  MlpBuffers b;
+  b.plan = carve_plan(c, pairs, E);
+  b.splits1 = pick_splits(pairs, E, b.plan.bn, 2 * I, H);
+  b.splits2 = pick_splits(pairs, E, b.plan.bn, H, I);
+  b.xq = c.take<int8_t>((size_t)pairs * H);
+  b.ascale = c.take<float>((size_t)pairs);
+  b.hq = c.take<int8_t>((size_t)pairs * I);
+  b.hscale = c.take<float>((size_t)pairs);
+  b.planes1 = b.splits1 > 1 ? c.take<int32_t>((size_t)b.splits1 * pairs * 2 * I) : nullptr;
+  b.h = b.splits1 > 1 ? nullptr : c.take<float>((size_t)pairs * I);
+  b.amax = b.splits1 > 1 ? nullptr : c.take<unsigned>((size_t)pairs);
+  b.planes2 = c.take<int32_t>((size_t)b.splits2 * pairs * H);
+  return b;
+}
+
+// Sizes that every call has to have; `N` rows and `K` columns of an expert's matrix.
+static int check_sizes(long T, int topk, int E, int N, int K) {
+  if (T < 1 || topk < 1 || E < 1 || N < 1 || K < 1) return LQ_ERR_BAD_ARG;
+  if (topk > kMaxTopk || E > kMaxExperts || K % 128) return LQ_ERR_SHAPE;
+  if (T * topk > (1L << 24) || (long)E * ((N + 127) / 128 * 128) > 0x7fffffffL) return LQ_ERR_SHAPE;
+  return LQ_OK;
+}
+static bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+}  // namespace experts
+}  // namespace lq
+
+using namespace lq;
+using namespace lq::experts;
+
+extern "C" {
+
+int lq_moe_route(const void* logits, int logits_dtype, const float* bias, float* weights, int32_t* ids, int T, int E, int topk,
+                 int scoring, int n_group, int topk_group, int group_score, int renormalize, float scale, void* stream) {
+  if (!logits || !weights || !ids || T < 1 || E < 1 || topk < 1 || n_group < 1 || topk_group < 1) return LQ_ERR_BAD_ARG;
+  if (logits_dtype < 0 || logits_dtype > LQ_DT_F32 || scoring < 0 || scoring > 1 || group_score < 0 || group_score > 1)
+    return LQ_ERR_BAD_ARG;
+  if (E > kMaxExperts || topk > kMaxTopk || E % n_group || topk_group > n_group || topk > topk_group * (E / n_group))
+    return LQ_ERR_SHAPE;
+  RouteArgs a;
+  a.logits = logits;
+  a.bias = bias;
+  a.weights = weights;
+  a.ids = ids;
+  a.T = T;
+  a.E = E;
+  a.topk = topk;
+  a.n_group = topk_group == n_group ? 1 : n_group;   // every group stays: nothing to rank
+  a.topk_group = topk_group;
+  a.scale = scale;
+  a.sigmoid = scoring == 1;
+  a.top2 = group_score == 1;
+  a.renormalize = renormalize != 0;
+  // (sigmoid scores far below 1 would lose their ratio in float32's denormal range)
+  const bool wide = a.sigmoid || bias != nullptr || (a.n_group > 1 && a.top2);
+  cudaStream_t st = as_stream(stream);
+  if (logits_dtype == LQ_DT_BF16) return wide ? launch_route<__nv_bfloat16, double>(a, st) : launch_route<__nv_bfloat16, float>(a, st);
+  if (logits_dtype == LQ_DT_F16) return wide ? launch_route<__half, double>(a, st) : launch_route<__half, float>(a, st);
+  return wide ? launch_route<float, double>(a, st) : launch_route<float, float>(a, st);
+}
+
+size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K) {
+  if (check_sizes(T, topk, E, N, K)) return 0;
+  Carver c(nullptr);
+  carve_linear(c, (long)T * topk, E, N, K);
+  return c.used;
+}
+
+int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_per_pair, const int32_t* ids, const void* w,
+                      int w_kind, const float* s1, void* y, int out_dtype, int T, int topk, int E, int N, int K, void* scratch,
+                      size_t scratch_bytes, void* stream) {
+  if (!x || !ids || !w || !s1 || !y || x_dtype < 0 || x_dtype > 3 || (x_dtype == 3) != (x_scale != nullptr) || w_kind < 0 ||
+      w_kind > 1 || out_dtype < 0 || out_dtype > LQ_DT_F32)
+    return LQ_ERR_BAD_ARG;
+  if (int rc = check_sizes(T, topk, E, N, K)) return rc;
+  if (misaligned(x) || misaligned(w)) return LQ_ERR_SHAPE;
+  Carver c(scratch);
+  const long pairs = (long)T * topk;
+  const LinearBuffers b = carve_linear(c, pairs, E, N, K);
+  if (!scratch || scratch_bytes < c.used || misaligned(scratch)) return LQ_ERR_WORKSPACE;
+  cudaStream_t st = as_stream(stream);
+  if (int rc = run_plan(ids, pairs, E, b.plan, st)) return rc;
+  PlaceArgs pl = {};
+  pl.x = x;
+  pl.x_scale = x_scale;
+  pl.xq = b.xq;
+  pl.ascale = b.ascale;
+  pl.pos_of_pair = b.plan.pos_of_pair;
+  pl.y = b.planes ? nullptr : y;   // (from planes, the output pass writes every row)
+  pl.y_size = out_dtype == LQ_DT_F32 ? 4 : 2;
+  pl.per_row = x_per_pair ? 1 : topk;
+  pl.K = K;
+  pl.N = N;
+  if (int rc = run_place(pl, x_dtype, x_per_pair ? pairs : T, st)) return rc;
+  Product p = {};
+  p.w = w;
+  p.w_kind = w_kind;
+  p.s1 = s1;
+  p.x = b.xq;
+  p.ascale = b.ascale;
+  p.rows = pairs;
+  p.E = E;
+  p.N = N;
+  p.K = K;
+  p.splits = b.splits;
+  p.out_mode = b.planes ? kOutPlanes : kOutPairs;
+  p.out_dtype = out_dtype;
+  p.out = b.planes ? static_cast<void*>(b.planes) : y;
+  if (int rc = run_product(p, b.plan, st)) return rc;
+  if (!b.planes) return LQ_OK;
+  CombineArgs k = {};
+  k.planes = b.planes;
+  k.ascale = b.ascale;
+  k.s1 = s1;
+  k.ids = ids;
+  k.pos_of_pair = b.plan.pos_of_pair;
+  k.y = y;
+  k.rows = k.outs = pairs;
+  k.N = N;
+  k.topk = topk;
+  k.splits = b.splits;
+  k.out_dtype = out_dtype;
+  return run_combine(k, st);
+}
+
+size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I) {
+  if (check_sizes(T, topk, E, 2 * I, H) || check_sizes(T, topk, E, H, I)) return 0;
+  Carver c(nullptr);
+  carve_mlp(c, (long)T * topk, E, H, I);
+  return c.used;
+}
+
+int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32_t* ids, const void* w13, const float* s13,
+                   const void* w2, const float* s2, int w_kind, void* y, int out_dtype, int T, int topk, int E, int H, int I,
+                   void* scratch, size_t scratch_bytes, void* stream) {
+  if (!x || !weights || !ids || !w13 || !s13 || !w2 || !s2 || !y || x_dtype < 0 || x_dtype > LQ_DT_F32 || w_kind < 0 ||
+      w_kind > 1 || out_dtype < 0 || out_dtype > LQ_DT_F32)
+    return LQ_ERR_BAD_ARG;
+  if (I > (1 << 29)) return LQ_ERR_SHAPE;
+  if (int rc = check_sizes(T, topk, E, 2 * I, H)) return rc;
+  if (int rc = check_sizes(T, topk, E, H, I)) return rc;
+  if (misaligned(x) || misaligned(w13) || misaligned(w2) || misaligned(s13) || misaligned(s2)) return LQ_ERR_SHAPE;
+  Carver c(scratch);
+  const long pairs = (long)T * topk;
+  const MlpBuffers b = carve_mlp(c, pairs, E, H, I);
+  if (!scratch || scratch_bytes < c.used || misaligned(scratch)) return LQ_ERR_WORKSPACE;
+  cudaStream_t st = as_stream(stream);
+  if (int rc = run_plan(ids, pairs, E, b.plan, st)) return rc;
+  PlaceArgs pl = {};
+  pl.x = x;
+  pl.xq = b.xq;
+  pl.ascale = b.ascale;
+  pl.pos_of_pair = b.plan.pos_of_pair;
+  pl.amax = b.amax;
+  pl.per_row = topk;
+  pl.K = H;
+  if (int rc = run_place(pl, x_dtype, T, st)) return rc;
+  Product p = {};
+  p.w = w13;
+  p.w_kind = w_kind;
+  p.s1 = s13;
+  p.x = b.xq;
+  p.ascale = b.ascale;
+  p.rows = pairs;
+  p.E = E;
+  p.N = 2 * I;
+  p.K = H;
+  p.splits = b.splits1;
+  p.out_mode = b.planes1 ? kOutPlanes : kOutGated;
+  p.out = b.planes1 ? static_cast<void*>(b.planes1) : b.h;
+  p.amax = b.amax;
+  if (int rc = run_product(p, b.plan, st)) return rc;
+  HiddenArgs h = {};
+  h.planes = b.planes1;
+  h.h = b.h;
+  h.amax = b.amax;
+  h.ascale = b.ascale;
+  h.s1 = s13;
+  h.ids = ids;
+  h.counts = b.plan.counts;
+  h.pair_of_pos = b.plan.pair_of_pos;
+  h.hq = b.hq;
+  h.hscale = b.hscale;
+  h.rows = pairs;
+  h.I = I;
+  h.splits = b.splits1;
+  if (int rc = run_hidden(h, st)) return rc;
+  p.w = w2;
+  p.s1 = s2;
+  p.x = b.hq;
+  p.ascale = b.hscale;
+  p.N = H;
+  p.K = I;
+  p.splits = b.splits2;
+  p.out_mode = kOutPlanes;
+  p.out = b.planes2;
+  if (int rc = run_product(p, b.plan, st)) return rc;
+  CombineArgs k = {};
+  k.planes = b.planes2;
+  k.ascale = b.hscale;
+  k.s1 = s2;
+  k.weights = weights;
+  k.ids = ids;
+  k.pos_of_pair = b.plan.pos_of_pair;
+  k.y = y;
+  k.rows = pairs;
+  k.outs = T;
+  k.N = H;
+  k.topk = topk;
+  k.splits = b.splits2;
+  k.out_dtype = out_dtype;
+  return run_combine(k, st);
+}
+
+}  // extern "C"
