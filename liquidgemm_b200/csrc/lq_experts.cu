@@ -60,7 +60,8 @@ struct Cfg {
   static constexpr int kCols = kAcc * BN + (W4 ? 32 * kNT : 0);
   static constexpr int kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
   static constexpr int kNumBars = 2 * NS + 2 * kNT + 2 * kAcc;
-  static constexpr int kSmemBytes = 1024 /* alignment slack */ + NS * (kXStage + kWStage) + kNumBars * 8 + 16;
+  static constexpr int kRowInfo = 4 * kSets * (BN / 2);       // per warp: scale and destination of the rows it stores
+  static constexpr int kSmemBytes = 1024 /* alignment slack */ + NS * (kXStage + kWStage) + kNumBars * 8 + 16 + kRowInfo * 8;
   static_assert(kCols <= 256, "two CTAs per SM share 512 columns");
   static_assert(!W4 || NS % kSets == 0, "a set must see every use of its stages");
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
@@ -90,8 +91,9 @@ __device__ __forceinline__ Item item_at(const Args& a, int i) {
 // into a wrong code with probability d, so nothing is gained with fewer bits here.
 __device__ __forceinline__ float gated(float g, float u) { return __fmul_rn(__fdiv_rn(g, 1.0f + expf(-g)), u); }
 
-// Sixteen rows of one channel (see OutMode).  `full`: all 128 channels of the block exist.
-__device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c0, const int (&v)[16], int n, bool n_ok, float w_scale) {
+// Sixteen rows of one channel (see OutMode); `info` holds (scale, pair) of the chunk's rows.
+__device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c0, const int (&v)[16], int n, bool n_ok, float w_scale,
+                                            const float2* info) {
   const int lane = threadIdx.x & 31;
   const int valid = it.rows - c0;
   const long p0 = (long)it.row0 + c0;
@@ -104,15 +106,12 @@ __device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c
     }
     return;
   }
-  // lane j < 16 fetches the scale (and the destination) of row j; the others get them by shuffle
-  const float my_scale = lane < 16 && lane < valid ? a.ascale[p0 + lane] : 0.f;
   if (a.out_mode == kOutPairs) {
-    const int my_pair = lane < 16 && lane < valid ? a.pair_of_pos[p0 + lane] : 0;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const float sc = __shfl_sync(0xffffffffu, my_scale, j);
-      const int pair = __shfl_sync(0xffffffffu, my_pair, j);
-      if (n_ok && j < valid) store_out(a.out, (size_t)pair * a.N + n, lqq_scale(v[j], sc, w_scale), a.out_dtype);
+      const float2 row = info[j];
+      if (n_ok && j < valid)
+        store_out(a.out, (size_t)__float_as_int(row.y) * a.N + n, lqq_scale(v[j], row.x, w_scale), a.out_dtype);
     }
     return;
   }
@@ -122,8 +121,8 @@ __device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c
   float h[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float lo = lqq_scale(v[j], __shfl_sync(0xffffffffu, my_scale, j), w_scale);
-    const float hi = lqq_scale(v[j + 8], __shfl_sync(0xffffffffu, my_scale, j + 8), w_scale);
+    const float lo = lqq_scale(v[j], info[j].x, w_scale);
+    const float hi = lqq_scale(v[j + 8], info[j + 8].x, w_scale);
     const float other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
     h[j] = odd ? gated(other, hi) : gated(lo, other);
   }
@@ -171,6 +170,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   const uint32_t bar_accfree = bar_accfull + C::kAcc * 8;     // [kAcc] sums read out
   const uint32_t tmem_slot = bar_accfree + C::kAcc * 8;
   volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
+  float2* row_info = reinterpret_cast<float2*>(smem + (tmem_slot + 16 - base));   // [warp][BN / 2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -299,9 +299,27 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     Ring<kNT> tring;
     Ring<C::kAcc> accring;
     int turn = 0;
+    float2* info = row_info + (warp - 2) * (BN / 2);   // rows 16 set + 32 i + (0..15) at 16 i
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
       const Item it = item_at(args, i);
+      // What the epilogue needs beside the sums is requested here: behind the last MMA it would wait for the weight copies of
+      // the next item, which fill the queues to memory (a channel scale read there cost 3 to 5 us an item).
+      const int n = it.nt * 128 + row;
+      const bool n_ok = n < args.N;
+      float w_scale = 0.f;
+      if (args.out_mode != kOutPlanes) {
+        if (n_ok) w_scale = args.s1[(size_t)it.expert * args.N + n];
+        __syncwarp();   // every lane is done with the last item's rows
+#pragma unroll
+        for (int i2 = lane; i2 < BN / 2; i2 += 32) {
+          const int r = 32 * (i2 >> 4) + 16 * set + (i2 & 15);
+          const bool in = r < it.rows;
+          info[i2] = make_float2(in ? args.ascale[it.row0 + r] : 0.f,
+                                 __int_as_float(in && args.out_mode == kOutPairs ? args.pair_of_pos[it.row0 + r] : 0));
+        }
+        __syncwarp();
+      }
       if (W4) {
         for (int kt = it.kb; kt < it.ke; ++kt) {
           const bool mine = turn == set;
@@ -361,16 +379,13 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       ptx::tc_fence_after();
-      const int n = it.nt * 128 + row;
-      const bool n_ok = n < args.N;
-      const float w_scale = n_ok && args.out_mode != kOutPlanes ? args.s1[(size_t)it.expert * args.N + n] : 0.f;
       const uint32_t acc = tmem_acc + accring.s * BN + lane_addr;
 #pragma unroll 1
       for (int c0 = 16 * set; c0 < it.rows; c0 += 16 * kSets) {
         int v[16];
         ptx::tmem_ld16(acc + c0, v);
         ptx::tc_wait_ld();
-        store_chunk(args, it, c0, v, n, n_ok, w_scale);
+        store_chunk(args, it, c0, v, n, n_ok, w_scale, info + (c0 >> 5) * 16);
       }
       ptx::tc_fence_before();
       __syncwarp();
