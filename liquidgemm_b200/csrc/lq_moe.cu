@@ -18,9 +18,13 @@ namespace experts {
 // neighbouring experts are ranked by their largest key or by the sum of their two largest keys (without a bias: scores), and
 // only experts of the best groups stay.  Then `topk` times the largest key, the lowest index among equals.
 // Where scores decide what is chosen (keys with a bias, sums of two) they are worked out in float64: neighbouring keys may
-// lie closer than a float32 exponential's error, and a choice is a whole number.  The part has a float64 rate of half its
-// float32 rate, and the kernel is bound by its shuffles and reductions all the same.
+// lie closer than a float32 exponential's error, and a choice is a whole number.
 // A logit of -inf or NaN, or a bias that makes a key so, takes its expert out.
+//
+// Bound by instruction issue (a token's row is a few hundred bytes).  A choice is one 32-bit warp reduction over the keys'
+// upper halves and a ballot; the lower halves and the indices are compared only where several lanes hold the same upper half.
+// Groups are ranked from shared memory, 32 / G lanes to a group.  (A warp reduction of the 64-bit key for every group and
+// choice, as in the first form: 8192 tokens, 192 experts in 8 groups, 64 us.)
 
 // Orders numbers like unsigned integers; every number's image is above 0, which stands for "not to be chosen".
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -31,15 +35,10 @@ __device__ __forceinline__ unsigned long long ordered(double v) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
   return u ^ ((u >> 63) ? 0xffffffffffffffffull : 0x8000000000000000ull);
 }
-__device__ __forceinline__ double from_ordered(unsigned long long k) {
-  return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : 0xffffffffffffffffull)));
-}
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
-  return ((unsigned long long)hi << 32) | lo;
-}
+__device__ __forceinline__ uint32_t upper(uint32_t k) { return k; }
+__device__ __forceinline__ uint32_t upper(unsigned long long k) { return (uint32_t)(k >> 32); }
+__device__ __forceinline__ uint32_t lower(uint32_t) { return 0u; }
+__device__ __forceinline__ uint32_t lower(unsigned long long k) { return (uint32_t)k; }
 
 struct RouteArgs {
   const void* logits;
@@ -51,19 +50,61 @@ struct RouteArgs {
   bool sigmoid, top2, renormalize;
 };
 
-template <typename Key> struct KeyOf;
+template <typename S> struct KeyOf;
 template <> struct KeyOf<float> { using type = uint32_t; };
 template <> struct KeyOf<double> { using type = unsigned long long; };
 
+constexpr int kRouteWarps = 4;
+
+// Which groups stay: true for the groups of the topk_group highest ranks, the lowest index among equals.  `v` [E]: what the
+// groups are ranked by, -inf where an expert cannot be chosen; `rank` [n_group] and `kept` [n_group] are this warp's.
+template <typename S>
+__device__ __forceinline__ void rank_groups(const RouteArgs& a, const S* v, S* rank, uint8_t* kept) {
+  const int lane = threadIdx.x & 31;
+  const int G = a.n_group, size = a.E / G;
+  int L = 1;   // lanes of a group
+  while (2 * L * G <= 32) L *= 2;
+  for (int base = 0; base < G; base += 32 / L) {
+    const int g = base + lane / L;
+    S m1 = -INFINITY, m2 = -INFINITY;
+    if (g < G) {
+      for (int e = lane & (L - 1); e < size; e += L) {
+        const S x = v[g * size + e];
+        m2 = x > m1 ? m1 : x > m2 ? x : m2;
+        m1 = x > m1 ? x : m1;
+      }
+    }
+    for (int o = 1; o < L; o *= 2) {
+      const S b1 = __shfl_xor_sync(0xffffffffu, m1, o), b2 = __shfl_xor_sync(0xffffffffu, m2, o);
+      const S least = m1 < b1 ? m1 : b1;
+      m2 = m2 > b2 ? m2 : b2;
+      m2 = least > m2 ? least : m2;
+      m1 = m1 > b1 ? m1 : b1;
+    }
+    if (g < G && (lane & (L - 1)) == 0) rank[g] = a.top2 && m2 > (S)-INFINITY ? m1 + m2 : m1;
+  }
+  __syncwarp();
+  for (int g = lane; g < G; g += 32) {
+    const S mine = rank[g];
+    int before = 0;
+    for (int o = 0; o < G; ++o) before += (rank[o] > mine || (rank[o] == mine && o < g)) ? 1 : 0;
+    kept[g] = before < a.topk_group;
+  }
+  __syncwarp();
+}
+
 // S: the type of the scores (and with a bias of the keys).
 template <typename T, int PER, typename S>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(32 * kRouteWarps)
 route_kernel(const RouteArgs a) {
   using Key = typename KeyOf<S>::type;
+  __shared__ S values[kRouteWarps][PER * 32];
+  __shared__ S ranks[kRouteWarps][PER * 32];
+  __shared__ uint8_t kept[kRouteWarps][PER * 32];
   allow_dependents();
   dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long t = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long t = (long)blockIdx.x * kRouteWarps + warp;
   if (t >= a.T) return;
   const T* row = static_cast<const T*>(a.logits) + t * a.E;
   const float none = -INFINITY;
@@ -76,22 +117,20 @@ route_kernel(const RouteArgs a) {
     if (!(l[i] > none)) l[i] = none;   // NaN too
     top = fmaxf(top, l[i]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 
   S s[PER];
-  S sum = 0;
+  if (a.sigmoid) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const bool can = l[i] > none;
-    if (a.sigmoid) {
-      s[i] = can ? (S)1 / ((S)1 + exp(-(S)l[i])) : (S)0;
-    } else {
-      s[i] = !can ? (S)0 : l[i] == top ? (S)1 : exp((S)l[i] - (S)top);   // (equal to the largest: also where that is infinite)
+    for (int i = 0; i < PER; ++i) s[i] = l[i] > none ? (S)1 / ((S)1 + exp(-(S)l[i])) : (S)0;
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    S sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      s[i] = !(l[i] > none) ? (S)0 : l[i] == top ? (S)1 : exp((S)l[i] - (S)top);   // (equal to the largest: also where that is infinite)
       sum += s[i];
     }
-  }
-  if (!a.sigmoid) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const S d = sum > 0 ? sum : (S)1;
@@ -104,109 +143,55 @@ route_kernel(const RouteArgs a) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int e = lane + 32 * i;
-    key[i] = 0;
-    if (l[i] > none) {
-      const S v = by_score ? s[i] + (S)a.bias[e] : (S)l[i];
-      if (v > (S)none) key[i] = ordered(v);
-    }
+    S v = (S)none;
+    if (l[i] > none) v = by_score ? s[i] + (S)a.bias[e] : (S)l[i];
+    const bool can = v > (S)none;   // (false for NaN)
+    key[i] = can ? ordered(v) : 0;
+    if (a.n_group > 1) values[warp][e] = !can ? (S)none : a.top2 && !by_score ? s[i] : v;
   }
-
   if (a.n_group > 1) {
-    // lane g (and, above 32 groups, its further registers) keeps the rank key of group g
-    const int size = a.E / a.n_group;
-    Key rank[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) rank[i] = 0;
-    for (int g = 0; g < a.n_group; ++g) {
-      const int first = g * size, last = first + size;
-      Key best = 0;
-      Key mine = 0;
-      int at = -1;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        if (e >= first && e < last && key[i] > mine) mine = key[i], at = i;
-      }
-      best = warp_max(mine);
-      if (a.top2 && best != 0) {
-        // by_score: the keys' sum; else the scores of the two experts with the largest keys
-        const unsigned owner = __ballot_sync(0xffffffffu, mine == best && at >= 0);
-        const int first_lane = __ffs(owner) - 1;
-        Key second = 0;
-        int at2 = -1;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int e = lane + 32 * i;
-          if (e >= first && e < last && key[i] > second && !(lane == first_lane && i == at)) second = key[i], at2 = i;
-        }
-        const Key next = warp_max(second);
-        const unsigned owner2 = __ballot_sync(0xffffffffu, second == next && at2 >= 0);
-        S v1 = 0, v2 = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const S v = by_score ? s[i] + (S)a.bias[min(lane + 32 * i, a.E - 1)] : s[i];
-          if (i == at) v1 = v;
-          if (i == at2) v2 = v;
-        }
-        v1 = __shfl_sync(0xffffffffu, v1, first_lane);
-        v2 = __shfl_sync(0xffffffffu, v2, owner2 ? __ffs(owner2) - 1 : 0);
-        best = ordered(owner2 ? v1 + v2 : v1);
-      }
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (g == lane + 32 * i) rank[i] = best;
-    }
-    unsigned kept[PER];   // bit of lane: group lane + 32 i stays
-#pragma unroll
-    for (int i = 0; i < PER; ++i) kept[i] = 0;
-    for (int q = 0; q < a.topk_group; ++q) {
-      Key mine = 0;
-      int g = 1 << 20;
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (rank[i] > mine) mine = rank[i], g = lane + 32 * i;
-      const Key best = warp_max(mine);
-      if (best == 0) break;   // no group with an expert is left
-      const int win = (int)__reduce_min_sync(0xffffffffu, mine == best ? (unsigned)g : 1u << 20);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (win >> 5 == i) kept[i] |= 1u << (win & 31);
-        if (win == lane + 32 * i) rank[i] = 0;
-      }
-    }
+    __syncwarp();
+    rank_groups<S>(a, values[warp], ranks[warp], kept[warp]);
+    const unsigned size = a.E / a.n_group, inv = ((1u << 20) + size - 1) / size;   // e / size for e < 512
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int g = (lane + 32 * i) / size;
-      unsigned word = 0;
-#pragma unroll
-      for (int w = 0; w < PER; ++w)
-        if (g >> 5 == w) word = kept[w];
-      if (!((word >> (g & 31)) & 1u)) key[i] = 0;
+      const unsigned e = lane + 32 * i;
+      if (e < a.E && !kept[warp][e * inv >> 20]) key[i] = 0;
     }
   }
 
   // lane j ends up with choice j
   int my_id = -1;
   S my_w = 0;
+  Key mine = 0;
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (key[i] > mine) mine = key[i], at = i;
   for (int j = 0; j < a.topk; ++j) {
-    Key mine = 0;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] > mine) mine = key[i], at = i;
-    const Key best = warp_max(mine);
-    if (best == 0) break;
-    const int win = (int)__reduce_min_sync(0xffffffffu, mine == best ? (unsigned)(lane + 32 * at) : 1u << 20);
+    const uint32_t best = __reduce_max_sync(0xffffffffu, upper(mine));
+    if (best == 0) break;   // (no key's upper half is 0)
+    unsigned who = __ballot_sync(0xffffffffu, upper(mine) == best);
+    if (who & (who - 1)) {   // several lanes: the lower halves, then the index
+      const bool in = upper(mine) == best;
+      const uint32_t low = __reduce_max_sync(0xffffffffu, in ? lower(mine) : 0u);
+      const unsigned first = __reduce_min_sync(0xffffffffu, in && lower(mine) == low ? (unsigned)(lane + 32 * at) : 1u << 20);
+      who = 1u << (first & 31);
+    }
+    const int owner = __ffs(who) - 1;
+    const int id = __shfl_sync(0xffffffffu, lane + 32 * at, owner);
     S w = 0;
+    if (lane == owner) {
+      mine = 0;
+      const int gone = at;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (win == lane + 32 * i) {
-        key[i] = 0;
-        w = s[i];
+      for (int i = 0; i < PER; ++i) {
+        if (i == gone) key[i] = 0, w = s[i];
+        if (key[i] > mine) mine = key[i], at = i;
       }
     }
-    w = __shfl_sync(0xffffffffu, w, win & 31);
-    if (lane == j) my_id = win, my_w = w;
+    w = __shfl_sync(0xffffffffu, w, owner);
+    if (lane == j) my_id = id, my_w = w;
   }
   if (a.renormalize) {
     S total = my_w;
@@ -223,12 +208,14 @@ route_kernel(const RouteArgs a) {
 template <typename T, typename S>
 static int launch_route(const RouteArgs& a, cudaStream_t st) {
   const int per = (a.E + 31) / 32;
-  void (*kern)(RouteArgs) = per <= 1   ? route_kernel<T, 1, S>
-                            : per <= 2 ? route_kernel<T, 2, S>
-                            : per <= 4 ? route_kernel<T, 4, S>
-                            : per <= 8 ? route_kernel<T, 8, S>
-                                       : route_kernel<T, 16, S>;
-  const cudaError_t e = launch_overlapped(kern, dim3((a.T + 3) / 4), dim3(128), 0, st, a);
+  void (*kern)(RouteArgs) = per <= 1    ? route_kernel<T, 1, S>
+                            : per <= 2  ? route_kernel<T, 2, S>
+                            : per <= 4  ? route_kernel<T, 4, S>
+                            : per <= 6  ? route_kernel<T, 6, S>
+                            : per <= 8  ? route_kernel<T, 8, S>
+                            : per <= 12 ? route_kernel<T, 12, S>
+                                        : route_kernel<T, 16, S>;
+  const cudaError_t e = launch_overlapped(kern, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "route_kernel launch");
     return LQ_ERR_CUDA;
@@ -334,6 +321,12 @@ static int run_plan(const int* ids, long pairs, int E, const Plan& plan, cudaStr
 // One CTA per row of x (one per token, or one per pair): quantised as by quant_row_kernel of the dense linear, bit for bit,
 // and written to the places of its pairs.  NV 16-byte vectors per thread in registers; NV = 0: a row too long for that is read
 // twice.  Where the outputs are one row per pair, the rows of pairs without an expert are set to zero here.
+//
+// Up to kSortedHere pairs (`plan.tiles` set) there is no plan kernel before this one: a CTA finds the places of its own pairs
+// by counting the pairs that come before them, and one more CTA (the first) cuts the experts' rows into tiles.  That
+// saves a launch and its hand-over, 4 of the 9 us before the first product of a decode step; the counting grows with
+// the square of the pairs (at 2048 it takes the time of the plan kernel).
+constexpr int kSortedHere = 2048;
 struct PlaceArgs {
   const void* x;
   const float* x_scale;    // scales of INT8 rows
@@ -345,7 +338,76 @@ struct PlaceArgs {
   int y_size;              // bytes of an element of y
   int per_row;             // pairs of a row of x
   int K, N;
+  const int* ids;          // with plan.tiles: the sort is done here
+  int pairs, E;
+  Plan plan;
 };
+
+// Tiles and counts of the plan (one CTA of any size).
+__device__ __forceinline__ void make_tiles(const PlaceArgs& a) {
+  __shared__ int hist[kMaxExperts];
+  for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) hist[e] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.pairs; i += blockDim.x) {
+    const int e = a.ids[i];
+    if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
+  }
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  constexpr int kPer = kMaxExperts / 32;   // neighbouring experts of a lane
+  const int lane = threadIdx.x;
+  int rows = 0, tiles = 0;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int n = hist[lane * kPer + q];
+    rows += n;
+    tiles += (n + a.plan.bn - 1) / a.plan.bn;
+  }
+  int r = rows, t = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int pr = __shfl_up_sync(0xffffffffu, r, o), pt = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) r += pr, t += pt;
+  }
+  if (lane == 31) {
+    a.plan.counts[0] = t;
+    a.plan.counts[1] = r;
+  }
+  r -= rows;
+  t -= tiles;
+  for (int q = 0; q < kPer; ++q) {
+    const int e = lane * kPer + q, n = hist[e];
+    for (int at = 0; at < n; at += a.plan.bn)
+      a.plan.tiles[t++] = make_int4(e, r + at, n - at < a.plan.bn ? n - at : a.plan.bn, 0);
+    r += n;
+  }
+}
+
+// The places of the pairs of row m, in `place` [per_row] (shared memory): read from the plan, or counted and entered there.
+__device__ __forceinline__ void find_places(const PlaceArgs& a, long m, int* place) {
+  if (!a.plan.tiles) {
+    for (int j = threadIdx.x; j < a.per_row; j += blockDim.x) place[j] = a.pos_of_pair[m * a.per_row + j];
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (int j = threadIdx.x >> 5; j < a.per_row; j += blockDim.x >> 5) {
+      const int pair = (int)m * a.per_row + j;
+      const int e = a.ids[pair];
+      int before = 0;
+#pragma unroll 4
+      for (int i = lane; i < a.pairs; i += 32) {
+        const int o = a.ids[i];
+        before += (o >= 0 && (o < e || (o == e && i < pair))) ? 1 : 0;
+      }
+      before = __reduce_add_sync(0xffffffffu, before);
+      if (lane == 0) {
+        const bool some = e >= 0 && e < a.E;
+        place[j] = some ? before : -1;
+        a.plan.pos_of_pair[pair] = some ? before : -1;
+        if (some) a.plan.pair_of_pos[before] = pair;
+      }
+    }
+  }
+}
 
 __device__ __forceinline__ void clear_output_row(const PlaceArgs& a, long pair) {
   if (a.y_size == 2) {
@@ -361,10 +423,15 @@ template <typename T, int NV>
 __global__ void __launch_bounds__(1024)
 place_rows_kernel(const PlaceArgs a) {
   __shared__ float red[32];
+  __shared__ int place[kMaxTopk];
   constexpr int VEC = 16 / sizeof(T);
   allow_dependents();
   dependency_wait();
-  const long m = blockIdx.x;
+  if (a.plan.tiles && blockIdx.x == 0) {
+    make_tiles(a);
+    return;
+  }
+  const long m = a.plan.tiles ? blockIdx.x - 1 : blockIdx.x;
   const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + m * a.K);
   const int nvec = a.K / VEC;
   uint4 raw[NV > 0 ? NV : 1];
@@ -380,12 +447,13 @@ place_rows_kernel(const PlaceArgs a) {
   } else {
     for (int v = threadIdx.x; v < nvec; v += blockDim.x) rm.take(xr[v]);
   }
-  const float amax = block_max(rm.value(), red);
+  find_places(a, m, place);
+  const float amax = block_max(rm.value(), red);   // (its barrier orders the places too)
   const float scale = __fdiv_rn(fmaxf(amax, 1e-12f), 127.0f);
   const float inv = __fdiv_rn(1.0f, scale);
   for (int j = 0; j < a.per_row; ++j) {
     const long pair = m * a.per_row + j;
-    const int p = a.pos_of_pair[pair];
+    const int p = place[j];
     if (p < 0) {
       if (a.y) clear_output_row(a, pair);
       continue;
@@ -419,14 +487,21 @@ place_rows_kernel(const PlaceArgs a) {
 // Rows that come in INT8 with their scales.
 __global__ void __launch_bounds__(256)
 place_i8_kernel(const PlaceArgs a) {
+  __shared__ int place[kMaxTopk];
   allow_dependents();
   dependency_wait();
-  const long m = blockIdx.x;
+  if (a.plan.tiles && blockIdx.x == 0) {
+    make_tiles(a);
+    return;
+  }
+  const long m = a.plan.tiles ? blockIdx.x - 1 : blockIdx.x;
+  find_places(a, m, place);
+  __syncthreads();
   const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const int8_t*>(a.x) + m * a.K);
   const float scale = a.x_scale[m];
   for (int j = 0; j < a.per_row; ++j) {
     const long pair = m * a.per_row + j;
-    const int p = a.pos_of_pair[pair];
+    const int p = place[j];
     if (p < 0) {
       if (a.y) clear_output_row(a, pair);
       continue;
@@ -447,7 +522,7 @@ static int launch_place(const PlaceArgs& a, long rows, cudaStream_t st) {
                             : nv == 8 ? place_rows_kernel<T, 8>
                                       : place_rows_kernel<T, 0>;
   if (nv == 0) threads = 1024;
-  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)rows), dim3(threads), 0, st, a);
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)rows + (a.plan.tiles ? 1u : 0u)), dim3(threads), 0, st, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "place_rows_kernel launch");
     return LQ_ERR_CUDA;
@@ -455,11 +530,21 @@ static int launch_place(const PlaceArgs& a, long rows, cudaStream_t st) {
   return check_launch("place_rows_kernel");
 }
 
-static int run_place(const PlaceArgs& a, int x_dtype, long rows, cudaStream_t st) {
+// Plan and rows.
+static int run_place(PlaceArgs& a, const int* ids, long pairs, int E, const Plan& plan, int x_dtype, long rows, cudaStream_t st) {
+  a.pos_of_pair = plan.pos_of_pair;
+  if (pairs <= kSortedHere) {
+    a.ids = ids;
+    a.pairs = (int)pairs;
+    a.E = E;
+    a.plan = plan;
+  } else if (int rc = run_plan(ids, pairs, E, plan, st)) {
+    return rc;
+  }
   if (x_dtype == LQ_DT_BF16) return launch_place<__nv_bfloat16>(a, rows, st);
   if (x_dtype == LQ_DT_F16) return launch_place<__half>(a, rows, st);
   if (x_dtype == LQ_DT_F32) return launch_place<float>(a, rows, st);
-  const cudaError_t e = launch_overlapped(place_i8_kernel, dim3((unsigned)rows), dim3(256), 0, st, a);
+  const cudaError_t e = launch_overlapped(place_i8_kernel, dim3((unsigned)rows + (a.plan.tiles ? 1u : 0u)), dim3(256), 0, st, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "place_i8_kernel launch");
     return LQ_ERR_CUDA;
@@ -539,28 +624,39 @@ hidden_planes_kernel(const HiddenArgs a) {
   }
 }
 
-// The hidden values and their rows' maxima are there: codes only.
+// The hidden values and their rows' maxima are there: codes only, 256 * NV 16-byte vectors of a row per CTA.
+template <int NV>
 __global__ void __launch_bounds__(256)
 hidden_quant_kernel(const HiddenArgs a) {
   allow_dependents();
   dependency_wait();
-  const long p = blockIdx.x;
+  const int pieces = (a.I / 4 + 256 * NV - 1) / (256 * NV);
+  const long p = blockIdx.x / pieces;
+  const int first = (int)(blockIdx.x - p * pieces) * 256 * NV + threadIdx.x;
   if (p >= a.counts[1]) return;
+  const uint4* src = reinterpret_cast<const uint4*>(a.h + p * a.I);
+  uint4 raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) raw[i] = first + 256 * i < a.I / 4 ? ld_stream_v4(src + first + 256 * i) : make_uint4(0u, 0u, 0u, 0u);
   const float scale = __fdiv_rn(fmaxf(__uint_as_float(a.amax[p]), 1e-12f), 127.0f);
   const float inv = __fdiv_rn(1.0f, scale);
-  if (threadIdx.x == 0) a.hscale[p] = scale;
-  const uint4* src = reinterpret_cast<const uint4*>(a.h + p * a.I);
+  if (first == 0) a.hscale[p] = scale;
   uint32_t* dst = reinterpret_cast<uint32_t*>(a.hq + p * a.I);
-  for (int v = threadIdx.x; v < a.I / 4; v += blockDim.x) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
     uint32_t out[1];
-    quant_vec<float>(ld_stream_v4(src + v), scale, inv, out);
-    dst[v] = out[0];
+    quant_vec<float>(raw[i], scale, inv, out);
+    if (first + 256 * i < a.I / 4) dst[first + 256 * i] = out[0];
   }
 }
 
 static int run_hidden(const HiddenArgs& a, cudaStream_t st) {
-  const cudaError_t e = a.planes ? launch_overlapped(hidden_planes_kernel, dim3((unsigned)a.rows), dim3(512), 0, st, a)
-                                 : launch_overlapped(hidden_quant_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  // few rows are spread over many CTAs, many rows keep four loads of a thread in flight
+  const int nv = a.rows * (a.I / 4) > 4L * sm_count() * 2048 ? 4 : 1;
+  const long pieces = (a.I / 4 + 256 * nv - 1) / (256 * nv);
+  const cudaError_t e = a.planes  ? launch_overlapped(hidden_planes_kernel, dim3((unsigned)a.rows), dim3(512), 0, st, a)
+                        : nv == 4 ? launch_overlapped(hidden_quant_kernel<4>, dim3((unsigned)(a.rows * pieces)), dim3(256), 0, st, a)
+                                  : launch_overlapped(hidden_quant_kernel<1>, dim3((unsigned)(a.rows * pieces)), dim3(256), 0, st, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "hidden rows launch");
     return LQ_ERR_CUDA;
@@ -792,19 +888,17 @@ int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_pe
   const LinearBuffers b = carve_linear(c, pairs, E, N, K);
   if (!scratch || scratch_bytes < c.used || misaligned(scratch)) return LQ_ERR_WORKSPACE;
   cudaStream_t st = as_stream(stream);
-  if (int rc = run_plan(ids, pairs, E, b.plan, st)) return rc;
   PlaceArgs pl = {};
   pl.x = x;
   pl.x_scale = x_scale;
   pl.xq = b.xq;
   pl.ascale = b.ascale;
-  pl.pos_of_pair = b.plan.pos_of_pair;
   pl.y = b.planes ? nullptr : y;   // (from planes, the output pass writes every row)
   pl.y_size = out_dtype == LQ_DT_F32 ? 4 : 2;
   pl.per_row = x_per_pair ? 1 : topk;
   pl.K = K;
   pl.N = N;
-  if (int rc = run_place(pl, x_dtype, x_per_pair ? pairs : T, st)) return rc;
+  if (int rc = run_place(pl, ids, pairs, E, b.plan, x_dtype, x_per_pair ? pairs : T, st)) return rc;
   Product p = {};
   p.w = w;
   p.w_kind = w_kind;
@@ -858,16 +952,14 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   const MlpBuffers b = carve_mlp(c, pairs, E, H, I);
   if (!scratch || scratch_bytes < c.used || misaligned(scratch)) return LQ_ERR_WORKSPACE;
   cudaStream_t st = as_stream(stream);
-  if (int rc = run_plan(ids, pairs, E, b.plan, st)) return rc;
   PlaceArgs pl = {};
   pl.x = x;
   pl.xq = b.xq;
   pl.ascale = b.ascale;
-  pl.pos_of_pair = b.plan.pos_of_pair;
   pl.amax = b.amax;
   pl.per_row = topk;
   pl.K = H;
-  if (int rc = run_place(pl, x_dtype, T, st)) return rc;
+  if (int rc = run_place(pl, ids, pairs, E, b.plan, x_dtype, T, st)) return rc;
   Product p = {};
   p.w = w13;
   p.w_kind = w_kind;
