@@ -12,9 +12,12 @@
 // end, zeros), whose sums are not stored.
 //
 // Per CTA: warp 0 = copies (8704-byte bulk copy of a blob tile, or a 128 x 128 box of INT8 weights; boxes of rows), warp 1 =
-// tensor-memory allocation and MMA issue, warps 2..5 and 6..9 = two sets that unpack alternate k-steps into tensor memory
-// (4-bit weights) and share every epilogue.  The stage counts are even wherever two sets take turns, so that a set
-// sees every use of its stages.  All waits are bounded; status codes 161-166.
+// tensor-memory allocation and MMA issue; with 4-bit weights warps 2..5 and 6..9 = two sets that unpack alternate k-steps into
+// tensor memory and warps 10..13 the epilogue, with INT8 weights warps 2..5 and 6..9 two epilogue groups.  The epilogue of an item
+// (3 us for 16 rows with the gated activation: one warp's chain of latencies) runs beside the next item's main loop; with
+// the sets doing it themselves the weight stream stood still meanwhile (28672 x 4096, eight experts: 4 of 14 us per item).
+// The stage counts are even wherever two sets take turns, so that a set sees every use of its stages.  All waits are bounded;
+// status codes 161-166.
 #include <cuda.h>
 
 #include <mutex>
@@ -31,8 +34,7 @@ int make_byte_matrix_map(CUtensorMap* map, const void* ptr, long rows, long row_
 namespace experts {
 
 constexpr int kBlobTile = 8704;
-constexpr int kSets = 2;
-constexpr int kThreads = 64 + 128 * kSets;
+constexpr int kSets = 2;                    // unpacking sets of four warps
 constexpr int kNT = 4;                      // operand stages in tensor memory (4-bit weights)
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
@@ -53,6 +55,8 @@ struct Args {
 
 template <int BN, int NS, bool W4>
 struct Cfg {
+  static constexpr int kGroups = W4 ? 1 : 2;                  // epilogue groups of four warps
+  static constexpr int kThreads = 64 + 128 * ((W4 ? kSets : 0) + kGroups);
   static constexpr int kBox = BN >= 64 ? 32 : 16;
   static constexpr int kXStage = BN * 128;
   static constexpr int kWStage = W4 ? kBlobTile : 128 * 128;
@@ -60,7 +64,7 @@ struct Cfg {
   static constexpr int kCols = kAcc * BN + (W4 ? 32 * kNT : 0);
   static constexpr int kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
   static constexpr int kNumBars = 2 * NS + 2 * kNT + 2 * kAcc;
-  static constexpr int kRowInfo = 4 * kSets * (BN / 2);       // per warp: scale and destination of the rows it stores
+  static constexpr int kRowInfo = 4 * BN;                     // per warp: scale and destination of the rows it stores
   static constexpr int kSmemBytes = 1024 /* alignment slack */ + NS * (kXStage + kWStage) + kNumBars * 8 + 16 + kRowInfo * 8;
   static_assert(kCols <= 256, "two CTAs per SM share 512 columns");
   static_assert(!W4 || NS % kSets == 0, "a set must see every use of its stages");
@@ -151,7 +155,7 @@ __device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c
 }
 
 template <int BN, int NS, bool W4>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(Cfg<BN, NS, W4>::kThreads, 2)
 experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Args args) {
   using C = Cfg<BN, NS, W4>;
   extern __shared__ uint8_t smem_raw[];
@@ -170,7 +174,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   const uint32_t bar_accfree = bar_accfull + C::kAcc * 8;     // [kAcc] sums read out
   const uint32_t tmem_slot = bar_accfree + C::kAcc * 8;
   volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
-  float2* row_info = reinterpret_cast<float2*>(smem + (tmem_slot + 16 - base));   // [warp][BN / 2]
+  float2* row_info = reinterpret_cast<float2*>(smem + (tmem_slot + 16 - base));   // [group][quarter][BN / kGroups]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -184,7 +188,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     }
     for (int b = 0; b < C::kAcc; ++b) {
       ptx::mbar_init(bar_accfull + 8 * b, 1);
-      ptx::mbar_init(bar_accfree + 8 * b, 4 * kSets);   // one arrival per epilogue warp
+      ptx::mbar_init(bar_accfree + 8 * b, 4 * C::kGroups);   // one arrival per epilogue warp
     }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tmap_x);
@@ -289,22 +293,81 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       if (ok && leader) ptx::tc_commit(bar_accfull + 8 * accring.s);
       accring.advance();
     }
-  } else {
-    // ------------------------------------------------------------------ unpacking and epilogue
+  } else if (W4 && warp < 2 + 4 * kSets) {
+    // ------------------------------------------------------------------ unpacking
     const int quad = warp & 3;               // TMEM lane quadrant this warp may access
     const int row = quad * 32 + lane;        // channel inside the block == TMEM lane
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    const int set = (threadIdx.x - 64) >> 7;
+    const int set = (warp - 2) >> 2;
     Ring<NS> ring;
     Ring<kNT> tring;
-    Ring<C::kAcc> accring;
     int turn = 0;
-    float2* info = row_info + (warp - 2) * (BN / 2);   // rows 16 set + 32 i + (0..15) at 16 i
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
       const Item it = item_at(args, i);
-      // What the epilogue needs beside the sums is requested here: behind the last MMA it would wait for the weight copies of
-      // the next item, which fill the queues to memory (a channel scale read there cost 3 to 5 us an item).
+      for (int kt = it.kb; kt < it.ke; ++kt) {
+        const bool mine = turn == set;
+        turn ^= 1;
+        if (!mine) {
+          ring.advance();
+          tring.advance();
+          continue;
+        }
+        if (!ptx::mbar_wait_bounded(bar_full + 8 * ring.s, ring.ph, kWaitLimitNs)) {
+          atomicExch(args.status, 164);
+          ok = false;
+          break;
+        }
+        const uint8_t* wst = smem + (ws - base) + ring.s * C::kWStage;
+        uint4 ch[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ch[c] = *reinterpret_cast<const uint4*>(wst + (c * 128 + row) * 16);
+        const uint32_t meta = *reinterpret_cast<const uint32_t*>(wst + 8192 + row * 4);
+        ptx::mbar_arrive(bar_empty + 8 * ring.s);
+        const uint32_t step0 = meta & 0xffu, a0 = ((meta >> 8) & 0xffu) * 0x01010101u;
+        const uint32_t step1 = (meta >> 16) & 0xffu, a1 = (meta >> 24) * 0x01010101u;
+        uint32_t v[4][8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t step = c < 2 ? step0 : step1;
+          const uint32_t ab = c < 2 ? a0 : a1;
+          const uint32_t pk[4] = {ch[c].x, ch[c].y, ch[c].z, ch[c].w};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            v[c][2 * h] = lqq_dequant4(pk[h] & 0x0F0F0F0Fu, step, ab);
+            v[c][2 * h + 1] = lqq_dequant4((pk[h] >> 4) & 0x0F0F0F0Fu, step, ab);
+          }
+        }
+        if (!ptx::mbar_wait_bounded(bar_afree + 8 * tring.s, tring.ph ^ 1u, kWaitLimitNs)) {
+          atomicExch(args.status, 165);
+          ok = false;
+          break;
+        }
+        __syncwarp();   // lanes leave the poll loops one by one; tcgen05.st / wait::st need the warp converged
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ptx::tmem_st8(tmem_a + lane_addr + tring.s * 32 + c * 8, v[c]);
+        ptx::tc_wait_st();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(bar_aready + 8 * tring.s);
+        ring.advance();
+        tring.advance();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    constexpr int kFirst = 2 + (W4 ? 4 * kSets : 0), kRows = BN / C::kGroups;
+    const int quad = warp & 3;               // TMEM lane quadrant this warp may access
+    const int row = quad * 32 + lane;        // channel inside the block == TMEM lane
+    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+    const int group = (warp - kFirst) >> 2;
+    float2* info = row_info + (warp - kFirst) * kRows;   // rows 16 (kGroups i + group) + (0..15) at 16 i
+    Ring<C::kAcc> accring;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      const Item it = item_at(args, i);
+      // What the epilogue needs beside the sums is requested ahead of them: behind the last MMA it would wait for the weight copies
+      // of the next item, which fill the queues to memory (a channel scale read there cost 3 to 5 us an item).
       const int n = it.nt * 128 + row;
       const bool n_ok = n < args.N;
       float w_scale = 0.f;
@@ -312,64 +375,13 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         if (n_ok) w_scale = args.s1[(size_t)it.expert * args.N + n];
         __syncwarp();   // every lane is done with the last item's rows
 #pragma unroll
-        for (int i2 = lane; i2 < BN / 2; i2 += 32) {
-          const int r = 32 * (i2 >> 4) + 16 * set + (i2 & 15);
+        for (int q = lane; q < kRows; q += 32) {
+          const int r = 16 * (C::kGroups * (q >> 4) + group) + (q & 15);
           const bool in = r < it.rows;
-          info[i2] = make_float2(in ? args.ascale[it.row0 + r] : 0.f,
-                                 __int_as_float(in && args.out_mode == kOutPairs ? args.pair_of_pos[it.row0 + r] : 0));
+          info[q] = make_float2(in ? args.ascale[it.row0 + r] : 0.f,
+                                __int_as_float(in && args.out_mode == kOutPairs ? args.pair_of_pos[it.row0 + r] : 0));
         }
         __syncwarp();
-      }
-      if (W4) {
-        for (int kt = it.kb; kt < it.ke; ++kt) {
-          const bool mine = turn == set;
-          turn ^= 1;
-          if (!mine) {
-            ring.advance();
-            tring.advance();
-            continue;
-          }
-          if (!ptx::mbar_wait_bounded(bar_full + 8 * ring.s, ring.ph, kWaitLimitNs)) {
-            atomicExch(args.status, 164);
-            ok = false;
-            break;
-          }
-          const uint8_t* wst = smem + (ws - base) + ring.s * C::kWStage;
-          uint4 ch[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) ch[c] = *reinterpret_cast<const uint4*>(wst + (c * 128 + row) * 16);
-          const uint32_t meta = *reinterpret_cast<const uint32_t*>(wst + 8192 + row * 4);
-          ptx::mbar_arrive(bar_empty + 8 * ring.s);
-          const uint32_t step0 = meta & 0xffu, a0 = ((meta >> 8) & 0xffu) * 0x01010101u;
-          const uint32_t step1 = (meta >> 16) & 0xffu, a1 = (meta >> 24) * 0x01010101u;
-          uint32_t v[4][8];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t step = c < 2 ? step0 : step1;
-            const uint32_t ab = c < 2 ? a0 : a1;
-            const uint32_t pk[4] = {ch[c].x, ch[c].y, ch[c].z, ch[c].w};
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              v[c][2 * h] = lqq_dequant4(pk[h] & 0x0F0F0F0Fu, step, ab);
-              v[c][2 * h + 1] = lqq_dequant4((pk[h] >> 4) & 0x0F0F0F0Fu, step, ab);
-            }
-          }
-          if (!ptx::mbar_wait_bounded(bar_afree + 8 * tring.s, tring.ph ^ 1u, kWaitLimitNs)) {
-            atomicExch(args.status, 165);
-            ok = false;
-            break;
-          }
-          __syncwarp();   // lanes leave the poll loops one by one; tcgen05.st / wait::st need the warp converged
-          ptx::tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) ptx::tmem_st8(tmem_a + lane_addr + tring.s * 32 + c * 8, v[c]);
-          ptx::tc_wait_st();
-          ptx::tc_fence_before();
-          ptx::mbar_arrive(bar_aready + 8 * tring.s);
-          ring.advance();
-          tring.advance();
-        }
-        if (!ok) break;
       }
       if (!ptx::mbar_wait_bounded(bar_accfull + 8 * accring.s, accring.ph, kWaitLimitNs)) {
         atomicExch(args.status, 166);
@@ -381,11 +393,11 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       ptx::tc_fence_after();
       const uint32_t acc = tmem_acc + accring.s * BN + lane_addr;
 #pragma unroll 1
-      for (int c0 = 16 * set; c0 < it.rows; c0 += 16 * kSets) {
+      for (int c0 = 16 * group, at = 0; c0 < it.rows; c0 += 16 * C::kGroups, at += 16) {
         int v[16];
         ptx::tmem_ld16(acc + c0, v);
         ptx::tc_wait_ld();
-        store_chunk(args, it, c0, v, n, n_ok, w_scale, info + (c0 >> 5) * 16);
+        store_chunk(args, it, c0, v, n, n_ok, w_scale, info + at);
       }
       ptx::tc_fence_before();
       __syncwarp();
@@ -443,7 +455,7 @@ static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
   if (!a.status) return LQ_ERR_CUDA;
   const long items = max_tiles(p.rows, p.E, plan.bn) * a.n_tiles * a.splits;
   const long slots = 2L * sm_count();
-  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(kThreads),
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(C::kThreads),
                                           (size_t)C::kSmemBytes, st, tx, tw, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "experts_kernel launch");
