@@ -334,7 +334,7 @@ LQ_API int lq_moe_route(const void* logits, int logits_dtype, const float* bias,
  * behind the other (lq_tile_blob_bytes(N, K) each), 1: INT8 [E, N, K].  s1 [E, N].  y [T, topk, N].
  * K % 128 == 0, E <= 512, topk <= 32, T * topk <= 2^24; x, w and scratch 16-byte aligned.
  * `scratch`: lq_experts_linear_scratch_bytes() bytes, any content (0 from that function: sizes out of range). */
-LQ_API size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K);
+LQ_API size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K, int w_kind);
 LQ_API int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_per_pair, const int32_t* ids,
                              const void* w, int w_kind, const float* s1, void* y, int out_dtype, int T, int topk, int E,
                              int N, int K, void* scratch, size_t scratch_bytes, void* stream);
@@ -345,7 +345,7 @@ LQ_API int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, i
  * w13 [E, 2 I, H] holds gate channel c in row 2 c and up channel c in row 2 c + 1; w2 [E, H, I]; both in the form of
  * w_kind.  weights [T, topk] float32; an id outside [0, E) adds nothing.  H % 128 == 0 and I % 128 == 0, the other limits as
  * above; s13 and s2 16-byte aligned. */
-LQ_API size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I);
+LQ_API size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I, int w_kind);
 LQ_API int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32_t* ids, const void* w13,
                           const float* s13, const void* w2, const float* s2, int w_kind, void* y, int out_dtype, int T,
                           int topk, int E, int H, int I, void* scratch, size_t scratch_bytes, void* stream);

@@ -67,10 +67,10 @@ _SIGNATURES = {
     "lq_i8_gemm_i32_ws": (c_int, [P, P, P, c_int, c_int, c_int, P, c_size_t, P]),
     "lq_i8_gemm_scaled_ws": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, P, c_size_t, P]),
     "lq_moe_route": (c_int, [P, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.c_float, P]),
-    "lq_experts_linear_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "lq_experts_linear_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "lq_experts_linear": (c_int, [P, c_int, P, c_int, P, P, c_int, P, P, c_int, c_int, c_int, c_int, c_int, c_int, P,
                                   c_size_t, P]),
-    "lq_experts_mlp_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "lq_experts_mlp_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "lq_experts_mlp": (c_int, [P, c_int, P, P, P, P, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, P,
                                c_size_t, P]),
 }

@@ -23,6 +23,7 @@
 #include <mutex>
 
 #include "lq_experts.cuh"
+#include "lq_experts_epi.cuh"
 #include "lq_sched.cuh"
 #include "lq_tc_ptx.cuh"
 
@@ -45,11 +46,8 @@ struct Args {
   const int* counts;
   const int4* tiles;
   const int* pair_of_pos;
-  void* out;
-  unsigned* amax;
+  EpiArgs epi;
   int* status;
-  long rows;
-  int out_mode, out_dtype;
   int N, kt_total, n_tiles, splits;
 };
 
@@ -91,70 +89,7 @@ __device__ __forceinline__ Item item_at(const Args& a, int i) {
   return it;
 }
 
-// silu(g) * u.  expf and a correctly rounded division: the hidden rows are quantised next, which turns an error of d counts
-// into a wrong code with probability d, so nothing is gained with fewer bits here.
-__device__ __forceinline__ float gated(float g, float u) { return __fmul_rn(__fdiv_rn(g, 1.0f + expf(-g)), u); }
-
-// Sixteen rows of one channel (see OutMode); `info` holds (scale, pair) of the chunk's rows.
-__device__ __forceinline__ void store_chunk(const Args& a, const Item& it, int c0, const int (&v)[16], int n, bool n_ok, float w_scale,
-                                            const float2* info) {
-  const int lane = threadIdx.x & 31;
-  const int valid = it.rows - c0;
-  const long p0 = (long)it.row0 + c0;
-  if (a.out_mode == kOutPlanes) {
-    if (n_ok) {
-      int32_t* o = static_cast<int32_t*>(a.out) + ((size_t)it.s * a.rows + p0) * a.N + n;
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < valid) o[(size_t)j * a.N] = v[j];
-    }
-    return;
-  }
-  if (a.out_mode == kOutPairs) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float2 row = info[j];
-      if (n_ok && j < valid)
-        store_out(a.out, (size_t)__float_as_int(row.y) * a.N + n, lqq_scale(v[j], row.x, w_scale), a.out_dtype);
-    }
-    return;
-  }
-  // Gated: an even lane holds the gate and the odd one beside it the up value of the same hidden channel.  The even lane
-  // takes rows 0..7 and the odd one rows 8..15, each handing over what the other needs.
-  const bool odd = lane & 1;
-  float h[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float lo = lqq_scale(v[j], info[j].x, w_scale);
-    const float hi = lqq_scale(v[j + 8], info[j + 8].x, w_scale);
-    const float other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
-    h[j] = odd ? gated(other, hi) : gated(lo, other);
-  }
-  const int first = odd ? 8 : 0;
-  float* o = static_cast<float*>(a.out) + (size_t)(p0 + first) * (a.N / 2) + (n >> 1);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (first + j < valid) o[(size_t)j * (a.N / 2)] = h[j];
-  // the rows' largest magnitudes over the warp's 16 hidden channels: after three halving steps every lane holds one row
-  float m[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m[j] = fabsf(h[j]);
-#pragma unroll
-  for (int w = 4; w >= 1; w >>= 1) {
-    const bool up = lane & (2 * (4 / w));   // lane bits 1, 2, 3
-#pragma unroll
-    for (int j = 0; j < w; ++j) {
-      const float keep = up ? m[j + w] : m[j], give = up ? m[j] : m[j + w];
-      m[j] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, 2 * (4 / w)));
-    }
-  }
-  m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], 16));
-  const int row = first + ((lane & 2) ? 4 : 0) + ((lane & 4) ? 2 : 0) + ((lane & 8) ? 1 : 0);
-  // magnitudes compare like their bits; the order of the atomics does not matter to a maximum
-  if (lane < 16 && row < valid) atomicMax(a.amax + p0 + row, __float_as_uint(m[0]));
-}
-
-template <int BN, int NS, bool W4>
+template <int BN, int NS, bool W4, int MODE>
 __global__ void __launch_bounds__(Cfg<BN, NS, W4>::kThreads, 2)
 experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Args args) {
   using C = Cfg<BN, NS, W4>;
@@ -174,7 +109,8 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   const uint32_t bar_accfree = bar_accfull + C::kAcc * 8;     // [kAcc] sums read out
   const uint32_t tmem_slot = bar_accfree + C::kAcc * 8;
   volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
-  float2* row_info = reinterpret_cast<float2*>(smem + (tmem_slot + 16 - base));   // [group][quarter][BN / kGroups]
+  float* row_scale = reinterpret_cast<float*>(smem + (tmem_slot + 16 - base));   // [epilogue warp][BN / kGroups]
+  int* row_pair = reinterpret_cast<int*>(row_scale + C::kRowInfo);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -361,7 +297,8 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     const int row = quad * 32 + lane;        // channel inside the block == TMEM lane
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const int group = (warp - kFirst) >> 2;
-    float2* info = row_info + (warp - kFirst) * kRows;   // rows 16 (kGroups i + group) + (0..15) at 16 i
+    float* sc = row_scale + (warp - kFirst) * kRows;   // rows 16 (kGroups i + group) + (0..15) at 16 i
+    int* pair = row_pair + (warp - kFirst) * kRows;
     Ring<C::kAcc> accring;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
@@ -371,15 +308,15 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       const int n = it.nt * 128 + row;
       const bool n_ok = n < args.N;
       float w_scale = 0.f;
-      if (args.out_mode != kOutPlanes) {
+      if (MODE != kOutPlanes) {
         if (n_ok) w_scale = args.s1[(size_t)it.expert * args.N + n];
         __syncwarp();   // every lane is done with the last item's rows
 #pragma unroll
         for (int q = lane; q < kRows; q += 32) {
           const int r = 16 * (C::kGroups * (q >> 4) + group) + (q & 15);
           const bool in = r < it.rows;
-          info[q] = make_float2(in ? args.ascale[it.row0 + r] : 0.f,
-                                __int_as_float(in && args.out_mode == kOutPairs ? args.pair_of_pos[it.row0 + r] : 0));
+          sc[q] = in ? args.ascale[it.row0 + r] : 0.f;
+          if (MODE == kOutPairs) pair[q] = in ? args.pair_of_pos[it.row0 + r] : 0;
         }
         __syncwarp();
       }
@@ -397,7 +334,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         int v[16];
         ptx::tmem_ld16(acc + c0, v);
         ptx::tc_wait_ld();
-        store_chunk(args, it, c0, v, n, n_ok, w_scale, info + at);
+        store_rows<MODE>(args.epi, v, (long)it.row0 + c0, it.rows - c0, n, n_ok, w_scale, sc + at, pair + at, it.s);
       }
       ptx::tc_fence_before();
       __syncwarp();
@@ -416,10 +353,10 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   }
 }
 
-template <int BN, int NS, bool W4>
-static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
+template <int BN, int NS, bool W4, int MODE>
+static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
   using C = Cfg<BN, NS, W4>;
-  auto kern = &experts_kernel<BN, NS, W4>;
+  auto kern = &experts_kernel<BN, NS, W4, MODE>;
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -442,12 +379,12 @@ static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
   a.counts = plan.counts;
   a.tiles = plan.tiles;
   a.pair_of_pos = plan.pair_of_pos;
-  a.out = p.out;
-  a.amax = p.amax;
+  a.epi.out = p.out;
+  a.epi.amax = p.amax;
+  a.epi.rows = p.rows;
+  a.epi.N = p.N;
+  a.epi.out_dtype = p.out_dtype;
   a.status = status_word();
-  a.rows = p.rows;
-  a.out_mode = p.out_mode;
-  a.out_dtype = p.out_dtype;
   a.N = p.N;
   a.kt_total = p.K / 128;
   a.n_tiles = (p.N + 127) / 128;
@@ -464,7 +401,15 @@ static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
   return check_launch("experts_kernel");
 }
 
+template <int BN, int NS, bool W4>
+static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
+  if (p.out_mode == kOutPlanes) return launch_mode<BN, NS, W4, kOutPlanes>(p, plan, st);
+  if (p.out_mode == kOutPairs) return launch_mode<BN, NS, W4, kOutPairs>(p, plan, st);
+  return launch_mode<BN, NS, W4, kOutGated>(p, plan, st);
+}
+
 int run_product(const Product& p, const Plan& plan, cudaStream_t st) {
+  if (plan.bn > 128) return run_product_pair(p, plan, st);
   if (p.w_kind == kBlob) {
     switch (plan.bn) {
       case 32: return launch_product<32, 8, true>(p, plan, st);

@@ -50,7 +50,10 @@ struct Product {
   void* out;
   unsigned* amax;
 };
-int run_product(const Product& p, const Plan& plan, cudaStream_t st);   // lq_experts.cu
+int run_product(const Product& p, const Plan& plan, cudaStream_t st);        // lq_experts.cu
+// Tiles of the CTA-pair kernel (lq_experts_pair.cu), which run_product takes for plans of that width.
+constexpr int kPairRowsBlob = 192, kPairRowsInt8 = 256;
+int run_product_pair(const Product& p, const Plan& plan, cudaStream_t st);
 
 }  // namespace experts
 }  // namespace lq

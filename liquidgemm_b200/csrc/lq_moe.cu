@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "lq_experts.cuh"
+#include "lq_experts_epi.cuh"
 
 namespace lq {
 namespace experts {
@@ -226,6 +227,17 @@ static int launch_route(const RouteArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------------------------
+// The tiles of expert e: as few as cover its n rows, and of equal widths in steps of 32 (a full tile and a narrow rest would
+// take as long as two full ones wherever the two run side by side).  Every one has a row: bn is a multiple of 32.
+__device__ __forceinline__ void write_tiles(const Plan& plan, int tile0, int e, int row0, int n, int tiles) {
+  if (tiles == 0) return;
+  const int per = ((n + tiles - 1) / tiles + 31) & ~31;
+  for (int i = 0; i < tiles; ++i) {
+    const int left = n - i * per;
+    plan.tiles[tile0 + i] = make_int4(e, row0 + i * per, left < per ? left : per, 0);
+  }
+}
+
 // One CTA of 32 warps.  Warp w counts the pairs of its contiguous share per expert, the counts are summed over warps and
 // experts, and in a second pass every pair's row is the running count of its (warp, expert): a stable sort, the same
 // on every run.
@@ -271,10 +283,7 @@ plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
   const int row0 = ra + a - n, tile0 = rb + b - tiles;
   if (e < E) {
     for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] += row0;
-    for (int i = 0; i < tiles; ++i) {
-      const int left = n - i * plan.bn;
-      plan.tiles[tile0 + i] = make_int4(e, row0 + i * plan.bn, left < plan.bn ? left : plan.bn, 0);
-    }
+    write_tiles(plan, tile0, e, row0, n, tiles);
   }
   if (threadIdx.x == blockDim.x - 1) {
     plan.counts[0] = rb + b;
@@ -377,8 +386,9 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a) {
   t -= tiles;
   for (int q = 0; q < kPer; ++q) {
     const int e = lane * kPer + q, n = hist[e];
-    for (int at = 0; at < n; at += a.plan.bn)
-      a.plan.tiles[t++] = make_int4(e, r + at, n - at < a.plan.bn ? n - at : a.plan.bn, 0);
+    const int mine = (n + a.plan.bn - 1) / a.plan.bn;
+    write_tiles(a.plan, t, e, r, n, mine);
+    t += mine;
     r += n;
   }
 }
@@ -570,8 +580,6 @@ struct HiddenArgs {
   int I, splits;
 };
 
-__device__ __forceinline__ float gated_hidden(float g, float u) { return __fmul_rn(__fdiv_rn(g, 1.0f + expf(-g)), u); }
-
 // Four hidden values of row p from the planes.
 __device__ __forceinline__ void hidden4(const HiddenArgs& a, long p, const float* s1, float as, int c, float (&h)[4]) {
   int4 g0 = make_int4(0, 0, 0, 0), g1 = g0;
@@ -582,10 +590,10 @@ __device__ __forceinline__ void hidden4(const HiddenArgs& a, long p, const float
     g1.x += v1.x; g1.y += v1.y; g1.z += v1.z; g1.w += v1.w;
   }
   const float4 f0 = *reinterpret_cast<const float4*>(s1 + 2 * c), f1 = *reinterpret_cast<const float4*>(s1 + 2 * c + 4);
-  h[0] = gated_hidden(lqq_scale(g0.x, as, f0.x), lqq_scale(g0.y, as, f0.y));
-  h[1] = gated_hidden(lqq_scale(g0.z, as, f0.z), lqq_scale(g0.w, as, f0.w));
-  h[2] = gated_hidden(lqq_scale(g1.x, as, f1.x), lqq_scale(g1.y, as, f1.y));
-  h[3] = gated_hidden(lqq_scale(g1.z, as, f1.z), lqq_scale(g1.w, as, f1.w));
+  h[0] = gated(lqq_scale(g0.x, as, f0.x), lqq_scale(g0.y, as, f0.y));
+  h[1] = gated(lqq_scale(g0.z, as, f0.z), lqq_scale(g0.w, as, f0.w));
+  h[2] = gated(lqq_scale(g1.x, as, f1.x), lqq_scale(g1.y, as, f1.y));
+  h[3] = gated(lqq_scale(g1.z, as, f1.z), lqq_scale(g1.w, as, f1.w));
 }
 
 __device__ __forceinline__ uint32_t quant4(const float (&h)[4], float scale, float inv) {
@@ -740,14 +748,16 @@ static int run_combine(const CombineArgs& a, cudaStream_t st) {
 // sizes
 // ---------------------------------------------------------------------------------------------
 // Rows of a tile: what an expert gets on average, with room for the uneven choice of a router.
-static int pick_bn(long pairs, int E) {
+static int pick_bn(long pairs, int E, int w_kind) {
   const long mean = pairs / E;
+  if (mean >= 96) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
   return mean <= 12 ? 32 : mean <= 40 ? 64 : 128;
 }
 
 // K-ranges of a product: only where the tiles of the experts that can be reached leave half of the CTA slots free, and with four
 // k-steps a range at least.
 static int pick_splits(long pairs, int E, int bn, int N, int K) {
+  if (bn > 128) return 1;   // the pair kernel takes whole tiles
   const long reached = pairs < E ? pairs : E;
   const long tiles = reached * ((pairs / reached + bn - 1) / bn) * ((N + 127) / 128);
   const long slots = 2L * sm_count();
@@ -771,9 +781,9 @@ struct Carver {
   }
 };
 
-static Plan carve_plan(Carver& c, long pairs, int E) {
+static Plan carve_plan(Carver& c, long pairs, int E, int w_kind) {
   Plan p;
-  p.bn = pick_bn(pairs, E);
+  p.bn = pick_bn(pairs, E, w_kind);
   p.counts = c.take<int>(4);
   p.tiles = c.take<int4>((size_t)max_tiles(pairs, E, p.bn));
   p.pos_of_pair = c.take<int>((size_t)pairs);
@@ -788,9 +798,9 @@ struct LinearBuffers {
   int32_t* planes;
   int splits;
 };
-static LinearBuffers carve_linear(Carver& c, long pairs, int E, int N, int K) {
+static LinearBuffers carve_linear(Carver& c, long pairs, int E, int N, int K, int w_kind) {
   LinearBuffers b;
-  b.plan = carve_plan(c, pairs, E);
+  b.plan = carve_plan(c, pairs, E, w_kind);
   b.splits = pick_splits(pairs, E, b.plan.bn, N, K);
   b.xq = c.take<int8_t>((size_t)pairs * K);
   b.ascale = c.take<float>((size_t)pairs);
@@ -806,9 +816,9 @@ struct MlpBuffers {
   int32_t *planes1, *planes2;
   int splits1, splits2;
 };
-static MlpBuffers carve_mlp(Carver& c, long pairs, int E, int H, int I) {
+static MlpBuffers carve_mlp(Carver& c, long pairs, int E, int H, int I, int w_kind) {
   MlpBuffers b;
-  b.plan = carve_plan(c, pairs, E);
+  b.plan = carve_plan(c, pairs, E, w_kind);
   b.splits1 = pick_splits(pairs, E, b.plan.bn, 2 * I, H);
   b.splits2 = pick_splits(pairs, E, b.plan.bn, H, I);
   b.xq = c.take<int8_t>((size_t)pairs * H);
@@ -868,10 +878,11 @@ int lq_moe_route(const void* logits, int logits_dtype, const float* bias, float*
   return wide ? launch_route<float, double>(a, st) : launch_route<float, float>(a, st);
 }
 
-size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K) {
+size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K, int w_kind) {
+  if (w_kind < 0 || w_kind > 1) return 0;
   if (check_sizes(T, topk, E, N, K)) return 0;
   Carver c(nullptr);
-  carve_linear(c, (long)T * topk, E, N, K);
+  carve_linear(c, (long)T * topk, E, N, K, w_kind);
   return c.used;
 }
 
@@ -885,7 +896,7 @@ int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_pe
   if (misaligned(x) || misaligned(w)) return LQ_ERR_SHAPE;
   Carver c(scratch);
   const long pairs = (long)T * topk;
-  const LinearBuffers b = carve_linear(c, pairs, E, N, K);
+  const LinearBuffers b = carve_linear(c, pairs, E, N, K, w_kind);
   if (!scratch || scratch_bytes < c.used || misaligned(scratch)) return LQ_ERR_WORKSPACE;
   cudaStream_t st = as_stream(stream);
   PlaceArgs pl = {};
@@ -930,10 +941,11 @@ int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_pe
   return run_combine(k, st);
 }
 
-size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I) {
+size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I, int w_kind) {
+  if (w_kind < 0 || w_kind > 1) return 0;
   if (check_sizes(T, topk, E, 2 * I, H) || check_sizes(T, topk, E, H, I)) return 0;
   Carver c(nullptr);
-  carve_mlp(c, (long)T * topk, E, H, I);
+  carve_mlp(c, (long)T * topk, E, H, I, w_kind);
   return c.used;
 }
 
@@ -949,7 +961,7 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   if (misaligned(x) || misaligned(w13) || misaligned(w2) || misaligned(s13) || misaligned(s2)) return LQ_ERR_SHAPE;
   Carver c(scratch);
   const long pairs = (long)T * topk;
-  const MlpBuffers b = carve_mlp(c, pairs, E, H, I);
+  const MlpBuffers b = carve_mlp(c, pairs, E, H, I, w_kind);
   if (!scratch || scratch_bytes < c.used || misaligned(scratch)) return LQ_ERR_WORKSPACE;
   cudaStream_t st = as_stream(stream);
   PlaceArgs pl = {};

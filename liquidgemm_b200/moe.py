@@ -140,7 +140,7 @@ def _experts_linear(x, ascale, ids, w, s1, N, K, out_dtype):
     per_pair = x.dim() == 3
     x = _aligned(x)
     with _dev_ctx(x):
-        scratch = _scratch(lib.lq_experts_linear_scratch_bytes(T, topk, E, N, K), x)
+        scratch = _scratch(lib.lq_experts_linear_scratch_bytes(T, topk, E, N, K, kind), x)
         check(lib.lq_experts_linear(_ptr(x), code, None if ascale is None else _ptr(ascale), int(per_pair), _ptr(ids), _ptr(w),
                                     kind, _ptr(s1), _ptr(y), int(out_dtype), T, topk, E, N, K, _ptr(scratch), scratch.numel(),
                                     _stream()), "experts_linear")
@@ -166,7 +166,7 @@ def _experts_mlp(x, weights, ids, w13, s13, w2, s2, out_dtype):
         return y
     x, weights = _aligned(x), weights.contiguous()
     with _dev_ctx(x):
-        scratch = _scratch(lib.lq_experts_mlp_scratch_bytes(T, topk, E, H, inner), x)
+        scratch = _scratch(lib.lq_experts_mlp_scratch_bytes(T, topk, E, H, inner, kind), x)
         check(lib.lq_experts_mlp(_ptr(x), _DTYPE_CODES[x.dtype], _ptr(weights), _ptr(ids), _ptr(w13), _ptr(s13), _ptr(w2),
                                  _ptr(s2), kind, _ptr(y), int(out_dtype), T, topk, E, H, inner, _ptr(scratch),
                                  scratch.numel(), _stream()), "experts_mlp")

@@ -2,9 +2,10 @@
 
 ``experts_linear`` is defined bit for bit (exact sums, two rounded float32 products, one rounding): tolerance none.
 
-``experts_mlp`` quantises hidden values that carry float32 rounding: with g and u off by 3 * 2^-24 (the conversion of the sum, two
-products) the gated value is off by a relative (12 + 3 |g|) 2^-24 at most (the exponential's argument, 2 units in the last place of
-the function, sum, division, product).  A code can differ by one only where its quotient lies that near to a half-integer, counting the
+``experts_mlp`` quantises hidden values that carry float32 rounding, counted in steps of 2^-24: g and u are off by 3 each (the
+conversion of the sum, two products); exp(-g) by 3 |g| for its argument and 4 for the function (2 units in the last place); the
+sum 1 + exp(-g) by no more than that and 1; its approximate reciprocal by 2 (one unit), the two products by 1 each:
+3 + 3 + 4 + 1 + 2 + 1 + 1 = 15, so a relative (16 + 3 |g|) 2^-24 with the products of errors.  A code can differ by one only where its quotient lies that near to a half-integer, counting the
 scale's error too; the tolerance adds up what such codes can change, exactly where they are, and behind it the float32
 roundings of the weighted sum (topk + 6 of 2^-24) and half a step of the output type."""
 
@@ -123,14 +124,14 @@ def _mlp(x, weights, ids, q13, s13, q2, s2):
         amax, at = h.abs().max(1, keepdim=True)
         hs = (amax.clamp_min(1e-12) / 127.0).float().double()
         quot = h / hs
-        off = ((12 + 3 * g.abs()) + (12 + 3 * g.abs().gather(1, at)) + 3) * EPS24        # relative, of the quotient
+        off = ((16 + 3 * g.abs()) + (16 + 3 * g.abs().gather(1, at)) + 3) * EPS24        # relative, of the quotient
         near = ((quot.abs() % 1.0) - 0.5).abs() <= quot.abs() * off + 1e-30
         code = torch.round(quot.float()).clamp(-127, 127).double()
         w = weights.reshape(-1)[mine, None].double()
         o = (code @ q2[e].t()) * hs * s2[e].double() * w
         y.index_add_(0, rows, o)
         flips = (near.double() @ q2[e].abs().t()) * hs * s2[e].double() * w.abs()
-        scale_off = (12 + 3 * g.abs().gather(1, at) + 4) * EPS24
+        scale_off = (16 + 3 * g.abs().gather(1, at) + 4) * EPS24
         tol.index_add_(0, rows, flips + o.abs() * (scale_off + (k + 6) * EPS24))
     return y, tol
 

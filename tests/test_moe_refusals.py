@@ -46,12 +46,13 @@ def test_linear_bad_shapes(change):
 
 @pytest.mark.parametrize("kind", [0, 1])
 def test_linear_scratch(kind):
-    need = lib.lq_experts_linear_scratch_bytes(4, 2, 8, 256, 256)
+    need = lib.lq_experts_linear_scratch_bytes(4, 2, 8, 256, 256, kind)
     assert need > 4 * 2 * 256
     for scratch, nbytes in ((None, BIG), (P, need - 1), (P + 8, BIG)):
         assert _linear(kind=kind, scratch=scratch, nbytes=nbytes) == WORKSPACE
     for bad in ((0, 2, 8, 256, 256), (4, 33, 8, 256, 256), (4, 2, 513, 256, 256), (4, 2, 8, 256, 200), (4, 2, 8, 0, 256)):
-        assert lib.lq_experts_linear_scratch_bytes(*bad) == 0
+        assert lib.lq_experts_linear_scratch_bytes(*bad, kind) == 0
+    assert lib.lq_experts_linear_scratch_bytes(4, 2, 8, 256, 256, 2) == 0
 
 
 def _mlp(x=P, x_dtype=0, weights=P, ids=P, w13=P, s13=P, w2=P, s2=P, kind=0, y=P, out=0, T=4, topk=2, E=8, H=256, inner=256,
@@ -72,11 +73,11 @@ def test_mlp_bad_shapes(change):
 
 
 def test_mlp_scratch():
-    need = lib.lq_experts_mlp_scratch_bytes(4, 2, 8, 256, 384)
+    need = lib.lq_experts_mlp_scratch_bytes(4, 2, 8, 256, 384, 0)
     assert need > 4 * 2 * (256 + 384)
     for scratch, nbytes in ((None, BIG), (P, need - 1), (P + 8, BIG)):
         assert _mlp(inner=384, scratch=scratch, nbytes=nbytes) == WORKSPACE
-    assert lib.lq_experts_mlp_scratch_bytes(4, 2, 8, 256, 100) == 0
+    assert lib.lq_experts_mlp_scratch_bytes(4, 2, 8, 256, 100, 0) == 0 and lib.lq_experts_mlp_scratch_bytes(4, 2, 8, 256, 384, 2) == 0
 
 
 # ---- Python checks that need no device -----------------------------------------------------------------------------
