@@ -145,41 +145,42 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
 
   if (warp == 0) {
     // ------------------------------------------------------------------ copies
-    if (lane == 0) {
-      Ring<NS> ring;
-      int issued = 0;
-      bool ok = true;
-      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-        const Item it = item_at(args, i);
-        const int boxes = (it.rows + C::kBox - 1) / C::kBox;
-        const uint32_t tx = (uint32_t)(boxes * C::kBox * 128 + C::kWStage);
-        const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;
-        const int wrow = W4 ? 0 : it.expert * args.N + it.nt * 128;
-        for (int kt = it.kb; kt < it.ke; ++kt) {
-          if (!ptx::mbar_wait_bounded(bar_empty + 8 * ring.s, ring.ph ^ 1u, kWaitLimitNs)) {
-            atomicExch(args.status, 161);
-            ok = false;
-            break;
-          }
-          const uint32_t full = bar_full + 8 * ring.s;
-          ptx::mbar_expect_tx(full, tx);
-          if (W4) {
-            ptx::bulk_load(ws + ring.s * C::kWStage, src, kBlobTile, full);
-            src += kBlobTile;
-          } else {
-            ptx::tensor_load_2d(ws + ring.s * C::kWStage, &tmap_w, kt * 128, wrow, full);
-          }
-          for (int b = 0; b < boxes; ++b)
-            ptx::tensor_load_2d(xs + ring.s * C::kXStage + b * C::kBox * 128, &tmap_x, kt * 128, it.row0 + b * C::kBox, full);
-          ring.advance();
-          ++issued;
+    // The whole warp walks the loop and one elected lane issues, as with the MMAs (see ptx::elect_one): a loop that only thread 0
+    // walks takes about 450 cycles a k-step.
+    const bool leader = ptx::elect_one();
+    Ring<NS> ring;
+    int issued = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      const Item it = item_at(args, i);
+      const int boxes = (it.rows + C::kBox - 1) / C::kBox;
+      const uint32_t tx = (uint32_t)(boxes * C::kBox * 128 + C::kWStage);
+      const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;
+      const int wrow = W4 ? 0 : it.expert * args.N + it.nt * 128;
+      for (int kt = it.kb; kt < it.ke; ++kt) {
+        ok = ptx::mbar_wait_bounded(bar_empty + 8 * ring.s, ring.ph ^ 1u, kWaitLimitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (leader) atomicExch(args.status, 161);
+          break;
         }
+        const uint32_t full = bar_full + 8 * ring.s;
+        const uint32_t wdst = ws + ring.s * C::kWStage, xdst = xs + ring.s * C::kXStage;
+        if (leader) {
+          ptx::mbar_expect_tx(full, tx);
+          if (W4) ptx::bulk_load(wdst, src, kBlobTile, full);
+          else ptx::tensor_load_2d(wdst, &tmap_w, kt * 128, wrow, full);
+          for (int b = 0; b < boxes; ++b) ptx::tensor_load_2d(xdst + b * C::kBox * 128, &tmap_x, kt * 128, it.row0 + b * C::kBox, full);
+        }
+        if (W4) src += kBlobTile;
+        ring.advance();
+        ++issued;
       }
-      if (!ok) {
-        // copies already issued still write shared memory: let them land before the CTA exits
-        for (int q = issued > NS ? issued - NS : 0; q < issued; ++q)
-          ptx::mbar_wait_bounded(bar_full + 8 * (q % NS), (uint32_t)(q / NS) & 1u, kWaitLimitNs);
-      }
+    }
+    if (!ok) {
+      // copies already issued still write shared memory: let them land before the CTA exits
+      for (int q = issued > NS ? issued - NS : 0; q < issued; ++q)
+        ptx::mbar_wait_bounded(bar_full + 8 * (q % NS), (uint32_t)(q / NS) & 1u, kWaitLimitNs);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue

@@ -88,7 +88,7 @@ __device__ __forceinline__ int width(int rows) { return (rows + 31) & ~31; }
 
 template <bool W4, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<W4>::kThreads, 1)
-experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x64, const __grid_constant__ CUtensorMap tmap_x16,
+experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_xfull, const __grid_constant__ CUtensorMap tmap_x64, const __grid_constant__ CUtensorMap tmap_x16,
                     const __grid_constant__ CUtensorMap tmap_w, const Args args) {
   using C = Cfg<W4>;
   constexpr int kNS = C::kNS, kBN = C::kBN;
@@ -133,6 +133,7 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x64, const __grid_c
       ptx::mbar_init(bar_accfree + 8 * b, 2 * 4 * C::kGroups);   // one arrival per epilogue warp, both CTAs
     }
     ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmap_xfull);
     ptx::prefetch_tensormap(&tmap_x64);
     ptx::prefetch_tensormap(&tmap_x16);
     if (!W4) ptx::prefetch_tensormap(&tmap_w);
@@ -156,53 +157,61 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x64, const __grid_c
   const int items = row_tiles * args.n2_tiles;
 
   if (warp == 0 || warp == 2) {
-    // ------------------------------------------------------------------ producers (one thread each)
-    if (lane == 0) {
-      const bool weights = (warp == 0);
-      Ring<kNS> ring;
-      int issued = 0;
-      bool ok = true;
-      for (int i = pair; ok && i < items; i += args.pairs) {
-        const Tile t = tile_at(args, i, row_tiles);
-        const int nt = 2 * t.n2 + (int)rank;
-        const uint8_t* wsrc = W4 ? args.blob + ((size_t)t.expert * args.n_tiles + (nt < args.n_tiles ? nt : args.n_tiles - 1)) *
-                                                   (size_t)args.kt_total * kBlobTile : nullptr;
-        const int half = width(t.rows) / 2;
-        const int row0 = weights ? t.expert * args.N + nt * 128 : t.row0 + (int)rank * half;
-        for (int kt = 0; kt < args.kt_total; ++kt) {
-          if (!ptx::mbar_wait_bounded(bar_empty + 8 * ring.s, ring.ph ^ 1u, kWaitLimitNs)) {
-            atomicExch(args.status, 171);
-            ok = false;
-            break;
-          }
-          const uint32_t full = bar_full + 8 * ring.s;
-          if (weights) {
+    // ------------------------------------------------------------------ producers
+    // As with the MMAs the whole warp walks the loop and one elected lane issues: a loop that only thread 0 walks needed about
+    // 450 cycles to issue a k-step's copies, and the rings of the 4-bit kernel, whose k-step is 415 cycles of MMAs, ran dry.
+    const bool leader = ptx::elect_one();
+    const bool weights = (warp == 0);
+    Ring<kNS> ring;
+    int issued = 0;
+    bool ok = true;
+    for (int i = pair; ok && i < items; i += args.pairs) {
+      const Tile t = tile_at(args, i, row_tiles);
+      const int nt = 2 * t.n2 + (int)rank;
+      const uint8_t* wsrc = W4 ? args.blob + ((size_t)t.expert * args.n_tiles + (nt < args.n_tiles ? nt : args.n_tiles - 1)) *
+                                                 (size_t)args.kt_total * kBlobTile : nullptr;
+      const int half = width(t.rows) / 2;
+      const int row0 = weights ? t.expert * args.N + nt * 128 : t.row0 + (int)rank * half;
+      for (int kt = 0; kt < args.kt_total; ++kt) {
+        ok = ptx::mbar_wait_bounded(bar_empty + 8 * ring.s, ring.ph ^ 1u, kWaitLimitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (leader) atomicExch(args.status, 171);
+          break;
+        }
+        const uint32_t full = bar_full + 8 * ring.s;
+        if (weights) {
+          const uint32_t dst = ws + ring.s * C::kWStage;
+          if (leader) {
             ptx::mbar_expect_tx(full, C::kWStage);
-            if (W4) {
-              ptx::bulk_load(ws + ring.s * C::kWStage, wsrc, kBlobTile, full);
-              wsrc += kBlobTile;
-            } else {
-              ptx::tensor_load_2d(ws + ring.s * C::kWStage, &tmap_w, kt * 128, row0, full);
-            }
-          } else {
-            ptx::mbar_expect_tx(full, (uint32_t)half * 128u);
-            const uint32_t dst = xs + ring.s * C::kXStage;
-            int r = 0;
-            for (; r + 64 <= half; r += 64) ptx::tensor_load_2d(dst + r * 128, &tmap_x64, kt * 128, row0 + r, full);
-            for (; r < half; r += 16) ptx::tensor_load_2d(dst + r * 128, &tmap_x16, kt * 128, row0 + r, full);
+            if (W4) ptx::bulk_load(dst, wsrc, kBlobTile, full);
+            else ptx::tensor_load_2d(dst, &tmap_w, kt * 128, row0, full);
           }
-          ring.advance();
-          ++issued;
+          if (W4) wsrc += kBlobTile;
+        } else {
+          const uint32_t dst = xs + ring.s * C::kXStage;
+          if (leader) {
+            ptx::mbar_expect_tx(full, (uint32_t)half * 128u);
+            if (half == kBN / 2) {
+              ptx::tensor_load_2d(dst, &tmap_xfull, kt * 128, row0, full);
+            } else {
+              int r = 0;
+              for (; r + 64 <= half; r += 64) ptx::tensor_load_2d(dst + r * 128, &tmap_x64, kt * 128, row0 + r, full);
+              for (; r < half; r += 16) ptx::tensor_load_2d(dst + r * 128, &tmap_x16, kt * 128, row0 + r, full);
+            }
+          }
         }
+        ring.advance();
+        ++issued;
       }
-      if (!ok) {
-        // copies already issued still write shared memory: let them land before the CTA exits
-        Ring<kNS> back;
-        const int first = issued > kNS ? issued - kNS : 0;
-        for (int q = 0; q < issued; ++q) {
-          if (q >= first) ptx::mbar_wait_bounded(bar_full + 8 * back.s, back.ph, kWaitLimitNs);
-          back.advance();
-        }
+    }
+    if (!ok) {
+      // copies already issued still write shared memory: let them land before the CTA exits
+      Ring<kNS> back;
+      const int first = issued > kNS ? issued - kNS : 0;
+      for (int q = 0; q < issued; ++q) {
+        if (q >= first) ptx::mbar_wait_bounded(bar_full + 8 * back.s, back.ph, kWaitLimitNs);
+        back.advance();
       }
     }
   } else if (warp == 3) {
@@ -275,9 +284,9 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x64, const __grid_c
         accring.advance();
       }
     }
-  } else if (warp < 4 + 4 * C::kSets) {
+  } else if (W4 && warp >= 8 && warp < 8 + 4 * C::kSets) {
     // ------------------------------------------------------------------ unpacking (kSets sets, k-steps in turn)
-    const int my_set = (warp - 4) >> 2;
+    const int my_set = (warp - 8) >> 2;
     const int quad = warp & 3;               // TMEM lane quadrant this warp may access
     const int row = quad * 32 + lane;        // channel inside the CTA's block == TMEM lane
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
@@ -341,7 +350,7 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x64, const __grid_c
     }
   } else {
     // ------------------------------------------------------------------ epilogue (kGroups groups share every tile)
-    const int g = (warp - 4 - 4 * C::kSets) >> 2;
+    const int g = W4 ? (warp >= 8 ? 1 : 0) : (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
@@ -440,7 +449,8 @@ static int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
     }
     cap = v;
   }
-  CUtensorMap x64, x16, tw;
+  CUtensorMap xfull, x64, x16, tw;
+  if (int rc = make_byte_matrix_map(&xfull, p.x, p.rows, p.K, C::kBN / 2, 128)) return rc;
   if (int rc = make_byte_matrix_map(&x64, p.x, p.rows, p.K, 64, 128)) return rc;
   if (int rc = make_byte_matrix_map(&x16, p.x, p.rows, p.K, 16, 128)) return rc;
   if (W4) tw = x16;
@@ -465,7 +475,7 @@ static int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
   if (!a.status) return LQ_ERR_CUDA;
   const long items = max_tiles(p.rows, p.E, plan.bn) * a.n2_tiles;
   a.pairs = (int)(items < cap ? items : cap);
-  const cudaError_t e = launch_overlapped(kern, dim3(2 * a.pairs), dim3(C::kThreads), (size_t)C::kSmemBytes, st, x64, x16, tw, a);
+  const cudaError_t e = launch_overlapped(kern, dim3(2 * a.pairs), dim3(C::kThreads), (size_t)C::kSmemBytes, st, xfull, x64, x16, tw, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "experts_pair_kernel launch");
     return LQ_ERR_CUDA;
