@@ -7,9 +7,9 @@
 // item start while the sums of the last one are read out.  Item order: channel blocks fastest, so that the
 // CTAs at work at one time share a few row tiles, and the row tiles of one expert follow each other and find its weights in L2.
 //
-// A tile's width is what its rows need: the rows come in boxes of kBox rows, as many as cover the tile, and the MMA's N is
-// that many rows.  A box may reach past the last row of its expert: it then holds rows of the next expert (or, past the
-// end, zeros), whose sums are not stored.
+// A tile's width is what its rows need: the MMA's N is its rows in steps of 16 or 32, and the rows come in one box of BN or BN / 2
+// rows (one copy a k-step).  Rows of the box behind the tile's are those of the next expert, or zeros; their sums
+// are not stored.
 //
 // Per CTA: warp 0 = copies (8704-byte bulk copy of a blob tile, or a 128 x 128 box of INT8 weights; boxes of rows), warp 1 =
 // tensor-memory allocation and MMA issue; with 4-bit weights warps 2..5 and 6..9 = two sets that unpack alternate k-steps into
@@ -55,7 +55,7 @@ template <int BN, int NS, bool W4>
 struct Cfg {
   static constexpr int kGroups = W4 ? 1 : 2;                  // epilogue groups of four warps
   static constexpr int kThreads = 64 + 128 * ((W4 ? kSets : 0) + kGroups);
-  static constexpr int kBox = BN >= 64 ? 32 : 16;
+  static constexpr int kStep = BN >= 64 ? 32 : 16;            // of the MMA's N
   static constexpr int kXStage = BN * 128;
   static constexpr int kWStage = W4 ? kBlobTile : 128 * 128;
   static constexpr int kAcc = BN <= 64 || !W4 ? 2 : 1;        // accumulators
@@ -91,7 +91,8 @@ __device__ __forceinline__ Item item_at(const Args& a, int i) {
 
 template <int BN, int NS, bool W4, int MODE>
 __global__ void __launch_bounds__(Cfg<BN, NS, W4>::kThreads, 2)
-experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Args args) {
+experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_xhalf,
+               const __grid_constant__ CUtensorMap tmap_w, const Args args) {
   using C = Cfg<BN, NS, W4>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -128,6 +129,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tmap_x);
+    ptx::prefetch_tensormap(&tmap_xhalf);
     if (!W4) ptx::prefetch_tensormap(&tmap_w);
   }
   if (warp == 1) {
@@ -153,8 +155,8 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
       const Item it = item_at(args, i);
-      const int boxes = (it.rows + C::kBox - 1) / C::kBox;
-      const uint32_t tx = (uint32_t)(boxes * C::kBox * 128 + C::kWStage);
+      const bool few = it.rows <= BN / 2;
+      const uint32_t tx = (uint32_t)((few ? BN / 2 : BN) * 128 + C::kWStage);
       const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;
       const int wrow = W4 ? 0 : it.expert * args.N + it.nt * 128;
       for (int kt = it.kb; kt < it.ke; ++kt) {
@@ -170,7 +172,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           ptx::mbar_expect_tx(full, tx);
           if (W4) ptx::bulk_load(wdst, src, kBlobTile, full);
           else ptx::tensor_load_2d(wdst, &tmap_w, kt * 128, wrow, full);
-          for (int b = 0; b < boxes; ++b) ptx::tensor_load_2d(xdst + b * C::kBox * 128, &tmap_x, kt * 128, it.row0 + b * C::kBox, full);
+          ptx::tensor_load_2d(xdst, few ? &tmap_xhalf : &tmap_x, kt * 128, it.row0, full);
         }
         if (W4) src += kBlobTile;
         ring.advance();
@@ -192,7 +194,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
       const Item it = item_at(args, i);
-      const uint32_t idesc = ptx::idesc_i8((it.rows + C::kBox - 1) / C::kBox * C::kBox);
+      const uint32_t idesc = ptx::idesc_i8((it.rows + C::kStep - 1) / C::kStep * C::kStep);
       ok = ptx::mbar_wait_bounded(bar_accfree + 8 * accring.s, accring.ph ^ 1u, kWaitLimitNs);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
@@ -369,8 +371,9 @@ static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
     record_cuda_error(attr_err, "cudaFuncSetAttribute(experts_kernel)");
     return LQ_ERR_CUDA;
   }
-  CUtensorMap tx, tw;
-  if (int rc = make_byte_matrix_map(&tx, p.x, p.rows, p.K, C::kBox, 128)) return rc;
+  CUtensorMap tx, txh, tw;
+  if (int rc = make_byte_matrix_map(&tx, p.x, p.rows, p.K, BN, 128)) return rc;
+  if (int rc = make_byte_matrix_map(&txh, p.x, p.rows, p.K, BN / 2, 128)) return rc;
   if (W4) tw = tx;
   else if (int rc = make_byte_matrix_map(&tw, p.w, (long)p.E * p.N, p.K, 128, 128)) return rc;
   Args a;
@@ -394,7 +397,7 @@ static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
   const long items = max_tiles(p.rows, p.E, plan.bn) * a.n_tiles * a.splits;
   const long slots = 2L * sm_count();
   const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(C::kThreads),
-                                          (size_t)C::kSmemBytes, st, tx, tw, a);
+                                          (size_t)C::kSmemBytes, st, tx, txh, tw, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "experts_kernel launch");
     return LQ_ERR_CUDA;
