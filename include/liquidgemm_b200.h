@@ -344,7 +344,7 @@ LQ_API int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, i
  *   y[t] = sum_j weights[t, j] * (product of h with w2[e])  in float32, slot by slot, rounded once.
  * w13 [E, 2 I, H] holds gate channel c in row 2 c and up channel c in row 2 c + 1; w2 [E, H, I]; both in the form of
  * w_kind.  weights [T, topk] float32; an id outside [0, E) adds nothing.  H % 128 == 0 and I % 128 == 0, the other limits as
- * above; s13 and s2 16-byte aligned. */
+ * above; s13, s2 and y 16-byte aligned. */
 LQ_API size_t lq_experts_mlp_scratch_bytes(int T, int topk, int E, int H, int I, int w_kind);
 LQ_API int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32_t* ids, const void* w13,
                           const float* s13, const void* w2, const float* s2, int w_kind, void* y, int out_dtype, int T,

@@ -645,20 +645,24 @@ hidden_planes_kernel(const HiddenArgs a) {
   }
 }
 
-// The hidden values and their rows' maxima are there: codes only, 256 * NV 16-byte vectors of a row per CTA.
+// The hidden values and their rows' maxima are there: codes only.  A warp takes 32 * NV 16-byte vectors of a row, all of a
+// lane's in flight together.
+constexpr int kHiddenWarps = 8;
 template <int NV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(32 * kHiddenWarps)
 hidden_quant_kernel(const HiddenArgs a) {
   allow_dependents();
   dependency_wait();
-  const int pieces = (a.I / 4 + 256 * NV - 1) / (256 * NV);
-  const long p = blockIdx.x / pieces;
-  const int first = (int)(blockIdx.x - p * pieces) * 256 * NV + threadIdx.x;
+  const int pieces = (a.I / 4 + 32 * NV - 1) / (32 * NV);
+  const long task = (long)blockIdx.x * kHiddenWarps + (threadIdx.x >> 5);
+  const long p = task / pieces;
   if (p >= a.counts[1]) return;
-  const uint4* src = reinterpret_cast<const uint4*>(a.h + p * a.I);
+  const int first = (int)(task - p * pieces) * 32 * NV + (threadIdx.x & 31);
+  const float* src = a.h + p * a.I;
   uint4 raw[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) raw[i] = first + 256 * i < a.I / 4 ? ld_stream_v4(src + first + 256 * i) : make_uint4(0u, 0u, 0u, 0u);
+  for (int i = 0; i < NV; ++i)
+    raw[i] = first + 32 * i < a.I / 4 ? ld_stream_v4(src + 4 * (first + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
   const float scale = __fdiv_rn(fmaxf(__uint_as_float(a.amax[p]), 1e-12f), 127.0f);
   const float inv = __fdiv_rn(1.0f, scale);
   if (first == 0) a.hscale[p] = scale;
@@ -667,17 +671,19 @@ hidden_quant_kernel(const HiddenArgs a) {
   for (int i = 0; i < NV; ++i) {
     uint32_t out[1];
     quant_vec<float>(raw[i], scale, inv, out);
-    if (first + 256 * i < a.I / 4) dst[first + 256 * i] = out[0];
+    if (first + 32 * i < a.I / 4) dst[first + 32 * i] = out[0];
   }
 }
 
 static int run_hidden(const HiddenArgs& a, cudaStream_t st) {
-  // few rows are spread over many CTAs, many rows keep four loads of a thread in flight
-  const int nv = a.rows * (a.I / 4) > 4L * sm_count() * 2048 ? 4 : 1;
-  const long pieces = (a.I / 4 + 256 * nv - 1) / (256 * nv);
+  // few rows are spread over many warps, many rows keep eight loads of a lane in flight (13332 rows of 1792: 42 -> 22 us against
+  // CTAs of one row)
+  const int nv = a.rows * (a.I / 4) > 4L * sm_count() * 2048 ? 8 : 1;
+  const long tasks = a.rows * ((a.I / 4 + 32 * nv - 1) / (32 * nv));
+  const dim3 grid((unsigned)((tasks + kHiddenWarps - 1) / kHiddenWarps)), block(32 * kHiddenWarps);
   const cudaError_t e = a.planes  ? launch_overlapped(hidden_planes_kernel, dim3((unsigned)a.rows), dim3(512), 0, st, a)
-                        : nv == 4 ? launch_overlapped(hidden_quant_kernel<4>, dim3((unsigned)(a.rows * pieces)), dim3(256), 0, st, a)
-                                  : launch_overlapped(hidden_quant_kernel<1>, dim3((unsigned)(a.rows * pieces)), dim3(256), 0, st, a);
+                        : nv == 8 ? launch_overlapped(hidden_quant_kernel<8>, grid, block, 0, st, a)
+                                  : launch_overlapped(hidden_quant_kernel<1>, grid, block, 0, st, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "hidden rows launch");
     return LQ_ERR_CUDA;
@@ -700,30 +706,31 @@ struct CombineArgs {
   int N, topk, splits, out_dtype;
 };
 
-// y = sum_j weight_j * (sums * row scale * channel scale), the experts of a token in the order of their slots, in float32,
-// rounded once.  Bound by memory (4 bytes a sum in).  A thread makes IT times VEC neighbouring channels of one output
-// row; a CTA of 256 threads a row or, with IT = 1 (few rows), a piece of one.  The rows' places, scales and weights are
-// fetched by the lanes in parallel, and the sums of two slots (of one k-range) are requested together, so that a thread pays its
-// chain of small loads once for up to 128 bytes of sums: with 32 bytes behind the chain, 8192 tokens x 2 x 4096 took 135 us.
-template <int VEC>
-__device__ __forceinline__ void load_sums(const int32_t* src, int (&v)[VEC]) {
-  if constexpr (VEC == 4) {
-    const uint4 q = ld_stream_v4(src);
-    v[0] = (int)q.x; v[1] = (int)q.y; v[2] = (int)q.z; v[3] = (int)q.w;
+// Four neighbouring outputs, at an offset that is a multiple of four.
+__device__ __forceinline__ void store_out4(void* y, size_t at, const float (&v)[4], int out_dtype) {
+  if (out_dtype == LQ_DT_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(y) + at) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
-    v[0] = src[0];
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_out(h, i, v[i], out_dtype);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(y) + at) =
+        make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
   }
 }
 
-template <int VEC, int IT>
+// y = sum_j weight_j * (sums * row scale * channel scale), the experts of a token in the order of their slots, in float32,
+// rounded once: products whose k was cut (few rows).  A thread makes VEC neighbouring channels; the rows' places, scales
+// and weights are fetched by the lanes in parallel.
+template <int VEC>
 __global__ void __launch_bounds__(256)
 combine_kernel(const CombineArgs a) {
   allow_dependents();
   dependency_wait();
   const int lane = threadIdx.x & 31;
-  const int pieces = (a.N + 256 * VEC * IT - 1) / (256 * VEC * IT);
+  const int pieces = (a.N + 256 * VEC - 1) / (256 * VEC);
   const long m = blockIdx.x / pieces;
-  const int c0 = ((int)(blockIdx.x - m * pieces) * 256 * IT + threadIdx.x) * VEC;
+  const int c = ((int)(blockIdx.x - m * pieces) * 256 + threadIdx.x) * VEC;
   const int slots = a.weights ? a.topk : 1;
   // lane j: slot j of the row
   int my_p = -1, my_e = 0;
@@ -734,83 +741,122 @@ combine_kernel(const CombineArgs a) {
     if (a.weights) my_w = a.weights[m * slots + lane];
     if (my_p >= 0) my_scale = a.ascale[my_p];
   }
-  float sum[IT][VEC];
+  const bool in = c < a.N;   // the warp stays together for the shuffles
+  float sum[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+  for (int j = 0; j < slots; ++j) {
+    const int p = __shfl_sync(0xffffffffu, my_p, j), e = __shfl_sync(0xffffffffu, my_e, j);
+    const float as = __shfl_sync(0xffffffffu, my_scale, j), w = __shfl_sync(0xffffffffu, my_w, j);
+    if (p < 0 || !in) continue;
+    const float* s1 = a.s1 + (size_t)e * a.N + c;
+    float f[VEC];
+    int v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      f[i] = s1[i];
+      v[i] = 0;
+    }
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+      const int32_t* src = a.planes + ((size_t)s * a.rows + p) * a.N + c;
+      if constexpr (VEC == 4) {
+        const uint4 q = ld_stream_v4(src);
+        v[0] += (int)q.x; v[1] += (int)q.y; v[2] += (int)q.z; v[3] += (int)q.w;
+      } else {
+        v[0] += src[0];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float o = lqq_scale(v[i], as, f[i]);
+      sum[i] = a.weights ? __fmaf_rn(w, o, sum[i]) : o;
+    }
+  }
+  if (!in) return;
+  if constexpr (VEC == 4) store_out4(a.y, (size_t)m * a.N + c, sum, a.out_dtype);
+  else store_out(a.y, (size_t)m * a.N + c, sum[0], a.out_dtype);
+}
+
+// The same weighted sum where the product wrote scaled rows in float32, one per pair in the tokens' order: the addresses
+// are known at once, so all loads of a thread (four slots of IT * 4 channels) are in flight together; rows of pairs without an expert
+// hold anything and are not used.  Bound by memory.  (From int32 sums in sorted order, each behind its pair's place, its row's scale
+// and the channels' scales, which are as many bytes again out of L2: 8192 tokens x 2 x 4096 115 -> 60 us, 3333 x 4 x 4096
+// 75 -> 43.)
+template <int IT>
+__global__ void __launch_bounds__(256)
+weighted_sum_kernel(const float* rows, const float* weights, const int* ids, void* y, int E, int N, int topk, int out_dtype) {
+  allow_dependents();
+  dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int pieces = (N + 1024 * IT - 1) / (1024 * IT);
+  const long m = blockIdx.x / pieces;
+  const int c0 = ((int)(blockIdx.x - m * pieces) * 256 * IT + threadIdx.x) * 4;
+  int my_e = -1;
+  float my_w = 0.f;
+  if (lane < topk) {
+    my_e = ids[m * topk + lane];
+    my_w = weights[m * topk + lane];
+  }
+  float sum[IT][4];
 #pragma unroll
   for (int t = 0; t < IT; ++t)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[t][i] = 0.f;
-  constexpr int kBatch = 2;
-  for (int j0 = 0; j0 < slots; j0 += kBatch) {
-    int q[kBatch][IT][VEC];
-    int p[kBatch];
+    for (int i = 0; i < 4; ++i) sum[t][i] = 0.f;
+  constexpr int kBatch = 4;
+  for (int j0 = 0; j0 < topk; j0 += kBatch) {
+    uint4 q[kBatch][IT];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      p[b] = __shfl_sync(0xffffffffu, my_p, (j0 + b) & 31);
-      if (j0 + b >= slots) p[b] = -1;
+    for (int b = 0; b < kBatch; ++b)
 #pragma unroll
-      for (int t = 0; t < IT; ++t) {
-        const int c = c0 + t * 256 * VEC;
-        if (p[b] >= 0 && c < a.N) load_sums<VEC>(a.planes + (size_t)p[b] * a.N + c, q[b][t]);
-      }
-    }
+      for (int t = 0; t < IT; ++t)
+        if (j0 + b < topk && c0 + 1024 * t < N) q[b][t] = ld_stream_v4(rows + (size_t)(m * topk + j0 + b) * N + c0 + 1024 * t);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int e = __shfl_sync(0xffffffffu, my_e, (j0 + b) & 31);
-      const float as = __shfl_sync(0xffffffffu, my_scale, (j0 + b) & 31), w = __shfl_sync(0xffffffffu, my_w, (j0 + b) & 31);
-      if (p[b] < 0) continue;   // (the whole warp)
+      const float w = __shfl_sync(0xffffffffu, my_w, (j0 + b) & 31);
+      if (j0 + b >= topk || e < 0 || e >= E) continue;   // (the whole warp)
 #pragma unroll
       for (int t = 0; t < IT; ++t) {
-        const int c = c0 + t * 256 * VEC;
-        if (c >= a.N) continue;
-        for (int s = 1; s < a.splits; ++s) {
-          int more[VEC];
-          load_sums<VEC>(a.planes + ((size_t)s * a.rows + p[b]) * a.N + c, more);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) q[b][t][i] += more[i];
-        }
-        const float* s1 = a.s1 + (size_t)e * a.N + c;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float o = lqq_scale(q[b][t][i], as, s1[i]);
-          sum[t][i] = a.weights ? __fmaf_rn(w, o, sum[t][i]) : o;
-        }
+        if (c0 + 1024 * t >= N) continue;
+        sum[t][0] = __fmaf_rn(w, __uint_as_float(q[b][t].x), sum[t][0]);
+        sum[t][1] = __fmaf_rn(w, __uint_as_float(q[b][t].y), sum[t][1]);
+        sum[t][2] = __fmaf_rn(w, __uint_as_float(q[b][t].z), sum[t][2]);
+        sum[t][3] = __fmaf_rn(w, __uint_as_float(q[b][t].w), sum[t][3]);
       }
     }
   }
 #pragma unroll
-  for (int t = 0; t < IT; ++t) {
-    const int c = c0 + t * 256 * VEC;
-    if (c >= a.N) continue;
-    const size_t at = (size_t)m * a.N + c;
-    if constexpr (VEC == 4) {
-      if (a.out_dtype == LQ_DT_F32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(sum[t][0], sum[t][1], sum[t][2], sum[t][3]);
-      } else {
-        uint16_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) store_out(h, i, sum[t][i], a.out_dtype);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) =
-            make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
-      }
-    } else {
-      store_out(a.y, at, sum[t][0], a.out_dtype);
-    }
-  }
+  for (int t = 0; t < IT; ++t)
+    if (c0 + 1024 * t < N) store_out4(y, (size_t)m * N + c0 + 1024 * t, sum[t], out_dtype);
 }
 
 static int run_combine(const CombineArgs& a, cudaStream_t st) {
   const bool vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
-  const bool many = vec && a.N > 1024 && a.outs * (a.N / 1024) > 16L * sm_count();
-  const long pieces = (a.N + (many ? 4096 : vec ? 1024 : 256) - 1) / (many ? 4096 : vec ? 1024 : 256);
-  const dim3 grid((unsigned)(a.outs * pieces));
-  const cudaError_t e = many  ? launch_overlapped(combine_kernel<4, 4>, grid, dim3(256), 0, st, a)
-                        : vec ? launch_overlapped(combine_kernel<4, 1>, grid, dim3(256), 0, st, a)
-                              : launch_overlapped(combine_kernel<1, 1>, grid, dim3(256), 0, st, a);
+  const int piece = vec ? 1024 : 256;
+  const dim3 grid((unsigned)(a.outs * ((a.N + piece - 1) / piece)));
+  const cudaError_t e = vec ? launch_overlapped(combine_kernel<4>, grid, dim3(256), 0, st, a)
+                            : launch_overlapped(combine_kernel<1>, grid, dim3(256), 0, st, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "combine_kernel launch");
     return LQ_ERR_CUDA;
   }
   return check_launch("combine_kernel");
+}
+
+// N a multiple of 4; rows and y 16-byte aligned.
+static int run_weighted_sum(const float* rows, const float* weights, const int* ids, void* y, long T, int E, int N, int topk,
+                            int out_dtype, cudaStream_t st) {
+  const bool many = N > 1024 && T * (N / 1024) > 16L * sm_count();
+  const int piece = many ? 2048 : 1024;
+  const dim3 grid((unsigned)(T * ((N + piece - 1) / piece)));
+  const cudaError_t e = many ? launch_overlapped(weighted_sum_kernel<2>, grid, dim3(256), 0, st, rows, weights, ids, y, E, N, topk, out_dtype)
+                             : launch_overlapped(weighted_sum_kernel<1>, grid, dim3(256), 0, st, rows, weights, ids, y, E, N, topk, out_dtype);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "weighted_sum_kernel launch");
+    return LQ_ERR_CUDA;
+  }
+  return check_launch("weighted_sum_kernel");
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1027,7 +1073,7 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   if (I > (1 << 29)) return LQ_ERR_SHAPE;
   if (int rc = check_sizes(T, topk, E, 2 * I, H)) return rc;
   if (int rc = check_sizes(T, topk, E, H, I)) return rc;
-  if (misaligned(x) || misaligned(w13) || misaligned(w2) || misaligned(s13) || misaligned(s2)) return LQ_ERR_SHAPE;
+  if (misaligned(x) || misaligned(w13) || misaligned(w2) || misaligned(s13) || misaligned(s2) || misaligned(y)) return LQ_ERR_SHAPE;
   Carver c(scratch);
   const long pairs = (long)T * topk;
   const MlpBuffers b = carve_mlp(c, pairs, E, H, I, w_kind);
@@ -1078,6 +1124,14 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   p.N = H;
   p.K = I;
   p.splits = b.splits2;
+  if (b.splits2 == 1) {
+    // whole k-ranges: scaled rows in the tokens' order, in the bytes of one plane
+    p.out_mode = kOutPairs;
+    p.out_dtype = LQ_DT_F32;
+    p.out = b.planes2;
+    if (int rc = run_product(p, b.plan, st)) return rc;
+    return run_weighted_sum(reinterpret_cast<const float*>(b.planes2), weights, ids, y, T, E, H, topk, out_dtype, st);
+  }
   p.out_mode = kOutPlanes;
   p.out = b.planes2;
   if (int rc = run_product(p, b.plan, st)) return rc;

@@ -67,7 +67,8 @@ def test_mlp_bad_arguments(change):
 
 
 @pytest.mark.parametrize("change", [dict(H=200), dict(inner=192), dict(topk=33), dict(E=513), dict(T=1 << 24), dict(inner=1 << 30),
-                                    dict(x=P + 8), dict(w13=P + 8), dict(w2=P + 8), dict(s13=P + 4), dict(s2=P + 4)])
+                                    dict(x=P + 8), dict(w13=P + 8), dict(w2=P + 8), dict(s13=P + 4), dict(s2=P + 4),
+                                    dict(y=P + 8)])
 def test_mlp_bad_shapes(change):
     assert _mlp(**change) == SHAPE
 
