@@ -73,14 +73,11 @@ struct Cfg {
 struct Item {
   int expert, row0, rows, nt, s, kb, ke;
 };
-__device__ __forceinline__ Item item_at(const Args& a, int i) {
+__device__ __forceinline__ Item item_of(const Args& a, int i, const int4& tile) {
   Item it;
-  const int per_tile = a.n_tiles * a.splits;
-  const int t = i / per_tile;
-  const int in = i - t * per_tile;
+  const int in = i % (a.n_tiles * a.splits);
   it.s = in / a.n_tiles;
   it.nt = in - it.s * a.n_tiles;
-  const int4 tile = __ldcg(a.tiles + t);
   it.expert = tile.x;
   it.row0 = tile.y;
   it.rows = tile.z;
@@ -88,6 +85,8 @@ __device__ __forceinline__ Item item_at(const Args& a, int i) {
   it.ke = ((it.s + 1) * a.kt_total) / a.splits;
   return it;
 }
+__device__ __forceinline__ int4 tile_of(const Args& a, int i) { return __ldcg(a.tiles + i / (a.n_tiles * a.splits)); }
+__device__ __forceinline__ Item item_at(const Args& a, int i) { return item_of(a, i, tile_of(a, i)); }
 
 template <int BN, int NS, bool W4, int MODE>
 __global__ void __launch_bounds__(Cfg<BN, NS, W4>::kThreads, 2)
@@ -143,6 +142,10 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   dependency_wait();   // the plan, the rows and the buffers written here belong to earlier kernels until now
   const uint32_t tmem_acc = *tmem_slot_p;
   const uint32_t tmem_a = tmem_acc + C::kAcc * BN;
+  // The first tile's entry is requested together with the number of tiles: the table has room for every tile that a launch of
+  // this grid can have, so an entry that is not there is read as anything and not used.
+  int4 tile = make_int4(0, 0, 0, 0);
+  if (warp == 0) tile = tile_of(args, blockIdx.x);
   const int items = __ldcg(args.counts) * args.n_tiles * args.splits;
 
   if (warp == 0) {
@@ -154,7 +157,8 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     int issued = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, i);
+      if (i != (int)blockIdx.x) tile = tile_of(args, i);
+      const Item it = item_of(args, i, tile);
       const bool few = it.rows <= BN / 2;
       const uint32_t tx = (uint32_t)((few ? BN / 2 : BN) * 128 + C::kWStage);
       const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;

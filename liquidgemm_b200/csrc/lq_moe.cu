@@ -656,14 +656,16 @@ hidden_quant_kernel(const HiddenArgs a) {
   const int pieces = (a.I / 4 + 32 * NV - 1) / (32 * NV);
   const long task = (long)blockIdx.x * kHiddenWarps + (threadIdx.x >> 5);
   const long p = task / pieces;
-  if (p >= a.counts[1]) return;
+  if (p >= a.rows) return;
   const int first = (int)(task - p * pieces) * 32 * NV + (threadIdx.x & 31);
   const float* src = a.h + p * a.I;
   uint4 raw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     raw[i] = first + 32 * i < a.I / 4 ? ld_stream_v4(src + 4 * (first + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
-  const float scale = __fdiv_rn(fmaxf(__uint_as_float(a.amax[p]), 1e-12f), 127.0f);
+  const unsigned amax = a.amax[p];
+  if (p >= a.counts[1]) return;   // (rows behind the last: requested like the others, so that no load waits for another)
+  const float scale = __fdiv_rn(fmaxf(__uint_as_float(amax), 1e-12f), 127.0f);
   const float inv = __fdiv_rn(1.0f, scale);
   if (first == 0) a.hscale[p] = scale;
   uint32_t* dst = reinterpret_cast<uint32_t*>(a.hq + p * a.I);
