@@ -18,28 +18,54 @@ namespace experts {
 // sigmoid(l).  Key: the logit itself without a bias (scores rise with it, and it is exact), else s + bias.  Groups of E / G
 // neighbouring experts are ranked by their largest key or by the sum of their two largest keys (without a bias: scores), and
 // only experts of the best groups stay.  Then `topk` times the largest key, the lowest index among equals.
-// Where scores decide what is chosen (keys with a bias, sums of two) they are worked out in float64: neighbouring keys may
-// lie closer than a float32 exponential's error, and a choice is a whole number.
 // A logit of -inf or NaN, or a bias that makes a key so, takes its expert out.
 //
-// Bound by instruction issue (a token's row is a few hundred bytes).  A choice is one 32-bit warp reduction over the keys'
-// upper halves and a ballot; the lower halves and the indices are compared only where several lanes hold the same upper half.
-// Groups are ranked from shared memory, 32 / G lanes to a group.  (A warp reduction of the 64-bit key for every group and
-// choice, as in the first form: 8192 tokens, 192 experts in 8 groups, 64 us.)
+// Where scores decide what is chosen (a bias, sums of two), neighbouring keys may lie closer than a float32 exponential's error, and
+// a choice is a whole number.  The choice is made in float32 first; a token where two numbers whose order matters are closer than
+// their errors together (about one in a thousand) is done again in float64.
+//
+// Bound by instruction issue (a token's row is a few hundred bytes).  A choice is one 32-bit warp reduction, of 16-bit logits with the
+// expert's index below them, or two, of the key and of the index; all lanes do the same throughout (the owner of a choice
+// looking for its next best alone, and handing its score out by shuffles, took as long as all the rest).
+// Groups are ranked from shared memory, 32 / G lanes to a group.  8192 tokens, 192 experts in 8 groups, sigmoid, bias: 64 us with
+// a reduction of the 64-bit key for every group and choice, 22 with all of it in float64, 19 now (without a bias and in one group 8).
 
 // Orders numbers like unsigned integers; every number's image is above 0, which stands for "not to be chosen".
 __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);   // -0 becomes 0: equal keys are equal bits
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float number(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ unsigned long long ordered(double v) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
   return u ^ ((u >> 63) ? 0xffffffffffffffffull : 0x8000000000000000ull);
 }
-__device__ __forceinline__ uint32_t upper(uint32_t k) { return k; }
-__device__ __forceinline__ uint32_t upper(unsigned long long k) { return (uint32_t)(k >> 32); }
-__device__ __forceinline__ uint32_t lower(uint32_t) { return 0u; }
-__device__ __forceinline__ uint32_t lower(unsigned long long k) { return (uint32_t)k; }
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return ((unsigned long long)hi << 32) | lo;
+}
+template <typename S> struct KeyOf;
+template <> struct KeyOf<float> { using type = uint32_t; };
+template <> struct KeyOf<double> { using type = unsigned long long; };
+
+// The upper 16 bits of a number that a 16-bit type holds, ordered like its 32-bit image.
+template <typename T> __device__ __forceinline__ uint32_t ordered16(float v);
+template <> __device__ __forceinline__ uint32_t ordered16<__nv_bfloat16>(float v) { return ordered(v) & 0xffff0000u; }
+template <> __device__ __forceinline__ uint32_t ordered16<__half>(float v) {
+  const uint32_t u = __half_as_ushort(__float2half_rn(v + 0.0f));   // exact: v came from a half
+  return (u ^ ((u & 0x8000u) ? 0xffffu : 0x8000u)) << 16;
+}
+template <typename T> __device__ __forceinline__ float number16(uint32_t k);
+template <> __device__ __forceinline__ float number16<__nv_bfloat16>(uint32_t k) {
+  // (the image of a negative number has ones below, which its upper half lost)
+  return number((k >> 31) ? (k & 0xffff0000u) : (k | 0xffffu));
+}
+template <> __device__ __forceinline__ float number16<__half>(uint32_t k) {
+  const uint32_t u = k >> 16;
+  return __half2float(__ushort_as_half((unsigned short)(u ^ ((u & 0x8000u) ? 0x8000u : 0xffffu))));
+}
 
 struct RouteArgs {
   const void* logits;
@@ -51,23 +77,70 @@ struct RouteArgs {
   bool sigmoid, top2, renormalize;
 };
 
-template <typename S> struct KeyOf;
-template <> struct KeyOf<float> { using type = uint32_t; };
-template <> struct KeyOf<double> { using type = unsigned long long; };
-
 constexpr int kRouteWarps = 4;
+constexpr float kNone = -INFINITY;
 
-// Which groups stay: true for the groups of the topk_group highest ranks, the lowest index among equals.  `v` [E]: what the
-// groups are ranked by, -inf where an expert cannot be chosen; `rank` [n_group] and `kept` [n_group] are this warp's.
+// The logits of the warp's token; -inf for what cannot be chosen.
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(const RouteArgs& a, long t, float (&l)[PER]) {
+  const T* row = static_cast<const T*>(a.logits) + t * a.E;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    l[i] = e < a.E ? to_f32<T>(row[e]) : kNone;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (!(l[i] > kNone)) l[i] = kNone;   // NaN too
+}
+
+// exp(l - top) of every expert (1 where equal: also where both are infinite) and their sum.
+template <int PER, typename S>
+__device__ __forceinline__ S softmax_terms(const float (&l)[PER], float& top, S (&s)[PER]) {
+  top = kNone;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) top = fmaxf(top, l[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  S sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    s[i] = !(l[i] > kNone) ? (S)0 : l[i] == top ? (S)1 : exp((S)l[i] - (S)top);
+    sum += s[i];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum > 0 ? sum : (S)1;
+}
+
+// Lane j has choice j (id -1: none left) and its score.
+__device__ __forceinline__ void store_choice(const RouteArgs& a, long t, int id, double score) {
+  const int lane = threadIdx.x & 31;
+  if (id < 0) score = 0;
+  if (a.renormalize) {
+    double total = score;
+    for (int o = 1; o < a.topk; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);   // (lanes behind the last slot hold 0)
+    if (total > 0) score = score / total;
+  }
+  if (lane < a.topk) {
+    a.weights[t * a.topk + lane] = (float)(score * (double)a.scale);
+    a.ids[t * a.topk + lane] = id;
+  }
+}
+
+// Which groups stay: those of the topk_group highest ranks, the lowest index among equals.  `v` [E]: what the groups are ranked by,
+// -inf where an expert cannot be chosen; `rank` [n_group] and `kept` [n_group] are this warp's.  False where two ranks are closer than
+// `near`.
 template <typename S>
-__device__ __forceinline__ void rank_groups(const RouteArgs& a, const S* v, S* rank, uint8_t* kept) {
+__device__ __forceinline__ bool rank_groups(const RouteArgs& a, bool top2, const S* v, S* rank, uint8_t* kept, S near) {
   const int lane = threadIdx.x & 31;
   const int G = a.n_group, size = a.E / G;
   int L = 1;   // lanes of a group
   while (2 * L * G <= 32) L *= 2;
   for (int base = 0; base < G; base += 32 / L) {
     const int g = base + lane / L;
-    S m1 = -INFINITY, m2 = -INFINITY;
+    S m1 = kNone, m2 = kNone;
     if (g < G) {
       for (int e = lane & (L - 1); e < size; e += L) {
         const S x = v[g * size + e];
@@ -82,146 +155,241 @@ __device__ __forceinline__ void rank_groups(const RouteArgs& a, const S* v, S* r
       m2 = least > m2 ? least : m2;
       m1 = m1 > b1 ? m1 : b1;
     }
-    if (g < G && (lane & (L - 1)) == 0) rank[g] = a.top2 && m2 > (S)-INFINITY ? m1 + m2 : m1;
+    if (g < G && (lane & (L - 1)) == 0) rank[g] = top2 && m2 > (S)kNone ? m1 + m2 : m1;
   }
   __syncwarp();
+  bool clear = true;
   for (int g = lane; g < G; g += 32) {
     const S mine = rank[g];
     int before = 0;
-    for (int o = 0; o < G; ++o) before += (rank[o] > mine || (rank[o] == mine && o < g)) ? 1 : 0;
+    for (int o = 0; o < G; ++o) {
+      const S other = rank[o];
+      before += (other > mine || (other == mine && o < g)) ? 1 : 0;
+      if (o != g && fabs(other - mine) <= near) clear = false;   // (-inf against -inf is NaN: clear)
+    }
     kept[g] = before < a.topk_group;
   }
   __syncwarp();
+  return __all_sync(0xffffffffu, clear);
+}
+// e / size for e < 512
+__device__ __forceinline__ unsigned group_of(const RouteArgs& a, unsigned e) {
+  const unsigned size = a.E / a.n_group, inv = ((1u << 20) + size - 1) / size;
+  return e * inv >> 20;
 }
 
-// S: the type of the scores (and with a bias of the keys).
-template <typename T, int PER, typename S>
+// Choice by logits: no bias, groups by their largest.
+template <typename T, int PER>
 __global__ void __launch_bounds__(32 * kRouteWarps)
-route_kernel(const RouteArgs a) {
-  using Key = typename KeyOf<S>::type;
-  __shared__ S values[kRouteWarps][PER * 32];
-  __shared__ S ranks[kRouteWarps][PER * 32];
+route_logits_kernel(const RouteArgs a) {
+  __shared__ float values[kRouteWarps][PER * 32], ranks[kRouteWarps][PER * 32];
   __shared__ uint8_t kept[kRouteWarps][PER * 32];
   allow_dependents();
   dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long t = (long)blockIdx.x * kRouteWarps + warp;
   if (t >= a.T) return;
-  const T* row = static_cast<const T*>(a.logits) + t * a.E;
-  const float none = -INFINITY;
+  constexpr bool k16 = sizeof(T) == 2;
   float l[PER];
-  float top = none;
+  load_logits<T, PER>(a, t, l);
+  uint32_t key[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int e = lane + 32 * i;
-    l[i] = e < a.E ? to_f32<T>(row[e]) : none;
-    if (!(l[i] > none)) l[i] = none;   // NaN too
-    top = fmaxf(top, l[i]);
-  }
-
-  S s[PER];
-  if (a.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = l[i] > none ? (S)1 / ((S)1 + exp(-(S)l[i])) : (S)0;
-  } else {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    S sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      s[i] = !(l[i] > none) ? (S)0 : l[i] == top ? (S)1 : exp((S)l[i] - (S)top);   // (equal to the largest: also where that is infinite)
-      sum += s[i];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const S d = sum > 0 ? sum : (S)1;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = s[i] / d;
-  }
-
-  const bool by_score = a.bias != nullptr;
-  Key key[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane + 32 * i;
-    S v = (S)none;
-    if (l[i] > none) v = by_score ? s[i] + (S)a.bias[e] : (S)l[i];
-    const bool can = v > (S)none;   // (false for NaN)
-    key[i] = can ? ordered(v) : 0;
-    if (a.n_group > 1) values[warp][e] = !can ? (S)none : a.top2 && !by_score ? s[i] : v;
+    if constexpr (k16) key[i] = l[i] > kNone ? ordered16<T>(l[i]) | (0xffffu - e) : 0u;
+    else key[i] = l[i] > kNone ? ordered(l[i]) : 0u;
+    if (a.n_group > 1) values[warp][e] = l[i];
   }
   if (a.n_group > 1) {
     __syncwarp();
-    rank_groups<S>(a, values[warp], ranks[warp], kept[warp]);
-    const unsigned size = a.E / a.n_group, inv = ((1u << 20) + size - 1) / size;   // e / size for e < 512
+    rank_groups<float>(a, false, values[warp], ranks[warp], kept[warp], -1.f);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const unsigned e = lane + 32 * i;
-      if (e < a.E && !kept[warp][e * inv >> 20]) key[i] = 0;
+      if (e < a.E && !kept[warp][group_of(a, e)]) key[i] = 0;
     }
   }
-
-  // lane j ends up with choice j
   int my_id = -1;
-  S my_w = 0;
-  Key mine = 0;
-  int at = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (key[i] > mine) mine = key[i], at = i;
+  float my_l = 0.f;
   for (int j = 0; j < a.topk; ++j) {
-    const uint32_t best = __reduce_max_sync(0xffffffffu, upper(mine));
-    if (best == 0) break;   // (no key's upper half is 0)
-    unsigned who = __ballot_sync(0xffffffffu, upper(mine) == best);
-    if (who & (who - 1)) {   // several lanes: the lower halves, then the index
-      const bool in = upper(mine) == best;
-      const uint32_t low = __reduce_max_sync(0xffffffffu, in ? lower(mine) : 0u);
-      const unsigned first = __reduce_min_sync(0xffffffffu, in && lower(mine) == low ? (unsigned)(lane + 32 * at) : 1u << 20);
-      who = 1u << (first & 31);
-    }
-    const int owner = __ffs(who) - 1;
-    const int id = __shfl_sync(0xffffffffu, lane + 32 * at, owner);
-    S w = 0;
-    if (lane == owner) {
-      mine = 0;
-      const int gone = at;
+    uint32_t mine = key[0];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (i == gone) key[i] = 0, w = s[i];
-        if (key[i] > mine) mine = key[i], at = i;
-      }
-    }
-    w = __shfl_sync(0xffffffffu, w, owner);
-    if (lane == j) my_id = id, my_w = w;
-  }
-  if (a.renormalize) {
-    S total = my_w;
+    for (int i = 1; i < PER; ++i) mine = max(mine, key[i]);
+    const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
+    if (best == 0) break;
+    int id;
+    if constexpr (k16) {
+      id = (int)(0xffffu - (best & 0xffffu));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (total > 0) my_w = my_w / total;
+      for (int i = 0; i < PER; ++i)
+        if (key[i] == best) key[i] = 0;
+    } else {
+      unsigned at = 1u << 20;
+#pragma unroll
+      for (int i = PER - 1; i >= 0; --i)
+        if (key[i] == best) at = lane + 32 * i;
+      id = (int)__reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (id == lane + 32 * i) key[i] = 0;
+    }
+    if (lane == j) {
+      my_id = id;
+      if constexpr (k16) my_l = number16<T>(best);
+      else my_l = number(best);
+    }
   }
-  if (lane < a.topk) {
-    a.weights[t * a.topk + lane] = (float)(my_w * (S)a.scale);
-    a.ids[t * a.topk + lane] = my_id;
+  double score;
+  if (a.sigmoid) {
+    score = 1.0 / (1.0 + exp(-(double)my_l));
+  } else {
+    float top, s[PER];
+    const float sum = softmax_terms<PER, float>(l, top, s);
+    score = (double)(my_l == top ? 1.f : expf(my_l - top)) / (double)sum;
   }
+  store_choice(a, t, my_id, score);
 }
 
-template <typename T, typename S>
+// The warp's buffers of the kernel below.
+template <int PER>
+struct RouteBuffers {
+  double values[PER * 32], ranks[PER * 32];
+  uint8_t kept[PER * 32];
+};
+
+// Choice by scores.  False where the order of numbers that matters is not certain (float32 only).
+// Errors of float32: a sigmoid is off by 6 * 2^-24 at most (exponential 2 units times e / (1 + e)^2, sum, quotient 2 units; 2^-21 is
+// used), a softmax score by 31 * 2^-24 (argument |x| e^x < 0.4, exponential 2 units, sum of 16 terms and over 32 lanes, quotient;
+// 2^-18 is used), the key by another |v| 2^-24; two keys by twice that, two sums of two by four times.
+template <int PER, typename S>
+__device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float (&l)[PER], RouteBuffers<PER>& buf, int& my_id, double& my_s) {
+  using Key = typename KeyOf<S>::type;
+  constexpr bool kFast = sizeof(S) == 4;
+  const int lane = threadIdx.x & 31;
+  const bool by_score = a.bias != nullptr;
+  S* values = reinterpret_cast<S*>(buf.values);
+  S s[PER];
+  if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if constexpr (kFast) s[i] = l[i] > kNone ? __fdividef(1.f, 1.f + expf(-l[i])) : 0.f;
+      else s[i] = l[i] > kNone ? 1.0 / (1.0 + exp(-(double)l[i])) : 0.0;
+    }
+  } else {
+    float top;
+    const S sum = softmax_terms<PER, S>(l, top, s);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = s[i] / sum;
+  }
+  Key key[PER];
+  S largest = 1;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    S v = (S)kNone;
+    if (l[i] > kNone) v = by_score ? s[i] + (S)a.bias[e] : (S)l[i];
+    const bool can = v > (S)kNone;   // (false for NaN)
+    key[i] = can ? ordered(v) : 0;
+    if (kFast && by_score && can) largest = fabs(v) > largest ? fabs(v) : largest;
+    if (a.n_group > 1) values[e] = !can ? (S)kNone : a.top2 && !by_score ? s[i] : v;
+  }
+  S near = (S)-1;
+  if (kFast) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const S other = __shfl_xor_sync(0xffffffffu, largest, o);
+      largest = other > largest ? other : largest;
+    }
+    near = (S)2 * ((a.sigmoid ? (S)0x1p-21f : (S)0x1p-18f) + largest * (S)0x1p-24f);
+  }
+  if (a.n_group > 1) {
+    __syncwarp();
+    const bool ranked_by_score = by_score || a.top2;
+    if (!rank_groups<S>(a, a.top2, values, reinterpret_cast<S*>(buf.ranks), buf.kept, ranked_by_score ? (S)2 * near : (S)-1)) return false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const unsigned e = lane + 32 * i;
+      if (e < a.E && !buf.kept[group_of(a, e)]) key[i] = 0;
+    }
+  }
+  // what the chosen ones' scores are taken from: the logit (a sigmoid is worked out again, in float64, a lane each) or the score
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) values[lane + 32 * i] = a.sigmoid ? (S)l[i] : s[i];
+  __syncwarp();
+  uint32_t last = 0;   // the choice before
+  const bool check = kFast && by_score;
+  for (int j = 0; j < a.topk + (check ? 1 : 0); ++j) {   // the first that is not chosen is looked at too
+    Key mine = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) mine = key[i] > mine ? key[i] : mine;
+    const Key best = warp_max(mine);
+    if (best == 0) break;
+    if constexpr (kFast) {
+      if (check && j > 0 && number(last) - number(best) <= near) return false;
+      last = best;
+    }
+    if (j == a.topk) break;
+    unsigned at = 1u << 20;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i)
+      if (key[i] == best) at = lane + 32 * i;
+    const int id = (int)__reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (id == lane + 32 * i) key[i] = 0;
+    if (lane == j) my_id = id;
+  }
+  if (my_id >= 0) {
+    my_s = (double)values[my_id];
+    if (a.sigmoid) my_s = 1.0 / (1.0 + exp(-my_s));
+  }
+  return true;
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(32 * kRouteWarps)
+route_scores_kernel(const RouteArgs a) {
+  __shared__ RouteBuffers<PER> buffers[kRouteWarps];
+  allow_dependents();
+  dependency_wait();
+  const int warp = threadIdx.x >> 5;
+  const long t = (long)blockIdx.x * kRouteWarps + warp;
+  if (t >= a.T) return;
+  float l[PER];
+  load_logits<T, PER>(a, t, l);
+  int id = -1;
+  double score = 0;
+  if (!choose_by_score<PER, float>(a, l, buffers[warp], id, score)) {
+    __syncwarp();
+    id = -1;
+    score = 0;
+    choose_by_score<PER, double>(a, l, buffers[warp], id, score);
+  }
+  store_choice(a, t, id, score);
+}
+
+template <typename T, int PER>
+static cudaError_t launch_route_per(const RouteArgs& a, cudaStream_t st) {
+  const bool scores = a.bias != nullptr || (a.n_group > 1 && a.top2);
+  return launch_overlapped(scores ? route_scores_kernel<T, PER> : route_logits_kernel<T, PER>,
+                           dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
+}
+template <typename T>
 static int launch_route(const RouteArgs& a, cudaStream_t st) {
   const int per = (a.E + 31) / 32;
-  void (*kern)(RouteArgs) = per <= 1    ? route_kernel<T, 1, S>
-                            : per <= 2  ? route_kernel<T, 2, S>
-                            : per <= 4  ? route_kernel<T, 4, S>
-                            : per <= 6  ? route_kernel<T, 6, S>
-                            : per <= 8  ? route_kernel<T, 8, S>
-                            : per <= 12 ? route_kernel<T, 12, S>
-                                        : route_kernel<T, 16, S>;
-  const cudaError_t e = launch_overlapped(kern, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
+  const cudaError_t e = per <= 1    ? launch_route_per<T, 1>(a, st)
+                        : per <= 2  ? launch_route_per<T, 2>(a, st)
+                        : per <= 4  ? launch_route_per<T, 4>(a, st)
+                        : per <= 6  ? launch_route_per<T, 6>(a, st)
+                        : per <= 8  ? launch_route_per<T, 8>(a, st)
+                        : per <= 12 ? launch_route_per<T, 12>(a, st)
+                                    : launch_route_per<T, 16>(a, st);
   if (e != cudaSuccess) {
-    record_cuda_error(e, "route_kernel launch");
+    record_cuda_error(e, "route kernel launch");
     return LQ_ERR_CUDA;
   }
-  return check_launch("route_kernel");
+  return check_launch("route kernel");
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -987,12 +1155,10 @@ int lq_moe_route(const void* logits, int logits_dtype, const float* bias, float*
   a.sigmoid = scoring == 1;
   a.top2 = group_score == 1;
   a.renormalize = renormalize != 0;
-  // (sigmoid scores far below 1 would lose their ratio in float32's denormal range)
-  const bool wide = a.sigmoid || bias != nullptr || (a.n_group > 1 && a.top2);
   cudaStream_t st = as_stream(stream);
-  if (logits_dtype == LQ_DT_BF16) return wide ? launch_route<__nv_bfloat16, double>(a, st) : launch_route<__nv_bfloat16, float>(a, st);
-  if (logits_dtype == LQ_DT_F16) return wide ? launch_route<__half, double>(a, st) : launch_route<__half, float>(a, st);
-  return wide ? launch_route<float, double>(a, st) : launch_route<float, float>(a, st);
+  if (logits_dtype == LQ_DT_BF16) return launch_route<__nv_bfloat16>(a, st);
+  if (logits_dtype == LQ_DT_F16) return launch_route<__half>(a, st);
+  return launch_route<float>(a, st);
 }
 
 size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K, int w_kind) {

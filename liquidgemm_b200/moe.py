@@ -108,8 +108,8 @@ def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, re
         _same_device(logits, bias=bias)
         bias = bias.contiguous()
     logits = logits.contiguous()
-    weights = torch.empty((T, topk), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((T, topk), dtype=torch.int32, device=logits.device)
+    weights = torch.empty(T, topk, dtype=torch.float32, device=logits.device)
+    ids = torch.empty(T, topk, dtype=torch.int32, device=logits.device)
     if T:
         with _dev_ctx(logits):
             check(lib.lq_moe_route(_ptr(logits), _DTYPE_CODES[logits.dtype], None if bias is None else _ptr(bias), _ptr(weights),
@@ -173,6 +173,14 @@ def _experts_mlp(x, weights, ids, w13, s13, w2, s2, out_dtype):
     return y
 
 
+def _plain_call(t: torch.Tensor) -> bool:
+    """Whether an operator may be called without torch's dispatcher: an ordinary tensor, nothing that traces or intercepts.  The
+    dispatcher's way into a Python kernel costs 4.5 us of the host's 17 for a router call, which is all that a small one
+    takes."""
+    return type(t) is torch.Tensor and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0 and \
+        not torch.jit.is_tracing() and t.is_cuda
+
+
 _impl.impl("moe_route", _moe_route)
 _impl.impl("experts_linear", _experts_linear)
 _impl.impl("experts_mlp", _experts_mlp)
@@ -193,8 +201,9 @@ def route(logits: torch.Tensor, topk: int, scoring: str = "softmax", bias: Optio
     its expert out; slots for which no expert is left have id -1 and weight 0 (the products skip them)."""
     _req(scoring in _SCORING, "scoring must be 'softmax' or 'sigmoid'")
     _req(group_score in _GROUP_SCORE, "group_score must be 'max' or 'top2'")
-    return torch.ops.liquidgemm.moe_route(logits, bias, int(topk), _SCORING[scoring], int(n_group), int(topk_group),
-                                          _GROUP_SCORE[group_score], bool(renormalize), float(scale))
+    run = _moe_route if _plain_call(logits) else torch.ops.liquidgemm.moe_route
+    return run(logits, bias, int(topk), _SCORING[scoring], int(n_group), int(topk_group), _GROUP_SCORE[group_score], bool(renormalize),
+               float(scale))
 
 
 def quantize_experts(w: torch.Tensor, w4: bool = True, gated: bool = False, group_size: int = 64) -> dict:
@@ -242,8 +251,8 @@ def experts_linear(x: torch.Tensor, ids: torch.Tensor, layer: dict, ascale: Opti
     _req(not layer["gated"], "a gated stack is stored for experts_mlp")
     out_dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.int8 else x.dtype)
     _req(out_dtype in _DTYPE_CODES, "out_dtype must be bfloat16, float16 or float32")
-    return torch.ops.liquidgemm.experts_linear(x, ascale, ids, layer["w"], layer["s1"], layer["N"], layer["K"],
-                                               _DTYPE_CODES[out_dtype])
+    run = _experts_linear if _plain_call(x) else torch.ops.liquidgemm.experts_linear
+    return run(x, ascale, ids, layer["w"], layer["s1"], layer["N"], layer["K"], _DTYPE_CODES[out_dtype])
 
 
 def experts_mlp(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w13: dict, w2: dict,
@@ -257,4 +266,5 @@ def experts_mlp(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w13: 
     _req(w13["gated"] and not w2["gated"], "w13 must be quantised with gated=True and w2 without")
     out_dtype = out_dtype or x.dtype
     _req(out_dtype in _DTYPE_CODES, "out_dtype must be bfloat16, float16 or float32")
-    return torch.ops.liquidgemm.experts_mlp(x, weights, ids, w13["w"], w13["s1"], w2["w"], w2["s1"], _DTYPE_CODES[out_dtype])
+    run = _experts_mlp if _plain_call(x) else torch.ops.liquidgemm.experts_mlp
+    return run(x, weights, ids, w13["w"], w13["s1"], w2["w"], w2["s1"], _DTYPE_CODES[out_dtype])

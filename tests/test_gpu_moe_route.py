@@ -139,6 +139,25 @@ def test_masked_experts(moe, dtype, how):
     assert torch.all((w.cpu().double() - want_w).abs() <= 2 * (40 + 28) * 2.0 ** -24 * want_w + 1e-37)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_keys_closer_than_float32_errors(moe, scoring):
+    """Biases that bring every key of a token within a few units of float32's last place of one another: the choice is that of 64 bits."""
+    T, E = 60, 64
+    l = _logits(T, E, torch.float32, 8)
+    s = torch.sigmoid(l.double()) if scoring == "sigmoid" else torch.softmax(l.double(), 1)
+    for t in (0, 7, 31):
+        bias = (0.75 - s[t]).float()                       # all keys of token t are 0.75 but for the bias' rounding
+        for how in (dict(), dict(n_group=8, topk_group=3), dict(n_group=8, topk_group=3, group_score="top2")):
+            check(moe, l, 6, scoring=scoring, bias=bias, **how)
+    # groups whose sums of two scores are nearly equal, without a bias
+    l[:, 32:] = l[:, :32] + torch.randn(T, 32, device="cuda", generator=_gen_like(9)) * 1e-6
+    check(moe, l, 6, scoring=scoring, n_group=2, topk_group=1, group_score="top2")
+
+
+def _gen_like(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
 def test_infinite_logits_share(moe):
     l = torch.zeros(1, 8, device="cuda")
     l[0, 2] = l[0, 5] = float("inf")
