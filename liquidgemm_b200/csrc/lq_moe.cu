@@ -73,6 +73,8 @@ struct RouteArgs {
   float* weights;
   int* ids;
   int T, E, topk, n_group, topk_group;
+  unsigned group_size, group_inv;   // E / n_group, and e / group_size = e * group_inv >> 20 for e < 512
+  int group_lanes;                  // 32 / n_group down to a power of two, at least 1
   float scale;
   bool sigmoid, top2, renormalize;
 };
@@ -114,17 +116,32 @@ __device__ __forceinline__ S softmax_terms(const float (&l)[PER], float& top, S 
   return sum > 0 ? sum : (S)1;
 }
 
-// Lane j has choice j (id -1: none left) and its score.
-__device__ __forceinline__ void store_choice(const RouteArgs& a, long t, int id, double score) {
+// sigmoid(l), for a token with a choice below -80 (`tiny`) times 2^100: the ratio of such scores to others would be lost in the
+// denormal range.
+__device__ __forceinline__ float sigmoid_score(float l, bool tiny) {
+  if (tiny) return (float)(0x1p100 / (1.0 + exp(-(double)l)));
+  return __fdividef(1.f, 1.f + expf(-l));
+}
+
+// Lane j has choice j (id -1: none left) and what its score comes from: the logit of a sigmoid, or the score itself.
+__device__ __forceinline__ void store_choice(const RouteArgs& a, long t, int id, float from) {
   const int lane = threadIdx.x & 31;
-  if (id < 0) score = 0;
+  bool tiny = false;
+  float score = from;
+  if (a.sigmoid) {
+    tiny = __any_sync(0xffffffffu, id >= 0 && from < -80.f);
+    score = sigmoid_score(from, tiny);
+  }
+  if (id < 0) score = 0.f;
   if (a.renormalize) {
-    double total = score;
+    float total = score;
     for (int o = 1; o < a.topk; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);   // (lanes behind the last slot hold 0)
-    if (total > 0) score = score / total;
+    if (total > 0.f) score = __fdiv_rn(score, total);
+  } else if (tiny) {
+    score *= 0x1p-100f;
   }
   if (lane < a.topk) {
-    a.weights[t * a.topk + lane] = (float)(score * (double)a.scale);
+    a.weights[t * a.topk + lane] = score * a.scale;
     a.ids[t * a.topk + lane] = id;
   }
 }
@@ -135,11 +152,9 @@ __device__ __forceinline__ void store_choice(const RouteArgs& a, long t, int id,
 template <typename S>
 __device__ __forceinline__ bool rank_groups(const RouteArgs& a, bool top2, const S* v, S* rank, uint8_t* kept, S near) {
   const int lane = threadIdx.x & 31;
-  const int G = a.n_group, size = a.E / G;
-  int L = 1;   // lanes of a group
-  while (2 * L * G <= 32) L *= 2;
-  for (int base = 0; base < G; base += 32 / L) {
-    const int g = base + lane / L;
+  const int G = a.n_group, size = (int)a.group_size, L = a.group_lanes, shift = __ffs(L) - 1;
+  for (int base = 0; base < G; base += 32 >> shift) {
+    const int g = base + (lane >> shift);
     S m1 = kNone, m2 = kNone;
     if (g < G) {
       for (int e = lane & (L - 1); e < size; e += L) {
@@ -172,11 +187,7 @@ __device__ __forceinline__ bool rank_groups(const RouteArgs& a, bool top2, const
   __syncwarp();
   return __all_sync(0xffffffffu, clear);
 }
-// e / size for e < 512
-__device__ __forceinline__ unsigned group_of(const RouteArgs& a, unsigned e) {
-  const unsigned size = a.E / a.n_group, inv = ((1u << 20) + size - 1) / size;
-  return e * inv >> 20;
-}
+__device__ __forceinline__ unsigned group_of(const RouteArgs& a, unsigned e) { return e * a.group_inv >> 20; }
 
 // Choice by logits: no bias, groups by their largest.
 template <typename T, int PER>
@@ -239,15 +250,12 @@ route_logits_kernel(const RouteArgs a) {
       else my_l = number(best);
     }
   }
-  double score;
-  if (a.sigmoid) {
-    score = 1.0 / (1.0 + exp(-(double)my_l));
-  } else {
+  if (!a.sigmoid) {
     float top, s[PER];
     const float sum = softmax_terms<PER, float>(l, top, s);
-    score = (double)(my_l == top ? 1.f : expf(my_l - top)) / (double)sum;
+    my_l = __fdiv_rn(my_l == top ? 1.f : expf(my_l - top), sum);
   }
-  store_choice(a, t, my_id, score);
+  store_choice(a, t, my_id, my_l);
 }
 
 // The warp's buffers of the kernel below.
@@ -262,7 +270,7 @@ struct RouteBuffers {
 // used), a softmax score by 31 * 2^-24 (argument |x| e^x < 0.4, exponential 2 units, sum of 16 terms and over 32 lanes, quotient;
 // 2^-18 is used), the key by another |v| 2^-24; two keys by twice that, two sums of two by four times.
 template <int PER, typename S>
-__device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float (&l)[PER], RouteBuffers<PER>& buf, int& my_id, double& my_s) {
+__device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float (&l)[PER], RouteBuffers<PER>& buf, int& my_id, float& my_from) {
   using Key = typename KeyOf<S>::type;
   constexpr bool kFast = sizeof(S) == 4;
   const int lane = threadIdx.x & 31;
@@ -312,7 +320,7 @@ __device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float 
       if (e < a.E && !buf.kept[group_of(a, e)]) key[i] = 0;
     }
   }
-  // what the chosen ones' scores are taken from: the logit (a sigmoid is worked out again, in float64, a lane each) or the score
+  // what the chosen ones' scores are taken from: the logit (a sigmoid is worked out again, a lane each) or the score
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < PER; ++i) values[lane + 32 * i] = a.sigmoid ? (S)l[i] : s[i];
@@ -340,10 +348,7 @@ __device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float 
       if (id == lane + 32 * i) key[i] = 0;
     if (lane == j) my_id = id;
   }
-  if (my_id >= 0) {
-    my_s = (double)values[my_id];
-    if (a.sigmoid) my_s = 1.0 / (1.0 + exp(-my_s));
-  }
+  if (my_id >= 0) my_from = (float)values[my_id];
   return true;
 }
 
@@ -359,14 +364,13 @@ route_scores_kernel(const RouteArgs a) {
   float l[PER];
   load_logits<T, PER>(a, t, l);
   int id = -1;
-  double score = 0;
-  if (!choose_by_score<PER, float>(a, l, buffers[warp], id, score)) {
+  float from = 0.f;
+  if (!choose_by_score<PER, float>(a, l, buffers[warp], id, from)) {
     __syncwarp();
     id = -1;
-    score = 0;
-    choose_by_score<PER, double>(a, l, buffers[warp], id, score);
+    choose_by_score<PER, double>(a, l, buffers[warp], id, from);
   }
-  store_choice(a, t, id, score);
+  store_choice(a, t, id, from);
 }
 
 template <typename T, int PER>
@@ -1151,6 +1155,10 @@ int lq_moe_route(const void* logits, int logits_dtype, const float* bias, float*
   a.topk = topk;
   a.n_group = topk_group == n_group ? 1 : n_group;   // every group stays: nothing to rank
   a.topk_group = topk_group;
+  a.group_size = (unsigned)(E / a.n_group);
+  a.group_inv = ((1u << 20) + a.group_size - 1) / a.group_size;
+  a.group_lanes = 1;
+  while (2 * a.group_lanes * a.n_group <= 32) a.group_lanes *= 2;
   a.scale = scale;
   a.sigmoid = scoring == 1;
   a.top2 = group_score == 1;

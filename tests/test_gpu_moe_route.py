@@ -158,6 +158,17 @@ def _gen_like(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
 
+def test_scores_far_below_one_keep_their_ratio(moe):
+    """Sigmoids below the smallest float32: the weights' ratio is that of the exponentials, and without renormalising they vanish."""
+    l = torch.full((3, 16), -150.0, device="cuda")
+    l[0, 3], l[0, 9] = -95.0, -95.5
+    l[1, 3], l[1, 9] = -120.0, -121.0
+    l[2, 3], l[2, 9] = -70.0, -90.0
+    check(moe, l, 2, scoring="sigmoid")
+    check(moe, l, 2, scoring="sigmoid", renormalize=False)
+    check(moe, l, 2, scoring="sigmoid", bias=torch.linspace(0, -1, 16, device="cuda"), renormalize=False)
+
+
 def test_infinite_logits_share(moe):
     l = torch.zeros(1, 8, device="cuda")
     l[0, 2] = l[0, 5] = float("inf")
