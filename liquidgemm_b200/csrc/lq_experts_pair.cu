@@ -5,9 +5,9 @@
 //
 // Work: pair p of P takes the tiles p, p + P, ... of the plan's row tiles x 256-channel blocks, in groups of eight row tiles (see
 // tile_coords), so that the tiles at work at one time share rows and weights in L2.  How many there are is known on the device
-// only.  A tile's MMA is as wide as its rows need, in steps of 32; each CTA stages half of them, in ONE box of a half or a quarter
-// of the widest tile's rows (boxes of 64 and 16 rows as needed: 28 % slower on full tiles of 192, the copies are bound by their
-// number).  Rows of the box behind the tile's are those of the next expert, or zeros; their sums are not stored.  With an odd number of 128-channel blocks the
+// only.  A tile's MMA is as wide as its rows need, in steps of 32; each CTA stages half of them in ONE box, for which there is a tensor
+// map of every width (boxes of 64 and 16 rows as needed: 28 % slower on full tiles of 192, the copies are bound by their number).
+// Rows of the box behind the tile's are those of the next expert, or zeros; their sums are not stored.  With an odd number of 128-channel blocks the
 // second CTA's half of the last tile lies behind the expert's channels: it computes with other weights and stores nothing.
 //
 // Per CTA, connected by mbarrier rings; rank = CTA's rank in its pair:
@@ -72,6 +72,12 @@ struct Cfg {
   static_assert(2 * kBN + (W4 ? 32 * kNT : 0) <= 512, "tensor memory budget exceeded");
 };
 
+// Tensor maps of the rows, x[i] with boxes of 16 (i + 1) rows, and of INT8 weights.
+struct Maps {
+  CUtensorMap x[kPairRowsInt8 / 32];
+  CUtensorMap w;
+};
+
 struct Tile {
   int expert, row0, rows, n2;
 };
@@ -89,8 +95,7 @@ __device__ __forceinline__ int width(int rows) { return (rows + 31) & ~31; }
 
 template <bool W4, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<W4>::kThreads, 1)
-experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_xfull, const __grid_constant__ CUtensorMap tmap_xhalf,
-                    const __grid_constant__ CUtensorMap tmap_w, const Args args) {
+experts_pair_kernel(const __grid_constant__ Maps maps, const Args args) {
   using C = Cfg<W4>;
   constexpr int kNS = C::kNS, kBN = C::kBN;
   extern __shared__ uint8_t smem_raw[];
@@ -134,9 +139,8 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_xfull, const __grid
       ptx::mbar_init(bar_accfree + 8 * b, 2 * 4 * C::kGroups);   // one arrival per epilogue warp, both CTAs
     }
     ptx::fence_mbar_init();
-    ptx::prefetch_tensormap(&tmap_xfull);
-    ptx::prefetch_tensormap(&tmap_xhalf);
-    if (!W4) ptx::prefetch_tensormap(&tmap_w);
+    ptx::prefetch_tensormap(&maps.x[kBN / 32 - 1]);
+    if (!W4) ptx::prefetch_tensormap(&maps.w);
   }
   if (warp == 1) {
     ptx::tmem_alloc_pair(tmem_slot, 512);
@@ -171,8 +175,7 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_xfull, const __grid
       const uint8_t* wsrc = W4 ? args.blob + ((size_t)t.expert * args.n_tiles + (nt < args.n_tiles ? nt : args.n_tiles - 1)) *
                                                  (size_t)args.kt_total * kBlobTile : nullptr;
       const int half = width(t.rows) / 2;
-      const bool few = half <= kBN / 4;
-      const uint32_t box = few ? kBN / 4 : kBN / 2;
+      const CUtensorMap* xmap = &maps.x[half / 16 - 1];
       const int row0 = weights ? t.expert * args.N + nt * 128 : t.row0 + (int)rank * half;
       for (int kt = 0; kt < args.kt_total; ++kt) {
         ok = ptx::mbar_wait_bounded(bar_empty + 8 * ring.s, ring.ph ^ 1u, kWaitLimitNs);
@@ -187,14 +190,14 @@ experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_xfull, const __grid
           if (leader) {
             ptx::mbar_expect_tx(full, C::kWStage);
             if (W4) ptx::bulk_load(dst, wsrc, kBlobTile, full);
-            else ptx::tensor_load_2d(dst, &tmap_w, kt * 128, row0, full);
+            else ptx::tensor_load_2d(dst, &maps.w, kt * 128, row0, full);
           }
           if (W4) wsrc += kBlobTile;
         } else {
           const uint32_t dst = xs + ring.s * C::kXStage;
           if (leader) {
-            ptx::mbar_expect_tx(full, box * 128u);
-            ptx::tensor_load_2d(dst, few ? &tmap_xhalf : &tmap_xfull, kt * 128, row0, full);
+            ptx::mbar_expect_tx(full, (uint32_t)half * 128u);
+            ptx::tensor_load_2d(dst, xmap, kt * 128, row0, full);
           }
         }
         ring.advance();
@@ -445,11 +448,12 @@ static int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
     }
     cap = v;
   }
-  CUtensorMap xfull, xhalf, tw;
-  if (int rc = make_byte_matrix_map(&xfull, p.x, p.rows, p.K, C::kBN / 2, 128)) return rc;
-  if (int rc = make_byte_matrix_map(&xhalf, p.x, p.rows, p.K, C::kBN / 4, 128)) return rc;
-  if (W4) tw = xhalf;
-  else if (int rc = make_byte_matrix_map(&tw, p.w, (long)p.E * p.N, p.K, 128, 128)) return rc;
+  Maps maps;
+  for (int i = 0; i < C::kBN / 32; ++i)
+    if (int rc = make_byte_matrix_map(&maps.x[i], p.x, p.rows, p.K, 16 * (i + 1), 128)) return rc;
+  for (int i = C::kBN / 32; i < kPairRowsInt8 / 32; ++i) maps.x[i] = maps.x[0];   // (no width selects these)
+  if (W4) maps.w = maps.x[0];
+  else if (int rc = make_byte_matrix_map(&maps.w, p.w, (long)p.E * p.N, p.K, 128, 128)) return rc;
   Args a;
   a.blob = static_cast<const uint8_t*>(p.w);
   a.s1 = p.s1;
@@ -470,7 +474,7 @@ static int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
   if (!a.status) return LQ_ERR_CUDA;
   const long items = max_tiles(p.rows, p.E, plan.bn) * a.n2_tiles;
   a.pairs = (int)(items < cap ? items : cap);
-  const cudaError_t e = launch_overlapped(kern, dim3(2 * a.pairs), dim3(C::kThreads), (size_t)C::kSmemBytes, st, xfull, xhalf, tw, a);
+  const cudaError_t e = launch_overlapped(kern, dim3(2 * a.pairs), dim3(C::kThreads), (size_t)C::kSmemBytes, st, maps, a);
   if (e != cudaSuccess) {
     record_cuda_error(e, "experts_pair_kernel launch");
     return LQ_ERR_CUDA;
