@@ -516,7 +516,7 @@ static int run_plan(const int* ids, long pairs, int E, const Plan& plan, cudaStr
 // and written to the places of its pairs.  NV 16-byte vectors per thread in registers; NV = 0: a row too long for that is read
 // twice.  Where the outputs are one row per pair, the rows of pairs without an expert are set to zero here.
 //
-// Up to kSortedHere pairs (`plan.tiles` set) there is no plan kernel before this one: a CTA finds the places of its own pairs
+// Up to kSortedHere pairs (SORT) there is no plan kernel before this one: a CTA finds the places of its own pairs
 // by counting the pairs that come before them, and one more CTA (the first) cuts the experts' rows into tiles.  That
 // saves a launch and its hand-over, 4 of the 9 us before the first product of a decode step; the counting grows with
 // the square of the pairs (at 2048 it takes the time of the plan kernel).
@@ -532,28 +532,45 @@ struct PlaceArgs {
   int y_size;              // bytes of an element of y
   int per_row;             // pairs of a row of x
   int K, N;
-  const int* ids;          // with plan.tiles: the sort is done here
+  const int* ids;          // SORT: the pairs and where the plan goes
   int pairs, E;
   Plan plan;
 };
 
+// The ids into shared memory, once per CTA: every CTA wants all of them at the same time, and asked for by each of its warps they
+// queue at the few L2 lines that hold them (1800 pairs: 8 us).
+__device__ __forceinline__ void fetch_ids(const PlaceArgs& a, int* ids) {
+  constexpr int kAhead = 8;   // of a thread in flight
+  for (int i0 = threadIdx.x; i0 < a.pairs; i0 += kAhead * blockDim.x) {
+    int e[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) e[q] = i0 + q * (int)blockDim.x < a.pairs ? a.ids[i0 + q * blockDim.x] : 0;
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (i0 + q * (int)blockDim.x < a.pairs) ids[i0 + q * blockDim.x] = e[q];
+  }
+}
+
 // Tiles and counts of the plan (one CTA of any size).
-__device__ __forceinline__ void make_tiles(const PlaceArgs& a) {
-  __shared__ int hist[kMaxExperts];
+__device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
   for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.pairs; i += blockDim.x) {
-    const int e = a.ids[i];
-    if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
+  constexpr int kAhead = 8;   // ids of a thread in flight
+  for (int i0 = threadIdx.x; i0 < a.pairs; i0 += kAhead * blockDim.x) {
+    int e[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) e[q] = i0 + q * (int)blockDim.x < a.pairs ? a.ids[i0 + q * blockDim.x] : -1;
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (e[q] >= 0 && e[q] < a.E) atomicAdd(&hist[e[q]], 1);
   }
   __syncthreads();
   if (threadIdx.x >= 32) return;
-  constexpr int kPer = kMaxExperts / 32;   // neighbouring experts of a lane
+  const int per = (a.E + 31) / 32;   // neighbouring experts of a lane
   const int lane = threadIdx.x;
   int rows = 0, tiles = 0;
-#pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    const int n = hist[lane * kPer + q];
+  for (int q = 0; q < per; ++q) {
+    const int n = hist[lane * per + q];
     rows += n;
     tiles += (n + a.plan.bn - 1) / a.plan.bn;
   }
@@ -569,8 +586,8 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a) {
   }
   r -= rows;
   t -= tiles;
-  for (int q = 0; q < kPer; ++q) {
-    const int e = lane * kPer + q, n = hist[e];
+  for (int q = 0; q < per; ++q) {
+    const int e = lane * per + q, n = hist[e];
     const int mine = (n + a.plan.bn - 1) / a.plan.bn;
     write_tiles(a.plan, t, e, r, n, mine);
     t += mine;
@@ -578,19 +595,23 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a) {
   }
 }
 
-// The places of the pairs of row m, in `place` [per_row] (shared memory): read from the plan, or counted and entered there.
-__device__ __forceinline__ void find_places(const PlaceArgs& a, long m, int* place) {
-  if (!a.plan.tiles) {
+// The places of the pairs of row m, in `place` [per_row] (shared memory): read from the plan, or counted (`ids`: room for all) and
+// entered there.
+template <bool SORT>
+__device__ __forceinline__ void find_places(const PlaceArgs& a, long m, int* ids, int* place) {
+  if constexpr (!SORT) {
     for (int j = threadIdx.x; j < a.per_row; j += blockDim.x) place[j] = a.pos_of_pair[m * a.per_row + j];
   } else {
+    fetch_ids(a, ids);
+    __syncthreads();
     const int lane = threadIdx.x & 31;
     for (int j = threadIdx.x >> 5; j < a.per_row; j += blockDim.x >> 5) {
       const int pair = (int)m * a.per_row + j;
-      const int e = a.ids[pair];
+      const int e = ids[pair];
       int before = 0;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = lane; i < a.pairs; i += 32) {
-        const int o = a.ids[i];
+        const int o = ids[i];
         before += (o >= 0 && (o < e || (o == e && i < pair))) ? 1 : 0;
       }
       before = __reduce_add_sync(0xffffffffu, before);
@@ -614,19 +635,20 @@ __device__ __forceinline__ void clear_output_row(const PlaceArgs& a, long pair) 
   }
 }
 
-template <typename T, int NV>
+template <typename T, int NV, bool SORT>
 __global__ void __launch_bounds__(1024)
 place_rows_kernel(const PlaceArgs a) {
   __shared__ float red[32];
   __shared__ int place[kMaxTopk];
+  __shared__ int ids[SORT ? kSortedHere : 1];
   constexpr int VEC = 16 / sizeof(T);
   allow_dependents();
   dependency_wait();
-  if (a.plan.tiles && blockIdx.x == 0) {
-    make_tiles(a);
+  if (SORT && blockIdx.x == 0) {
+    make_tiles(a, ids);
     return;
   }
-  const long m = a.plan.tiles ? blockIdx.x - 1 : blockIdx.x;
+  const long m = SORT ? blockIdx.x - 1 : blockIdx.x;
   const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + m * a.K);
   const int nvec = a.K / VEC;
   uint4 raw[NV > 0 ? NV : 1];
@@ -642,10 +664,16 @@ place_rows_kernel(const PlaceArgs a) {
   } else {
     for (int v = threadIdx.x; v < nvec; v += blockDim.x) rm.take(xr[v]);
   }
-  find_places(a, m, place);
+  find_places<SORT>(a, m, ids, place);
   const float amax = block_max(rm.value(), red);   // (its barrier orders the places too)
   const float scale = __fdiv_rn(fmaxf(amax, 1e-12f), 127.0f);
   const float inv = __fdiv_rn(1.0f, scale);
+  constexpr int kWords = 4 / sizeof(T);   // of four codes, from one vector
+  uint32_t q[NV > 0 ? NV : 1][kWords];
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) quant_vec<T>(raw[i], scale, inv, q[i]);
+  }
   for (int j = 0; j < a.per_row; ++j) {
     const long pair = m * a.per_row + j;
     const int p = place[j];
@@ -657,40 +685,39 @@ place_rows_kernel(const PlaceArgs a) {
       a.ascale[p] = scale;
       if (a.amax) a.amax[p] = 0u;
     }
-    int8_t* qr = a.xq + (long)p * a.K;
+    uint32_t* qr = reinterpret_cast<uint32_t*>(a.xq + (long)p * a.K);
     if constexpr (NV > 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v >= nvec) break;
-        uint32_t out[4 / sizeof(T)];
-        quant_vec<T>(raw[i], scale, inv, out);
-        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(qr)[v] = out[0];
-        else reinterpret_cast<uint2*>(qr)[v] = make_uint2(out[0], out[1]);
+        if constexpr (kWords == 1) qr[v] = q[i][0];
+        else reinterpret_cast<uint2*>(qr)[v] = make_uint2(q[i][0], q[i][1]);
       }
     } else {
       for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
-        uint32_t out[4 / sizeof(T)];
-        quant_vec<T>(xr[v], scale, inv, out);
-        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(qr)[v] = out[0];
-        else reinterpret_cast<uint2*>(qr)[v] = make_uint2(out[0], out[1]);
+        quant_vec<T>(xr[v], scale, inv, q[0]);
+        if constexpr (kWords == 1) qr[v] = q[0][0];
+        else reinterpret_cast<uint2*>(qr)[v] = make_uint2(q[0][0], q[0][1]);
       }
     }
   }
 }
 
 // Rows that come in INT8 with their scales.
+template <bool SORT>
 __global__ void __launch_bounds__(256)
 place_i8_kernel(const PlaceArgs a) {
   __shared__ int place[kMaxTopk];
+  __shared__ int ids[SORT ? kSortedHere : 1];
   allow_dependents();
   dependency_wait();
-  if (a.plan.tiles && blockIdx.x == 0) {
-    make_tiles(a);
+  if (SORT && blockIdx.x == 0) {
+    make_tiles(a, ids);
     return;
   }
-  const long m = a.plan.tiles ? blockIdx.x - 1 : blockIdx.x;
-  find_places(a, m, place);
+  const long m = SORT ? blockIdx.x - 1 : blockIdx.x;
+  find_places<SORT>(a, m, ids, place);
   __syncthreads();
   const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const int8_t*>(a.x) + m * a.K);
   const float scale = a.x_scale[m];
@@ -707,22 +734,30 @@ place_i8_kernel(const PlaceArgs a) {
   }
 }
 
-template <typename T>
-static int launch_place(const PlaceArgs& a, long rows, cudaStream_t st) {
+template <typename T, bool SORT>
+static cudaError_t launch_place(const PlaceArgs& a, long rows, cudaStream_t st) {
   int threads = 0;
   const int nv = row_units_per_thread(rows, a.K / (16 / (int)sizeof(T)), 8, 128, 1024, &threads);
-  void (*kern)(PlaceArgs) = nv == 1   ? place_rows_kernel<T, 1>
-                            : nv == 2 ? place_rows_kernel<T, 2>
-                            : nv == 4 ? place_rows_kernel<T, 4>
-                            : nv == 8 ? place_rows_kernel<T, 8>
-                                      : place_rows_kernel<T, 0>;
+  void (*kern)(PlaceArgs) = nv == 1   ? place_rows_kernel<T, 1, SORT>
+                            : nv == 2 ? place_rows_kernel<T, 2, SORT>
+                            : nv == 4 ? place_rows_kernel<T, 4, SORT>
+                            : nv == 8 ? place_rows_kernel<T, 8, SORT>
+                                      : place_rows_kernel<T, 0, SORT>;
   if (nv == 0) threads = 1024;
-  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)rows + (a.plan.tiles ? 1u : 0u)), dim3(threads), 0, st, a);
+  return launch_overlapped(kern, dim3((unsigned)rows + (SORT ? 1u : 0u)), dim3(threads), 0, st, a);
+}
+template <bool SORT>
+static int launch_place_any(const PlaceArgs& a, int x_dtype, long rows, cudaStream_t st) {
+  const cudaError_t e = x_dtype == LQ_DT_BF16  ? launch_place<__nv_bfloat16, SORT>(a, rows, st)
+                        : x_dtype == LQ_DT_F16 ? launch_place<__half, SORT>(a, rows, st)
+                        : x_dtype == LQ_DT_F32 ? launch_place<float, SORT>(a, rows, st)
+                                               : launch_overlapped(place_i8_kernel<SORT>, dim3((unsigned)rows + (SORT ? 1u : 0u)),
+                                                                   dim3(256), 0, st, a);
   if (e != cudaSuccess) {
-    record_cuda_error(e, "place_rows_kernel launch");
+    record_cuda_error(e, "place kernel launch");
     return LQ_ERR_CUDA;
   }
-  return check_launch("place_rows_kernel");
+  return check_launch("place kernel");
 }
 
 // Plan and rows.
@@ -733,18 +768,10 @@ static int run_place(PlaceArgs& a, const int* ids, long pairs, int E, const Plan
     a.pairs = (int)pairs;
     a.E = E;
     a.plan = plan;
-  } else if (int rc = run_plan(ids, pairs, E, plan, st)) {
-    return rc;
+    return launch_place_any<true>(a, x_dtype, rows, st);
   }
-  if (x_dtype == LQ_DT_BF16) return launch_place<__nv_bfloat16>(a, rows, st);
-  if (x_dtype == LQ_DT_F16) return launch_place<__half>(a, rows, st);
-  if (x_dtype == LQ_DT_F32) return launch_place<float>(a, rows, st);
-  const cudaError_t e = launch_overlapped(place_i8_kernel, dim3((unsigned)rows + (a.plan.tiles ? 1u : 0u)), dim3(256), 0, st, a);
-  if (e != cudaSuccess) {
-    record_cuda_error(e, "place_i8_kernel launch");
-    return LQ_ERR_CUDA;
-  }
-  return check_launch("place_i8_kernel");
+  if (int rc = run_plan(ids, pairs, E, plan, st)) return rc;
+  return launch_place_any<false>(a, x_dtype, rows, st);
 }
 
 // ---------------------------------------------------------------------------------------------
