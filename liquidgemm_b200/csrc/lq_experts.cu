@@ -48,7 +48,7 @@ struct Args {
   const int* pair_of_pos;
   EpiArgs epi;
   int* status;
-  int N, kt_total, n_tiles, splits;
+  int N, kt_total, n_tiles, which;
 };
 
 template <int BN, int NS, bool W4>
@@ -73,20 +73,20 @@ struct Cfg {
 struct Item {
   int expert, row0, rows, nt, s, kb, ke;
 };
-__device__ __forceinline__ Item item_of(const Args& a, int i, const int4& tile) {
+__device__ __forceinline__ Item item_of(const Args& a, int splits, int i, const int4& tile) {
   Item it;
-  const int in = i % (a.n_tiles * a.splits);
+  const int in = i % (a.n_tiles * splits);
   it.s = in / a.n_tiles;
   it.nt = in - it.s * a.n_tiles;
   it.expert = tile.x;
   it.row0 = tile.y;
   it.rows = tile.z;
-  it.kb = (it.s * a.kt_total) / a.splits;
-  it.ke = ((it.s + 1) * a.kt_total) / a.splits;
+  it.kb = (it.s * a.kt_total) / splits;
+  it.ke = ((it.s + 1) * a.kt_total) / splits;
   return it;
 }
-__device__ __forceinline__ int4 tile_of(const Args& a, int i) { return __ldcg(a.tiles + i / (a.n_tiles * a.splits)); }
-__device__ __forceinline__ Item item_at(const Args& a, int i) { return item_of(a, i, tile_of(a, i)); }
+__device__ __forceinline__ int4 tile_of(const Args& a, int splits, int i) { return __ldcg(a.tiles + i / (a.n_tiles * splits)); }
+__device__ __forceinline__ Item item_at(const Args& a, int splits, int i) { return item_of(a, splits, i, tile_of(a, splits, i)); }
 
 template <int BN, int NS, bool W4, int MODE>
 __global__ void __launch_bounds__(Cfg<BN, NS, W4>::kThreads, 2)
@@ -142,11 +142,13 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   dependency_wait();   // the plan, the rows and the buffers written here belong to earlier kernels until now
   const uint32_t tmem_acc = *tmem_slot_p;
   const uint32_t tmem_a = tmem_acc + C::kAcc * BN;
-  // The first tile's entry is requested together with the number of tiles: the table has room for every tile that a launch of
-  // this grid can have, so an entry that is not there is read as anything and not used.
+  // Where k is whole the first tile's entry is requested together with the number of tiles: the table has room for every tile that
+  // a launch of this grid can have, so an entry that is not there is read as anything and not used.
   int4 tile = make_int4(0, 0, 0, 0);
-  if (warp == 0) tile = tile_of(args, blockIdx.x);
-  const int items = __ldcg(args.counts) * args.n_tiles * args.splits;
+  if (MODE != kOutPlanes && warp == 0) tile = tile_of(args, 1, blockIdx.x);
+  const int4 counts = __ldcg(reinterpret_cast<const int4*>(args.counts));
+  const int splits = MODE != kOutPlanes ? 1 : args.which == 0 ? counts.z : counts.w;
+  const int items = counts.x * args.n_tiles * splits;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ copies
@@ -157,8 +159,8 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     int issued = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      if (i != (int)blockIdx.x) tile = tile_of(args, i);
-      const Item it = item_of(args, i, tile);
+      if (MODE == kOutPlanes || i != (int)blockIdx.x) tile = tile_of(args, splits, i);
+      const Item it = item_of(args, splits, i, tile);
       const bool few = it.rows <= BN / 2;
       const uint32_t tx = (uint32_t)((few ? BN / 2 : BN) * 128 + C::kWStage);
       const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;
@@ -197,7 +199,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     Ring<C::kAcc> accring;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, i);
+      const Item it = item_at(args, splits, i);
       const uint32_t idesc = ptx::idesc_i8((it.rows + C::kStep - 1) / C::kStep * C::kStep);
       ok = ptx::mbar_wait_bounded(bar_accfree + 8 * accring.s, accring.ph ^ 1u, kWaitLimitNs);
       ok = __all_sync(0xffffffffu, ok);
@@ -247,7 +249,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     int turn = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, i);
+      const Item it = item_at(args, splits, i);
       for (int kt = it.kb; kt < it.ke; ++kt) {
         const bool mine = turn == set;
         turn ^= 1;
@@ -309,7 +311,7 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     Ring<C::kAcc> accring;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, i);
+      const Item it = item_at(args, splits, i);
       // What the epilogue needs beside the sums is requested ahead of them: behind the last MMA it would wait for the weight copies
       // of the next item, which fill the queues to memory (a channel scale read there cost 3 to 5 us an item).
       const int n = it.nt * 128 + row;
@@ -396,10 +398,10 @@ static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
   a.N = p.N;
   a.kt_total = p.K / 128;
   a.n_tiles = (p.N + 127) / 128;
-  a.splits = p.splits;
+  a.which = p.which;
   if (!a.status) return LQ_ERR_CUDA;
-  const long items = max_tiles(p.rows, p.E, plan.bn) * a.n_tiles * a.splits;
-  const long slots = 2L * sm_count();
+  const long items = max_tiles(p.rows, p.E, plan.bn) * a.n_tiles * (MODE == kOutPlanes ? plan.rule[p.which].most : 1);
+  const long slots = plan.slots;
   const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(C::kThreads),
                                           (size_t)C::kSmemBytes, st, tx, txh, tw, a);
   if (e != cudaSuccess) {

@@ -18,12 +18,31 @@ enum WeightKind { kBlob = 0, kInt8 = 1 };
 // A stable counting sort of the T * topk pairs by expert: pair i (token i / topk) gets row pos_of_pair[i] of the sorted
 // activations, the pair at row p is pair_of_pos[p].  Pairs whose id is no expert get no row (-1).  The rows of an expert
 // are cut into tiles of at most `bn` rows; tiles[i] = (expert, first row, rows, 0).
+//
+// Where few tiles meet many CTA slots a product's k is cut into ranges, whose int32 sums go to planes.  Whether it may be cut is
+// decided by the host from the sizes (`most` > 1), how often on the device from the number of tiles the tokens made.
+struct SplitRule {
+  int n_tiles, kt;   // 128-channel blocks of an expert, k-steps
+  int most;          // planes there is room for; 1: k stays whole
+};
+// Cuts that give the shortest time: rounds of CTAs times k-steps of a range, with six steps for its start and end.
+__host__ __device__ inline int best_splits(long tiles, const SplitRule& r, int slots) {
+  int best = 1;
+  long least = 0;
+  for (int s = 1; s <= r.most; ++s) {
+    const long items = tiles * r.n_tiles * s;
+    const long cost = (items + slots - 1) / slots * ((r.kt + s - 1) / s + 6);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
+}
 struct Plan {
-  int* counts;        // [4]: tiles, rows
+  int* counts;        // [4]: tiles, rows, k-ranges of the first product and of the second
   int4* tiles;        // [max_tiles]
   int* pos_of_pair;   // [pairs]
   int* pair_of_pos;   // [pairs]
-  int bn;
+  int bn, slots;      // slots: CTAs of the tile kernel that run together
+  SplitRule rule[2];
 };
 inline long max_tiles(long pairs, int E, int bn) {
   const long by_rows = pairs / bn + E;
@@ -45,7 +64,7 @@ struct Product {
   const float* ascale;     // [rows]
   long rows;               // rows of `x`: at least as many as the plan has
   int E, N, K;
-  int splits;              // k-ranges (kOutPlanes; 1 otherwise)
+  int which;               // of the plan's rules (kOutPlanes; k is whole otherwise)
   int out_mode, out_dtype;
   void* out;
   unsigned* amax;

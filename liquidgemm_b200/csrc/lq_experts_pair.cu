@@ -484,7 +484,6 @@ static int launch_pair(const Product& p, const Plan& plan, cudaStream_t st) {
 
 template <bool W4>
 static int launch_kind(const Product& p, const Plan& plan, cudaStream_t st) {
-  if (p.out_mode == kOutPlanes) return launch_pair<W4, kOutPlanes>(p, plan, st);
   if (p.out_mode == kOutPairs) return launch_pair<W4, kOutPairs>(p, plan, st);
   return launch_pair<W4, kOutGated>(p, plan, st);
 }
@@ -492,7 +491,7 @@ static int launch_kind(const Product& p, const Plan& plan, cudaStream_t st) {
 }  // namespace pair
 
 int run_product_pair(const Product& p, const Plan& plan, cudaStream_t st) {
-  if (p.splits != 1 || plan.bn != (p.w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8)) return LQ_ERR_BAD_ARG;
+  if (p.out_mode == kOutPlanes || plan.bn != (p.w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8)) return LQ_ERR_BAD_ARG;
   return p.w_kind == kBlob ? pair::launch_kind<true>(p, plan, st) : pair::launch_kind<false>(p, plan, st);
 }
 

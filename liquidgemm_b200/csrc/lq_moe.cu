@@ -401,6 +401,11 @@ static int launch_route(const RouteArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------------
 // The tiles of expert e: as few as cover its n rows, and of equal widths in steps of 32 (a full tile and a narrow rest would
 // take as long as two full ones wherever the two run side by side).  Every one has a row: bn is a multiple of 32.
+__device__ __forceinline__ void write_counts(const Plan& plan, int tiles, int rows) {
+  plan.counts[0] = tiles;
+  plan.counts[1] = rows;
+  for (int w = 0; w < 2; ++w) plan.counts[2 + w] = best_splits(tiles, plan.rule[w], plan.slots);
+}
 __device__ __forceinline__ void write_tiles(const Plan& plan, int tile0, int e, int row0, int n, int tiles) {
   if (tiles == 0) return;
   const int per = ((n + tiles - 1) / tiles + 31) & ~31;
@@ -462,10 +467,7 @@ plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
     for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] += row0;
     write_tiles(plan, tile0, e, row0, n, tiles);
   }
-  if (threadIdx.x == blockDim.x - 1) {
-    plan.counts[0] = rb + b;
-    plan.counts[1] = ra + a;
-  }
+  if (threadIdx.x == blockDim.x - 1) write_counts(plan, rb + b, ra + a);
   __syncthreads();
   for (long i0 = begin; i0 < end; i0 += 32 * kAhead) {
     int id[kAhead];
@@ -580,10 +582,7 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
     const int pr = __shfl_up_sync(0xffffffffu, r, o), pt = __shfl_up_sync(0xffffffffu, t, o);
     if (lane >= o) r += pr, t += pt;
   }
-  if (lane == 31) {
-    a.plan.counts[0] = t;
-    a.plan.counts[1] = r;
-  }
+  if (lane == 31) write_counts(a.plan, t, r);
   r -= rows;
   t -= tiles;
   for (int q = 0; q < per; ++q) {
@@ -789,13 +788,13 @@ struct HiddenArgs {
   int8_t* hq;                // [rows][I]
   float* hscale;             // [rows]
   long rows;
-  int I, splits;
+  int I;
 };
 
 // Four hidden values of row p from the planes.
-__device__ __forceinline__ void hidden4(const HiddenArgs& a, long p, const float* s1, float as, int c, float (&h)[4]) {
+__device__ __forceinline__ void hidden4(const HiddenArgs& a, int splits, long p, const float* s1, float as, int c, float (&h)[4]) {
   int4 g0 = make_int4(0, 0, 0, 0), g1 = g0;
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = 0; s < splits; ++s) {
     const int4* src = reinterpret_cast<const int4*>(a.planes + ((size_t)s * a.rows + p) * 2 * a.I + 2 * c);
     const int4 v0 = src[0], v1 = src[1];
     g0.x += v0.x; g0.y += v0.y; g0.z += v0.z; g0.w += v0.w;
@@ -827,10 +826,11 @@ hidden_planes_kernel(const HiddenArgs a) {
   const int e = a.ids[a.pair_of_pos[p]];
   const float* s1 = a.s1 + (size_t)e * 2 * a.I;
   const float as = a.ascale[p];
+  const int splits = a.counts[2];
   float m = 0.f;
   for (int c = threadIdx.x * 4; c < a.I; c += blockDim.x * 4) {
     float h[4];
-    hidden4(a, p, s1, as, c, h);
+    hidden4(a, splits, p, s1, as, c, h);
     m = fmaxf(fmaxf(m, fmaxf(fabsf(h[0]), fabsf(h[1]))), fmaxf(fabsf(h[2]), fabsf(h[3])));
   }
   m = block_max(m, red);
@@ -839,7 +839,7 @@ hidden_planes_kernel(const HiddenArgs a) {
   if (threadIdx.x == 0) a.hscale[p] = scale;
   for (int c = threadIdx.x * 4; c < a.I; c += blockDim.x * 4) {
     float h[4];
-    hidden4(a, p, s1, as, c, h);
+    hidden4(a, splits, p, s1, as, c, h);
     *reinterpret_cast<uint32_t*>(a.hq + p * a.I + c) = quant4(h, scale, inv);
   }
 }
@@ -904,7 +904,8 @@ struct CombineArgs {
   const int* pos_of_pair;
   void* y;                   // [T][N] or [T * topk][N]
   long rows, outs;           // rows of a plane, rows of y
-  int N, topk, splits, out_dtype;
+  const int* counts;         // of the plan: counts[2 + which] planes
+  int N, topk, which, out_dtype;
 };
 
 // Four neighbouring outputs, at an offset that is a multiple of four.
@@ -933,6 +934,7 @@ combine_kernel(const CombineArgs a) {
   const long m = blockIdx.x / pieces;
   const int c = ((int)(blockIdx.x - m * pieces) * 256 + threadIdx.x) * VEC;
   const int slots = a.weights ? a.topk : 1;
+  const int splits = a.counts[2 + a.which];
   // lane j: slot j of the row
   int my_p = -1, my_e = 0;
   float my_scale = 0.f, my_w = 1.f;
@@ -959,7 +961,7 @@ combine_kernel(const CombineArgs a) {
       v[i] = 0;
     }
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < splits; ++s) {
       const int32_t* src = a.planes + ((size_t)s * a.rows + p) * a.N + c;
       if constexpr (VEC == 4) {
         const uint4 q = ld_stream_v4(src);
@@ -1070,17 +1072,26 @@ static int pick_bn(long pairs, int E, int w_kind) {
   return mean <= 12 ? 32 : mean <= 40 ? 64 : 128;
 }
 
-// K-ranges of a product: only where the tiles of the experts that can be reached leave half of the CTA slots free, and with four
-// k-steps a range at least.
-static int pick_splits(long pairs, int E, int bn, int N, int K) {
-  if (bn > 128) return 1;   // the pair kernel takes whole tiles
+// Whether a product's k may be cut, and into how many ranges at most, from the tiles that evenly chosen experts would make: where
+// cutting shortens the time by a fifth (the planes are read again, by a pass behind the product), four k-steps a range at
+// least, with room for twice the ranges in case the tokens choose fewer experts than that.
+static SplitRule split_rule(long pairs, int E, int bn, int N, int K) {
+  SplitRule r;
+  r.n_tiles = (N + 127) / 128;
+  r.kt = K / 128;
+  r.most = 1;
+  if (bn > 128) return r;   // the pair kernel takes whole tiles
   const long reached = pairs < E ? pairs : E;
-  const long tiles = reached * ((pairs / reached + bn - 1) / bn) * ((N + 127) / 128);
-  const long slots = 2L * sm_count();
-  int S = (int)(slots / tiles);
-  if (S > K / 512) S = K / 512;
-  if (S > 16) S = 16;
-  return S < 1 ? 1 : S;
+  const long tiles = reached * ((pairs / reached + bn - 1) / bn);
+  const int slots = 2 * sm_count(), room = K / 512 < 16 ? K / 512 : 16;
+  SplitRule all = r;
+  all.most = room;
+  const int s = room > 1 ? best_splits(tiles, all, slots) : 1;
+  if (s <= 1) return r;
+  auto cost = [&](int n) { return (tiles * r.n_tiles * n + slots - 1) / slots * ((r.kt + n - 1) / n + 6); };
+  if (cost(s) * 5 > cost(1) * 4) return r;
+  r.most = 2 * s < room ? 2 * s : room;
+  return r;
 }
 
 static size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
@@ -1097,9 +1108,13 @@ struct Carver {
   }
 };
 
-static Plan carve_plan(Carver& c, long pairs, int E, int w_kind) {
+// `N1`, `K1` and `N2`, `K2`: the products that use the plan (N2 = 0: one).
+static Plan carve_plan(Carver& c, long pairs, int E, int w_kind, int N1, int K1, int N2, int K2) {
   Plan p;
   p.bn = pick_bn(pairs, E, w_kind);
+  p.slots = 2 * sm_count();
+  p.rule[0] = split_rule(pairs, E, p.bn, N1, K1);
+  p.rule[1] = N2 ? split_rule(pairs, E, p.bn, N2, K2) : SplitRule{1, 1, 1};
   p.counts = c.take<int>(4);
   p.tiles = c.take<int4>((size_t)max_tiles(pairs, E, p.bn));
   p.pos_of_pair = c.take<int>((size_t)pairs);
@@ -1111,16 +1126,15 @@ struct LinearBuffers {
   Plan plan;
   int8_t* xq;
   float* ascale;
-  int32_t* planes;
-  int splits;
+  int32_t* planes;   // null: k stays whole
 };
 static LinearBuffers carve_linear(Carver& c, long pairs, int E, int N, int K, int w_kind) {
   LinearBuffers b;
-  b.plan = carve_plan(c, pairs, E, w_kind);
-  b.splits = pick_splits(pairs, E, b.plan.bn, N, K);
+  b.plan = carve_plan(c, pairs, E, w_kind, N, K, 0, 0);
+  const int most = b.plan.rule[0].most;
   b.xq = c.take<int8_t>((size_t)pairs * K);
   b.ascale = c.take<float>((size_t)pairs);
-  b.planes = b.splits > 1 ? c.take<int32_t>((size_t)b.splits * pairs * N) : nullptr;
+  b.planes = most > 1 ? c.take<int32_t>((size_t)most * pairs * N) : nullptr;
   return b;
 }
 
@@ -1129,22 +1143,20 @@ struct MlpBuffers {
   int8_t *xq, *hq;
   float *ascale, *hscale, *h;
   unsigned* amax;
-  int32_t *planes1, *planes2;
-  int splits1, splits2;
+  int32_t *planes1, *planes2;   // planes1 null: the product leaves h; planes2: the scaled rows where k stays whole
 };
 static MlpBuffers carve_mlp(Carver& c, long pairs, int E, int H, int I, int w_kind) {
   MlpBuffers b;
-  b.plan = carve_plan(c, pairs, E, w_kind);
-  b.splits1 = pick_splits(pairs, E, b.plan.bn, 2 * I, H);
-  b.splits2 = pick_splits(pairs, E, b.plan.bn, H, I);
+  b.plan = carve_plan(c, pairs, E, w_kind, 2 * I, H, H, I);
+  const int most1 = b.plan.rule[0].most, most2 = b.plan.rule[1].most;
   b.xq = c.take<int8_t>((size_t)pairs * H);
   b.ascale = c.take<float>((size_t)pairs);
   b.hq = c.take<int8_t>((size_t)pairs * I);
   b.hscale = c.take<float>((size_t)pairs);
-  b.planes1 = b.splits1 > 1 ? c.take<int32_t>((size_t)b.splits1 * pairs * 2 * I) : nullptr;
-  b.h = b.splits1 > 1 ? nullptr : c.take<float>((size_t)pairs * I);
-  b.amax = b.splits1 > 1 ? nullptr : c.take<unsigned>((size_t)pairs);
-  b.planes2 = c.take<int32_t>((size_t)b.splits2 * pairs * H);
+  b.planes1 = most1 > 1 ? c.take<int32_t>((size_t)most1 * pairs * 2 * I) : nullptr;
+  b.h = most1 > 1 ? nullptr : c.take<float>((size_t)pairs * I);
+  b.amax = most1 > 1 ? nullptr : c.take<unsigned>((size_t)pairs);
+  b.planes2 = c.take<int32_t>((size_t)most2 * pairs * H);
   return b;
 }
 
@@ -1238,7 +1250,7 @@ int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_pe
   p.E = E;
   p.N = N;
   p.K = K;
-  p.splits = b.splits;
+  p.which = 0;
   p.out_mode = b.planes ? kOutPlanes : kOutPairs;
   p.out_dtype = out_dtype;
   p.out = b.planes ? static_cast<void*>(b.planes) : y;
@@ -1254,7 +1266,8 @@ int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_pe
   k.rows = k.outs = pairs;
   k.N = N;
   k.topk = topk;
-  k.splits = b.splits;
+  k.counts = b.plan.counts;
+  k.which = 0;
   k.out_dtype = out_dtype;
   return run_combine(k, st);
 }
@@ -1300,7 +1313,7 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   p.E = E;
   p.N = 2 * I;
   p.K = H;
-  p.splits = b.splits1;
+  p.which = 0;
   p.out_mode = b.planes1 ? kOutPlanes : kOutGated;
   p.out = b.planes1 ? static_cast<void*>(b.planes1) : b.h;
   p.amax = b.amax;
@@ -1318,7 +1331,6 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   h.hscale = b.hscale;
   h.rows = pairs;
   h.I = I;
-  h.splits = b.splits1;
   if (int rc = run_hidden(h, st)) return rc;
   p.w = w2;
   p.s1 = s2;
@@ -1326,8 +1338,8 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   p.ascale = b.hscale;
   p.N = H;
   p.K = I;
-  p.splits = b.splits2;
-  if (b.splits2 == 1) {
+  p.which = 1;
+  if (b.plan.rule[1].most == 1) {
     // whole k-ranges: scaled rows in the tokens' order, in the bytes of one plane
     p.out_mode = kOutPairs;
     p.out_dtype = LQ_DT_F32;
@@ -1350,7 +1362,8 @@ int lq_experts_mlp(const void* x, int x_dtype, const float* weights, const int32
   k.outs = T;
   k.N = H;
   k.topk = topk;
-  k.splits = b.splits2;
+  k.counts = b.plan.counts;
+  k.which = 1;
   k.out_dtype = out_dtype;
   return run_combine(k, st);
 }
