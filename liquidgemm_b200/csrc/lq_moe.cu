@@ -443,10 +443,14 @@ plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
   // thread e: the pairs of expert e, and how many of them lie before each warp's share
   const int e = threadIdx.x;
   int n = 0, tiles = 0;
+  int share_of[kPlanWarps];
   if (e < E) {
+#pragma unroll
+    for (int w = 0; w < kPlanWarps; ++w) share_of[w] = hist[w * E + e];
+#pragma unroll
     for (int w = 0; w < kPlanWarps; ++w) {
-      const int c = hist[w * E + e];
-      hist[w * E + e] = n;
+      const int c = share_of[w];
+      share_of[w] = n;
       n += c;
     }
     tiles = (n + plan.bn - 1) / plan.bn;
@@ -464,7 +468,8 @@ plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
   for (int w = 0; w < warp; ++w) ra += sums[0][w], rb += sums[1][w];
   const int row0 = ra + a - n, tile0 = rb + b - tiles;
   if (e < E) {
-    for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] += row0;
+#pragma unroll
+    for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] = share_of[w] + row0;
     write_tiles(plan, tile0, e, row0, n, tiles);
   }
   if (threadIdx.x == blockDim.x - 1) write_counts(plan, rb + b, ra + a);
@@ -1065,11 +1070,15 @@ static int run_weighted_sum(const float* rows, const float* weights, const int* 
 // ---------------------------------------------------------------------------------------------
 // sizes
 // ---------------------------------------------------------------------------------------------
-// Rows of a tile: what an expert gets on average, with room for the uneven choice of a router.
+// Rows of a tile, by what an expert gets on average (the router's choice is uneven: a tile holds twice that and more).  Measured
+// on 8 x 28672 x 4096, 64 x 2048 x 2048 and 16 x 4096 x 4096 with uneven experts, tiles of 32 / 64 / 128 rows and the pair
+// kernel, us.  4-bit: 8 rows on average 82 / 85 / 92 / 101 (28672 x 4096), 24 rows 113 / 102 / 101 / 121, 40 rows 160 / 112 / 111 /
+// 133, 128 rows 410 / 246 / 167 / 180, 192 rows 620 / 381 / 279 / 229.  INT8, whose operands need no unpacking: 8 rows 170 / 155 /
+// 164 / 159, 32 rows 217 / 186 / 169 / 166, 48 rows 257 / 195 / 178 / 153, 192 rows 630 / 433 / 333 / 281.
 static int pick_bn(long pairs, int E, int w_kind) {
   const long mean = pairs / E;
-  if (mean >= 96) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
-  return mean <= 12 ? 32 : mean <= 40 ? 64 : 128;
+  if (mean >= (w_kind == kBlob ? 144 : 45)) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
+  return mean <= 10 ? 32 : mean <= 32 ? 64 : 128;
 }
 
 // Whether a product's k may be cut, and into how many ranges at most, from the tiles that evenly chosen experts would make: where
