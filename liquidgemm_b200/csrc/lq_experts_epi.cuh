@@ -112,7 +112,7 @@ __device__ __forceinline__ void store_rows(const EpiArgs& a, const int (&v)[16],
     // the rows' largest magnitudes over the warp's 16 hidden channels: after three halving steps every lane holds one row
     float m[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = fabsf(h[j]);
+    for (int j = 0; j < 8; ++j) m[j] = fmaxf(fabsf(h[j]), 0.f);   // a NaN counts as zero, as in the row quantisers
 #pragma unroll
     for (int w = 4; w >= 1; w >>= 1) {
       const bool up = lane & (8 / w);   // lane bits 1, 2, 3

@@ -1173,6 +1173,7 @@ static MlpBuffers carve_mlp(Carver& c, long pairs, int E, int H, int I, int w_ki
 static int check_sizes(long T, int topk, int E, int N, int K) {
   if (T < 1 || topk < 1 || E < 1 || N < 1 || K < 1) return LQ_ERR_BAD_ARG;
   if (topk > kMaxTopk || E > kMaxExperts || K % 128) return LQ_ERR_SHAPE;
+  if (K >= 131072) return LQ_ERR_SHAPE;   // 2^17 products of -128 and -128 do not fit an int32 sum
   if (T * topk > (1L << 24) || (long)E * ((N + 127) / 128 * 128) > 0x7fffffffL) return LQ_ERR_SHAPE;
   return LQ_OK;
 }

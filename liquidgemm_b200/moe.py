@@ -82,6 +82,7 @@ def _weights(w: torch.Tensor, s1: torch.Tensor, N: int, K: int, name: str):
     E = s1.shape[0]
     _req(1 <= E <= MAX_EXPERTS, f"1..{MAX_EXPERTS} experts")
     _req(N >= 1 and K >= 128 and K % 128 == 0, f"{name}: K % 128 == 0 required")
+    _req(K < 131072, f"{name}: K below 131072 required (int32 sums)")
     if w.dtype == torch.uint8:
         need = E * ((N + 127) // 128) * (K // 128) * TILE_BYTES
         _req(w.numel() == need, f"{name} must hold {E} tile blobs for N={N}, K={K} ({need} bytes, got {w.numel()})")

@@ -166,6 +166,93 @@ def test_mlp(moe, w4, T, E, k, H, inner, how):
         _check_mlp(moe, T, E, k, H, inner, w4, how, dtype, T + E)
 
 
+# rows of each expert; with 144 rows on average (45 with INT8 weights) the pair kernel runs, whose tiles are 192 (256) rows at most
+COUNTS = [
+    [1, 400, 0, 250], [193, 192, 191, 31], [255, 256, 257, 33], [385, 513, 0, 1], [577, 0, 0, 0], [161, 129, 97, 224],
+    [0, 32, 64, 600], [96, 48, 16, 450],
+]
+
+
+@pytest.mark.parametrize("w4", [True, False], ids=["w4", "int8"])
+@pytest.mark.parametrize("counts", COUNTS)
+def test_every_tile_width(moe, w4, counts):
+    """Linear and MLP where the experts' rows end just behind, at and ahead of tile borders; channels an odd number of 128."""
+    E, K, N = len(counts), 256, 384
+    ids = torch.cat([torch.full((c,), e, dtype=torch.int32) for e, c in enumerate(counts)]).cuda()
+    ids = ids[torch.randperm(len(ids), device="cuda", generator=_gen(len(ids)))][:, None].contiguous()
+    layer, q, s1 = _stack(moe, E, N, K, w4, 5)
+    x = _rows((len(ids), K), torch.bfloat16, 6)
+    xq, scale = _quantise(x)
+    assert torch.equal(moe.experts_linear(x, ids, layer), _linear(xq, scale, ids, q, s1, False, torch.bfloat16))
+    w13, q13, s13 = _stack(moe, E, 2 * 128, K, w4, 7, gated=True)
+    w2, q2, s2 = _stack(moe, E, K, 128, w4, 8)
+    weights = torch.rand(len(ids), 1, device="cuda", generator=_gen(9))
+    want, tol = _mlp(x, weights, ids, q13, s13, q2, s2)
+    y = moe.experts_mlp(x, weights, ids, w13, w2)
+    assert torch.all((y.double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol) + 1e-30)
+
+
+@pytest.mark.parametrize("w4", [True, False], ids=["w4", "int8"])
+@pytest.mark.parametrize("T,E,k,N,K", [(64, 64, 1, 256, 4096), (200, 100, 2, 128, 8192), (7, 16, 3, 1024, 2048)])
+def test_fewer_experts_than_expected(moe, w4, T, E, k, N, K):
+    """All tokens choose one expert of many, so that k is cut more often than the sizes alone would have it; and the even choice."""
+    layer, q, s1 = _stack(moe, E, N, K, w4, T)
+    x = _rows((T, K), torch.float16, 2)
+    xq, scale = _quantise(x)
+    for how in ("one", "random"):
+        ids = _ids(T, E, k, T, how)
+        assert torch.equal(moe.experts_linear(x, ids, layer), _linear(xq, scale, ids, q, s1, False, torch.float16))
+
+
+@pytest.mark.parametrize("dtype,K", [(torch.bfloat16, 65536 + 128), (torch.float32, 32768 + 256), (torch.float16, 130944)])
+def test_rows_too_long_for_registers(moe, dtype, K):
+    layer, q, s1 = _stack(moe, 2, 65, K, True, 3)
+    x = _rows((5, K), dtype, 4)
+    for T in (1, 5):
+        ids = _ids(T, 2, 2, 5)
+        xq, scale = _quantise(x[:T])
+        assert torch.equal(moe.experts_linear(x[:T], ids, layer), _linear(xq, scale, ids, q, s1, False, dtype))
+
+
+def test_largest_sums(moe):
+    """Every product at its largest magnitude: the int32 sums of the longest rows."""
+    K = 130944
+    layer = {"w": torch.full((1, 128, K), -128, dtype=torch.int8, device="cuda"), "s1": torch.ones(1, 128, device="cuda"), "E": 1, "N": 128,
+             "K": K, "gated": False}
+    x = torch.full((3, K), -128, dtype=torch.int8, device="cuda")
+    y = moe.experts_linear(x, torch.zeros(3, 1, dtype=torch.int32, device="cuda"), layer, ascale=torch.ones(3, device="cuda"), out_dtype=torch.float32)
+    assert torch.all(y == float(128 * 128 * K))
+
+
+def test_groups_of_128(moe):
+    from liquidgemm_b200 import quant
+    w = (torch.randn(2, 192, 512, device="cuda", generator=_gen(1)) * 0.05).to(torch.bfloat16)
+    x, ids = _rows((40, 512), torch.bfloat16, 2), _ids(40, 2, 2, 3)
+    xq, scale = _quantise(x)
+    ref = [quant.quantize_weight(w[e].float().cpu(), group_size=128) for e in range(2)]
+    q = torch.stack([quant.dequantize_i8(r).cuda().double() for r in ref])
+    s1 = torch.stack([r.s1.cuda() for r in ref])
+    for w4 in (True, False):
+        assert torch.equal(moe.experts_linear(x, ids, moe.quantize_experts(w, w4=w4, group_size=128)),
+                           _linear(xq, scale, ids, q, s1, False, torch.bfloat16))
+
+
+@pytest.mark.parametrize("w4", [True, False], ids=["w4", "int8"])
+@pytest.mark.parametrize("T", [3, 40, 700])
+def test_infinite_rows_of_the_mlp_stay_with_their_tokens(moe, w4, T):
+    w13, w2 = _layer(moe, 3, 256, 1024, w4, 31)
+    x, ids, weights = _rows((T, 256), torch.float32, 5), _ids(T, 3, 2, 6), torch.rand(T, 2, device="cuda", generator=_gen(7))
+    clean = moe.experts_mlp(x, weights, ids, w13, w2)
+    bad = x.clone()
+    bad[0, 3], bad[2, 0] = float("inf"), float("nan")
+    got = moe.experts_mlp(bad, weights, ids, w13, w2)
+    keep = torch.ones(T, dtype=torch.bool, device="cuda")
+    keep[[0, 2]] = False
+    assert torch.equal(got[keep], clean[keep])
+    bad[2, 0] = 0.0
+    assert torch.equal(moe.experts_mlp(bad, weights, ids, w13, w2)[2], got[2])      # a NaN counts as zero
+
+
 def test_quantised_stacks_are_those_of_the_dense_linear(moe):
     from liquidgemm_b200 import ops
     w = (torch.randn(3, 200, 256, device="cuda", generator=_gen(1)) * 0.05).to(torch.bfloat16)

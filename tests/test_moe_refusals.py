@@ -39,7 +39,7 @@ def test_linear_bad_arguments(change):
 
 
 @pytest.mark.parametrize("change", [dict(K=192), dict(topk=33), dict(E=513), dict(T=1 << 24), dict(x=P + 8), dict(w=P + 4),
-                                    dict(E=512, N=1 << 23)])
+                                    dict(E=512, N=1 << 23), dict(K=131072)])
 def test_linear_bad_shapes(change):
     assert _linear(**change) == SHAPE
 
@@ -66,7 +66,7 @@ def test_mlp_bad_arguments(change):
     assert _mlp(**change) == BAD_ARG
 
 
-@pytest.mark.parametrize("change", [dict(H=200), dict(inner=192), dict(topk=33), dict(E=513), dict(T=1 << 24), dict(inner=1 << 30),
+@pytest.mark.parametrize("change", [dict(H=200), dict(inner=192), dict(H=131072), dict(inner=131072), dict(topk=33), dict(E=513), dict(T=1 << 24), dict(inner=1 << 30),
                                     dict(x=P + 8), dict(w13=P + 8), dict(w2=P + 8), dict(s13=P + 4), dict(s2=P + 4),
                                     dict(y=P + 8)])
 def test_mlp_bad_shapes(change):
@@ -124,3 +124,9 @@ def test_fake_kernels_give_the_shapes():
         assert y.shape == (5, 3, 256) and y.dtype == torch.float16
         z = torch.ops.liquidgemm.experts_mlp(x, w, ids, q, s, q, s, 0)
         assert z.shape == (5, 256) and z.dtype == torch.bfloat16
+        # the entry points themselves, on tensors that are not ordinary ones
+        layer = {"w": q, "s1": s, "N": 256, "K": 256, "gated": False}
+        w, ids = moe.route(logits, 3, scoring="sigmoid")
+        assert w.shape == (5, 3)
+        assert moe.experts_linear(x, ids, layer).shape == (5, 3, 256)
+        assert moe.experts_mlp(x, w, ids, dict(layer, gated=True), layer).shape == (5, 256)
