@@ -204,6 +204,25 @@ def test_fewer_experts_than_expected(moe, w4, T, E, k, N, K):
         assert torch.equal(moe.experts_linear(x, ids, layer), _linear(xq, scale, ids, q, s1, False, torch.float16))
 
 
+# pair kernel, long k: fewer tiles than pairs, and a few tiles behind full rounds
+@pytest.mark.parametrize("w4", [True, False], ids=["w4", "int8"])
+@pytest.mark.parametrize("T,E,N,K", [(200, 1, 256, 8192), (150, 1, 384, 14336), (700, 2, 640, 4096), (900, 3, 6400, 4096), (577, 1, 9600, 6144)])
+def test_long_k_and_partial_rounds(moe, w4, T, E, N, K):
+    layer, q, s1 = _stack(moe, E, N, K, w4, T)
+    ids = _ids(T, E, 1, T)
+    x = _rows((T, K), torch.bfloat16, 2)
+    xq, scale = _quantise(x)
+    want = _linear(xq, scale, ids, q, s1, False, torch.bfloat16)
+    for _ in range(5):
+        assert torch.equal(moe.experts_linear(x, ids, layer), want)
+
+
+@pytest.mark.parametrize("w4", [True, False], ids=["w4", "int8"])
+@pytest.mark.parametrize("T,E,H,inner", [(300, 1, 4096, 128), (300, 1, 128, 4096), (650, 2, 4096, 4096)])
+def test_mlp_of_long_and_short_k(moe, w4, T, E, H, inner):
+    _check_mlp(moe, T, E, 1, H, inner, w4, "random", torch.bfloat16, T)
+
+
 @pytest.mark.parametrize("dtype,K", [(torch.bfloat16, 65536 + 128), (torch.float32, 32768 + 256), (torch.float16, 130944)])
 def test_rows_too_long_for_registers(moe, dtype, K):
     layer, q, s1 = _stack(moe, 2, 65, K, True, 3)
