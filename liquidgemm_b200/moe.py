@@ -55,6 +55,10 @@ def _f_mlp(x, weights, ids, w13, s13, w2, s2, out_dtype):
     return x.new_empty(x.shape, dtype=_OUT_DTYPES[int(out_dtype)])
 
 
+def _refuse(msg: str):
+    raise RuntimeError(msg)
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous and on a 16-byte boundary (a view may start anywhere in its storage)."""
     t = t.contiguous()
@@ -63,13 +67,14 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _same_device(first, **others):
     for name, t in others.items():
-        _req(t is None or t.device == first.device, f"{name} must be on the device of the first argument")
+        t is None or t.device == first.device or _refuse(f"{name} must be on the device of the first argument")
 
 
 def _ids(ids: torch.Tensor) -> torch.Tensor:
     _req(ids.is_cuda and ids.dim() == 2 and ids.dtype in (torch.int32, torch.int64), "ids must be a CUDA [T, topk] tensor of int32 or int64")
-    _req(1 <= ids.shape[1] <= MAX_TOPK, f"topk must be 1..{MAX_TOPK}")
-    _req(ids.numel() <= MAX_PAIRS, f"at most {MAX_PAIRS} (token, expert) pairs")
+    # (messages with values are put together only where one is raised: a call of these costs the host as much as a kernel)
+    1 <= ids.shape[1] <= MAX_TOPK or _refuse(f"topk must be 1..{MAX_TOPK}")
+    ids.numel() <= MAX_PAIRS or _refuse(f"at most {MAX_PAIRS} (token, expert) pairs")
     if ids.dtype == torch.int64:
         ids = ids.clamp(-1, MAX_EXPERTS).to(torch.int32)   # what is no expert stays none
     return ids.contiguous()
@@ -77,17 +82,20 @@ def _ids(ids: torch.Tensor) -> torch.Tensor:
 
 def _weights(w: torch.Tensor, s1: torch.Tensor, N: int, K: int, name: str):
     """(kind, w, s1, E) of one stack of expert matrices [E, N, K]."""
-    _req(w.is_cuda and w.dtype in (torch.uint8, torch.int8), f"{name} must be a CUDA tensor: uint8 tile blobs or int8 rows")
-    _req(s1.is_cuda and s1.dtype == torch.float32 and s1.dim() == 2 and s1.shape[1] == N, f"the scales of {name} must be CUDA float32 [E, {N}]")
+    dtype = w.dtype
+    w.is_cuda and (dtype is torch.uint8 or dtype is torch.int8) or \
+        _refuse(f"{name} must be a CUDA tensor: uint8 tile blobs or int8 rows")
+    s1.is_cuda and s1.dtype is torch.float32 and s1.dim() == 2 and s1.shape[1] == N or \
+        _refuse(f"the scales of {name} must be CUDA float32 [E, {N}]")
     E = s1.shape[0]
-    _req(1 <= E <= MAX_EXPERTS, f"1..{MAX_EXPERTS} experts")
-    _req(N >= 1 and K >= 128 and K % 128 == 0, f"{name}: K % 128 == 0 required")
-    _req(K < 131072, f"{name}: K below 131072 required (int32 sums)")
-    if w.dtype == torch.uint8:
+    1 <= E <= MAX_EXPERTS or _refuse(f"1..{MAX_EXPERTS} experts")
+    N >= 1 and K >= 128 and K % 128 == 0 or _refuse(f"{name}: K % 128 == 0 required")
+    K < 131072 or _refuse(f"{name}: K below 131072 required (int32 sums)")
+    if dtype is torch.uint8:
         need = E * ((N + 127) // 128) * (K // 128) * TILE_BYTES
-        _req(w.numel() == need, f"{name} must hold {E} tile blobs for N={N}, K={K} ({need} bytes, got {w.numel()})")
+        w.numel() == need or _refuse(f"{name} must hold {E} tile blobs for N={N}, K={K} ({need} bytes, got {w.numel()})")
         return 0, _aligned(w), _aligned(s1), E
-    _req(w.numel() == E * N * K, f"{name} must be int8 [{E}, {N}, {K}]")
+    w.numel() == E * N * K or _refuse(f"{name} must be int8 [{E}, {N}, {K}]")
     return 1, _aligned(w), _aligned(s1), E
 
 
@@ -99,11 +107,12 @@ def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
 def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, renormalize, scale):
     _req(logits.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPE_CODES, "logits must be a 2-D CUDA tensor of bf16, fp16 or fp32")
     T, E = logits.shape
-    _req(1 <= E <= MAX_EXPERTS, f"1..{MAX_EXPERTS} experts")
+    1 <= E <= MAX_EXPERTS or _refuse(f"1..{MAX_EXPERTS} experts")
     _req(scoring in (0, 1) and group_score in (0, 1), "scoring and group_score must be 0 or 1")
     _req(n_group >= 1 and E % n_group == 0, "n_group must divide the number of experts")
     _req(1 <= topk_group <= n_group, "topk_group must be 1..n_group")
-    _req(1 <= topk <= min(MAX_TOPK, topk_group * (E // n_group)), f"topk must be 1..{MAX_TOPK} and at most the experts of topk_group groups")
+    1 <= topk <= min(MAX_TOPK, topk_group * (E // n_group)) or \
+        _refuse(f"topk must be 1..{MAX_TOPK} and at most the experts of topk_group groups")
     if bias is not None:
         _req(bias.is_cuda and bias.dtype == torch.float32 and bias.shape == (E,), "bias must be a CUDA float32 [E] tensor")
         _same_device(logits, bias=bias)
@@ -122,7 +131,7 @@ def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, re
 def _experts_linear(x, ascale, ids, w, s1, N, K, out_dtype):
     ids = _ids(ids)
     T, topk = ids.shape
-    _req(x.is_cuda and x.dim() in (2, 3) and x.shape[-1] == K, f"x must be a CUDA [T, {K}] or [T, topk, {K}] tensor")
+    x.is_cuda and x.dim() in (2, 3) and x.shape[-1] == K or _refuse(f"x must be a CUDA [T, {K}] or [T, topk, {K}] tensor")
     _req(tuple(x.shape[:-1]) in ((T,), (T, topk)), "x and ids must have the same tokens (and slots)")
     _req(int(out_dtype) in _OUT_DTYPES, "out_dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)")
     if ascale is None:
