@@ -7,6 +7,23 @@
 namespace lq {
 namespace experts {
 
+// The 128 codes of a weight row of a blob tile (four 16-byte chunks; step and offset of both groups in `meta`) as INT8, four a word in the
+// order of the operand's columns.  (The upper nibbles without a shift, as the upper half of (16 code) * (step << 28): 3 % slower, that
+// product has a quarter of the rate.)
+__device__ __forceinline__ void unpack_row(const uint4 (&ch)[4], uint32_t meta, uint32_t (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t m = c < 2 ? meta : meta >> 16;
+    const uint32_t step = m & 0xffu, ab = ((m >> 8) & 0xffu) * 0x01010101u;
+    const uint32_t pk[4] = {ch[c].x, ch[c].y, ch[c].z, ch[c].w};
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      v[8 * c + 2 * h] = lqq_dequant4(pk[h] & 0x0F0F0F0Fu, step, ab);
+      v[8 * c + 2 * h + 1] = lqq_dequant4((pk[h] >> 4) & 0x0F0F0F0Fu, step, ab);
+    }
+  }
+}
+
 // silu(g) * u.  The hidden values are quantised next, which turns an error of d counts into a wrong code with probability
 // d: expf (2 units in the last place) rather than the faster exponential, whose error grows with |g|.  The reciprocal
 // is the approximate one: one unit, against half of one and a dozen instructions for the division (in the pair kernel the
