@@ -210,8 +210,10 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       ptx::tc_fence_after();
       const uint32_t acc = tmem_acc + accring.s * BN;
       for (int kt = it.kb; kt < it.ke; ++kt) {
-        ok = ptx::mbar_wait_bounded(bar_full + 8 * ring.s, ring.ph, kWaitLimitNs);
-        if (ok && W4) ok = ptx::mbar_wait_bounded(bar_aready + 8 * tring.s, tring.ph, kWaitLimitNs);
+        // 4-bit weights: "operand ready" implies that the rows have landed (every unpacking thread saw its stage's full barrier, weights and
+        // rows, before it made the operand)
+        ok = W4 ? ptx::mbar_wait_bounded(bar_aready + 8 * tring.s, tring.ph, kWaitLimitNs)
+                : ptx::mbar_wait_bounded(bar_full + 8 * ring.s, ring.ph, kWaitLimitNs);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
           if (leader) atomicExch(args.status, 163);
