@@ -6,6 +6,8 @@
 // tiles x channel blocks x k-ranges and its rings run on from one item to the next: the copies and the unpacking of the next
 // item start while the sums of the last one are read out.  Item order: channel blocks fastest, so that the
 // CTAs at work at one time share a few row tiles, and the row tiles of one expert follow each other and find its weights in L2.
+// With few rows an expert the k-steps of all tiles may be dealt out in equal shares instead (cut_evenly says when): the two parts of a tile
+// that a share's end cuts are joined by whichever CTA comes second, through global memory, and nobody waits.
 //
 // A tile's width is what its rows need: the MMA's N is its rows in steps of 16 or 32, and the rows come in one box of BN or BN / 2
 // rows (one copy a k-step).  Rows of the box behind the tile's are those of the next expert, or zeros; their sums
@@ -47,6 +49,8 @@ struct Args {
   const int4* tiles;
   const int* pair_of_pos;
   EpiArgs epi;
+  int4* join;      // of the plan, for this product
+  int32_t* part;
   int* status;
   int N, kt_total, n_tiles, which;
 };
@@ -86,9 +90,43 @@ __device__ __forceinline__ Item item_of(const Args& a, int splits, int i, const 
   return it;
 }
 __device__ __forceinline__ int4 tile_of(const Args& a, int splits, int i) { return __ldcg(a.tiles + i / (a.n_tiles * splits)); }
-__device__ __forceinline__ Item item_at(const Args& a, int splits, int i) { return item_of(a, splits, i, tile_of(a, splits, i)); }
 
-template <int BN, int NS, bool W4, int MODE>
+// What a CTA has to do: the items blockIdx.x, blockIdx.x + grid, ... of all, or (`even`: k dealt out evenly, EVEN: that may be) the
+// k-steps [at, end) of all tiles in a row, whose first and last item may be parts.
+template <bool EVEN>
+struct Walk {
+  int at, end;
+  bool even;
+  __device__ __forceinline__ Walk(const Args& a, bool dealt, int items) : at(blockIdx.x), end(items), even(EVEN && dealt) {
+    if (even) {
+      const int total = items * a.kt_total, share = total / (int)gridDim.x, rest = total - share * (int)gridDim.x;
+      at = (int)blockIdx.x * share + ((int)blockIdx.x < rest ? (int)blockIdx.x : rest);
+      end = at + share + ((int)blockIdx.x < rest ? 1 : 0);
+    }
+  }
+  __device__ __forceinline__ bool more() const { return at < end; }
+  __device__ __forceinline__ int number(const Args& a) const { return even ? at / a.kt_total : at; }
+  __device__ __forceinline__ Item item(const Args& a, int splits, const int4& tile) const {
+    const int i = number(a);
+    Item it = item_of(a, splits, i, tile);
+    if (even) {
+      it.kb = at - i * a.kt_total;
+      it.ke = it.kb + (end - at) < a.kt_total ? it.kb + (end - at) : a.kt_total;
+    }
+    return it;
+  }
+  __device__ __forceinline__ Item item(const Args& a, int splits) const { return item(a, splits, tile_of(a, splits, number(a))); }
+  __device__ __forceinline__ void over(const Item& it) { at += even ? it.ke - it.kb : (int)gridDim.x; }
+};
+
+// The other part's sums of (up to) sixteen rows.
+__device__ __forceinline__ void add_part(int (&v)[16], const int32_t* other, int rows) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j < rows) v[j] += __ldcg(other + j * 128);
+}
+
+template <int BN, int NS, bool W4, int MODE, bool EVEN>
 __global__ void __launch_bounds__(Cfg<BN, NS, W4>::kThreads, 2)
 experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_xhalf,
                const __grid_constant__ CUtensorMap tmap_w, const Args args) {
@@ -147,8 +185,10 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   int4 tile = make_int4(0, 0, 0, 0);
   if (MODE != kOutPlanes && warp == 0) tile = tile_of(args, 1, blockIdx.x);
   const int4 counts = __ldcg(reinterpret_cast<const int4*>(args.counts));
-  const int splits = MODE != kOutPlanes ? 1 : args.which == 0 ? counts.z : counts.w;
+  const int cuts = args.which == 0 ? counts.z : counts.w;
+  const int splits = MODE != kOutPlanes ? 1 : cuts;
   const int items = counts.x * args.n_tiles * splits;
+  const bool dealt = EVEN && cuts == 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ copies
@@ -158,9 +198,10 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     Ring<NS> ring;
     int issued = 0;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      if (MODE == kOutPlanes || i != (int)blockIdx.x) tile = tile_of(args, splits, i);
-      const Item it = item_of(args, splits, i, tile);
+    for (Walk<EVEN> w(args, dealt, items); ok && w.more();) {
+      if (MODE == kOutPlanes || w.even || w.at != (int)blockIdx.x) tile = tile_of(args, splits, w.number(args));
+      const Item it = w.item(args, splits, tile);
+      w.over(it);
       const bool few = it.rows <= BN / 2;
       const uint32_t tx = (uint32_t)((few ? BN / 2 : BN) * 128 + C::kWStage);
       const uint8_t* src = W4 ? args.blob + ((size_t)((size_t)it.expert * args.n_tiles + it.nt) * args.kt_total + it.kb) * kBlobTile : nullptr;
@@ -198,8 +239,9 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     Ring<kNT> tring;
     Ring<C::kAcc> accring;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, splits, i);
+    for (Walk<EVEN> w(args, dealt, items); ok && w.more();) {
+      const Item it = w.item(args, splits);
+      w.over(it);
       const uint32_t idesc = ptx::idesc_i8((it.rows + C::kStep - 1) / C::kStep * C::kStep);
       ok = ptx::mbar_wait_bounded(bar_accfree + 8 * accring.s, accring.ph ^ 1u, kWaitLimitNs);
       ok = __all_sync(0xffffffffu, ok);
@@ -250,8 +292,9 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     Ring<kNT> tring;
     int turn = 0;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, splits, i);
+    for (Walk<EVEN> w(args, dealt, items); ok && w.more();) {
+      const Item it = w.item(args, splits);
+      w.over(it);
       // The set walks its own steps alone: with the other set's as iterations that do nothing the unpacking warps' issue slots cost
       // 4 % at one token.
       const int steps = it.ke - it.kb;
@@ -305,8 +348,9 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     int* pair = row_pair + (warp - kFirst) * kRows;
     Ring<C::kAcc> accring;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      const Item it = item_at(args, splits, i);
+    for (Walk<EVEN> w(args, dealt, items); ok && w.more();) {
+      const Item it = w.item(args, splits);
+      w.over(it);
       // What the epilogue needs beside the sums is requested ahead of them: behind the last MMA it would wait for the weight copies
       // of the next item, which fill the queues to memory (a channel scale read there cost 3 to 5 us an item).
       const int n = it.nt * 128 + row;
@@ -324,6 +368,18 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         }
         __syncwarp();
       }
+      // A part of a tile: this warp's sums go to memory, and the warp that comes second (the other CTA's, for the same channels and
+      // rows) adds both; it finds out ahead of its own sums, if it can.  Nobody waits.
+      const bool part = EVEN && it.ke - it.kb < args.kt_total;
+      const int side = it.kb > 0 ? 1 : 0, cut = (int)blockIdx.x - side;   // between the CTAs `cut` and `cut` + 1
+      int* here = reinterpret_cast<int*>(args.join + cut) + (warp - kFirst);
+      bool second = false;
+      if (part) {
+        int before = 0;
+        if (lane == 0) before = *reinterpret_cast<volatile int*>(here);
+        second = __shfl_sync(0xffffffffu, before, 0) != 0;
+        __threadfence();
+      }
       if (!ptx::mbar_wait_bounded(bar_accfull + 8 * accring.s, accring.ph, kWaitLimitNs)) {
         atomicExch(args.status, 166);
         ok = false;
@@ -333,11 +389,31 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       if (!ok) break;
       ptx::tc_fence_after();
       const uint32_t acc = tmem_acc + accring.s * BN + lane_addr;
+      if (part && !second) {
+        int32_t* mine = args.part + (size_t)((2 * cut + side) * BN) * 128 + row;
 #pragma unroll 1
-      for (int c0 = 16 * group, at = 0; c0 < it.rows; c0 += 16 * C::kGroups, at += 16) {
+        for (int c0 = 0; c0 < it.rows; c0 += 16) {
+          int v[16];
+          ptx::tmem_ld16(acc + c0, v);
+          ptx::tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < it.rows) mine[(c0 + j) * 128] = v[j];
+        }
+        __threadfence();
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) before = atomicAdd(here, 1);
+        second = __shfl_sync(0xffffffffu, before, 0) != 0;
+        __threadfence();
+      }
+      const int rows = part && !second ? 0 : it.rows;
+#pragma unroll 1
+      for (int c0 = 16 * group, at = 0; c0 < rows; c0 += 16 * C::kGroups, at += 16) {
         int v[16];
         ptx::tmem_ld16(acc + c0, v);
         ptx::tc_wait_ld();
+        if (part) add_part(v, args.part + (size_t)((2 * cut + 1 - side) * BN + c0) * 128 + row, it.rows - c0);
         store_rows<MODE>(args.epi, v, (long)it.row0 + c0, it.rows - c0, n, n_ok, w_scale, sc + at, pair + at, it.s);
       }
       ptx::tc_fence_before();
@@ -357,10 +433,10 @@ experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   }
 }
 
-template <int BN, int NS, bool W4, int MODE>
+template <int BN, int NS, bool W4, int MODE, bool EVEN = false>
 static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
   using C = Cfg<BN, NS, W4>;
-  auto kern = &experts_kernel<BN, NS, W4, MODE>;
+  auto kern = &experts_kernel<BN, NS, W4, MODE, EVEN>;
   static std::once_flag once[64];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -389,6 +465,8 @@ static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
   a.epi.rows = p.rows;
   a.epi.N = p.N;
   a.epi.out_dtype = p.out_dtype;
+  a.join = plan.join[p.which];
+  a.part = plan.part;
   a.status = status_word();
   a.N = p.N;
   a.kt_total = p.K / 128;
@@ -409,6 +487,11 @@ static int launch_mode(const Product& p, const Plan& plan, cudaStream_t st) {
 template <int BN, int NS, bool W4>
 static int launch_product(const Product& p, const Plan& plan, cudaStream_t st) {
   if (p.out_mode == kOutPlanes) return launch_mode<BN, NS, W4, kOutPlanes>(p, plan, st);
+  if constexpr (W4 && BN == kEvenRows) {
+    if (plan.rule[p.which].even)
+      return p.out_mode == kOutPairs ? launch_mode<BN, NS, W4, kOutPairs, true>(p, plan, st)
+                                     : launch_mode<BN, NS, W4, kOutGated, true>(p, plan, st);
+  }
   if (p.out_mode == kOutPairs) return launch_mode<BN, NS, W4, kOutPairs>(p, plan, st);
   return launch_mode<BN, NS, W4, kOutGated>(p, plan, st);
 }

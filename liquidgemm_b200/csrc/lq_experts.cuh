@@ -24,23 +24,34 @@ enum WeightKind { kBlob = 0, kInt8 = 1 };
 struct SplitRule {
   int n_tiles, kt;   // 128-channel blocks of an expert, k-steps
   int most;          // planes there is room for; 1: k stays whole
+  bool even;         // k whole: the k-steps of all tiles may be dealt out evenly (see cut_evenly)
 };
-// Cuts that give the shortest time: rounds of CTAs times k-steps of a range, with six steps for its start and end.
-__host__ __device__ inline int best_splits(long tiles, const SplitRule& r, int slots) {
-  int best = 1;
-  long least = 0;
-  for (int s = 1; s <= r.most; ++s) {
-    const long items = tiles * r.n_tiles * s;
-    const long cost = (items + slots - 1) / slots * ((r.kt + s - 1) / s + 6);
-    if (s == 1 || cost < least) best = s, least = cost;
-  }
-  return best;
+// Time of `s` ranges: rounds of CTAs times k-steps of a range, with six steps for its start and end.  Tiles times ranges fit 32 bits where
+// a product may be cut (the device divides 32 bits several times as fast as 64, and the product waits).
+__host__ __device__ inline unsigned split_cost(unsigned tiles, const SplitRule& r, int s, int slots) {
+  return (tiles * r.n_tiles * s + slots - 1) / slots * ((unsigned)(r.kt + s - 1) / s + 6);
+}
+// With k whole the CTAs' last round is seldom full.  Where that costs more than joining parts of tiles the k-steps of all tiles are
+// dealt out in equal, contiguous shares.  A share is a whole tile at least (more tiles than CTAs), so a tile has two parts at most.
+// The empty part of the last round counts half, a CTA alone on its SM being nearly twice as fast; against it stand the joins and
+// the order in which shares read memory, which cost more the more rounds there are.  Measured, one token, 4096 -> 28672, whole /
+// dealt out, us: 2 experts (1.5 rounds of CTAs) 29.3 / 27.2, 3 (2.3) 39.6 / 36.9, 4 (3.0) 46.0 / 45.7, 6 (4.5) 64.6 / 63.8, 8 (6.1) 79.2 /
+// 81.2; 8192 -> 28672: 50.5 / 45.2, 70.5 / 62.9, 85.0 / 79.8, 118.9 / 115.0, 150.7 / 149.6; 2048 -> 28672: 19.2 / 18.3, 23.9 / 23.8, 26.5 /
+// 28.0, 37.0 / 38.5, 44.1 / 47.3.  With INT8 weights, where the copies are all there is to do, 5 % slower.
+constexpr int kEvenRows = 32;    // for plans of this width, with 4-bit weights
+__host__ __device__ inline bool cut_evenly(long tiles, const SplitRule& r, int slots) {
+  const long items = tiles * r.n_tiles;
+  if (items <= slots || items > 8L * slots) return false;
+  const unsigned n = (unsigned)items, g = (unsigned)slots, rounds = (n + g - 1) / g;
+  return rounds * r.kt > (n * r.kt + g - 1) / g + 4 + 5 * rounds;
 }
 struct Plan {
-  int* counts;        // [4]: tiles, rows, k-ranges of the first product and of the second
+  int* counts;        // [4]: tiles, rows, k-ranges of the first product and of the second (0: dealt out evenly)
   int4* tiles;        // [max_tiles]
   int* pos_of_pair;   // [pairs]
   int* pair_of_pos;   // [pairs]
+  int4* join[2];      // [slots], zero before each product: for each epilogue warp, parts that are there of the tile cut between two CTAs
+  int32_t* part;      // [slots][2][bn][128]: their sums
   int bn, slots;      // slots: CTAs of the tile kernel that run together
   SplitRule rule[2];
 };

@@ -401,10 +401,27 @@ static int launch_route(const RouteArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------------
 // The tiles of expert e: as few as cover its n rows, and of equal widths in steps of 32 (a full tile and a narrow rest would
 // take as long as two full ones wherever the two run side by side).  Every one has a row: bn is a multiple of 32.
+// One warp; tiles and rows are lane 31's.  Each lane takes a number of ranges, the fewest of the best are kept.
 __device__ __forceinline__ void write_counts(const Plan& plan, int tiles, int rows) {
-  plan.counts[0] = tiles;
-  plan.counts[1] = rows;
-  for (int w = 0; w < 2; ++w) plan.counts[2 + w] = best_splits(tiles, plan.rule[w], plan.slots);
+  const int lane = threadIdx.x & 31;
+  tiles = __shfl_sync(0xffffffffu, tiles, 31);
+  int cuts[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    cuts[w] = 1;
+    if (plan.rule[w].most > 1) {
+      const unsigned cost = lane < plan.rule[w].most ? split_cost(tiles, plan.rule[w], lane + 1, plan.slots) : 0xffffffffu;
+      cuts[w] = __ffs(__ballot_sync(0xffffffffu, cost == __reduce_min_sync(0xffffffffu, cost)));
+    } else if (plan.rule[w].even && cut_evenly(tiles, plan.rule[w], plan.slots)) {
+      cuts[w] = 0;
+    }
+  }
+  if (lane == 31) *reinterpret_cast<int4*>(plan.counts) = make_int4(tiles, rows, cuts[0], cuts[1]);
+}
+__device__ __forceinline__ void clear_joins(const Plan& plan, int thread, int threads) {
+  for (int w = 0; w < 2; ++w)
+    if (plan.rule[w].even)
+      for (int i = thread; i < plan.slots; i += threads) plan.join[w][i] = make_int4(0, 0, 0, 0);
 }
 __device__ __forceinline__ void write_tiles(const Plan& plan, int tile0, int e, int row0, int n, int tiles) {
   if (tiles == 0) return;
@@ -427,6 +444,7 @@ plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
   dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kPlanWarps * E; i += blockDim.x) hist[i] = 0;
+  clear_joins(plan, threadIdx.x, blockDim.x);
   __syncthreads();
   const long share = ((pairs + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
   const long begin = warp * share, end = begin + share < pairs ? begin + share : pairs;
@@ -472,7 +490,7 @@ plan_kernel(const int* ids, long pairs, int E, const Plan plan) {
     for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] = share_of[w] + row0;
     write_tiles(plan, tile0, e, row0, n, tiles);
   }
-  if (threadIdx.x == blockDim.x - 1) write_counts(plan, rb + b, ra + a);
+  if (warp == kPlanWarps - 1) write_counts(plan, rb + b, ra + a);
   __syncthreads();
   for (long i0 = begin; i0 < end; i0 += 32 * kAhead) {
     int id[kAhead];
@@ -558,7 +576,7 @@ __device__ __forceinline__ void fetch_ids(const PlaceArgs& a, int* ids) {
   }
 }
 
-// Tiles and counts of the plan (one CTA of any size).
+// Tiles and counts of the plan (one CTA of at least two warps).
 __device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
   for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
@@ -572,7 +590,10 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
       if (e[q] >= 0 && e[q] < a.E) atomicAdd(&hist[e[q]], 1);
   }
   __syncthreads();
-  if (threadIdx.x >= 32) return;
+  if (threadIdx.x >= 32) {
+    clear_joins(a.plan, threadIdx.x - 32, blockDim.x - 32);
+    return;
+  }
   const int per = (a.E + 31) / 32;   // neighbouring experts of a lane
   const int lane = threadIdx.x;
   int rows = 0, tiles = 0;
@@ -587,7 +608,7 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
     const int pr = __shfl_up_sync(0xffffffffu, r, o), pt = __shfl_up_sync(0xffffffffu, t, o);
     if (lane >= o) r += pr, t += pt;
   }
-  if (lane == 31) write_counts(a.plan, t, r);
+  write_counts(a.plan, t, r);
   r -= rows;
   t -= tiles;
   for (int q = 0; q < per; ++q) {
@@ -1083,23 +1104,24 @@ static int pick_bn(long pairs, int E, int w_kind) {
 
 // Whether a product's k may be cut, and into how many ranges at most, from the tiles that evenly chosen experts would make: where
 // cutting shortens the time by a fifth (the planes are read again, by a pass behind the product), four k-steps a range at
-// least, with room for twice the ranges in case the tokens choose fewer experts than that.
-static SplitRule split_rule(long pairs, int E, int bn, int N, int K) {
+// least, with room for twice the ranges in case the tokens choose fewer experts than that.  What may be cut has a few rounds of
+// CTAs at most.
+static SplitRule split_rule(long pairs, int E, int bn, int w_kind, int N, int K) {
   SplitRule r;
   r.n_tiles = (N + 127) / 128;
   r.kt = K / 128;
   r.most = 1;
+  r.even = false;
   if (bn > 128) return r;   // the pair kernel takes whole tiles
   const long reached = pairs < E ? pairs : E;
   const long tiles = reached * ((pairs / reached + bn - 1) / bn);
   const int slots = 2 * sm_count(), room = K / 512 < 16 ? K / 512 : 16;
-  SplitRule all = r;
-  all.most = room;
-  const int s = room > 1 ? best_splits(tiles, all, slots) : 1;
-  if (s <= 1) return r;
-  auto cost = [&](int n) { return (tiles * r.n_tiles * n + slots - 1) / slots * ((r.kt + n - 1) / n + 6); };
-  if (cost(s) * 5 > cost(1) * 4) return r;
-  r.most = 2 * s < room ? 2 * s : room;
+  int s = 1;
+  if (tiles * r.n_tiles <= 8L * slots)
+    for (int n = 2; n <= room; ++n)
+      if (split_cost(tiles, r, n, slots) < split_cost(tiles, r, s, slots)) s = n;
+  if (s > 1 && split_cost(tiles, r, s, slots) * 5 <= split_cost(tiles, r, 1, slots) * 4) r.most = 2 * s < room ? 2 * s : room;
+  r.even = r.most == 1 && w_kind == kBlob && bn == kEvenRows && cut_evenly(tiles, r, slots);
   return r;
 }
 
@@ -1122,12 +1144,14 @@ static Plan carve_plan(Carver& c, long pairs, int E, int w_kind, int N1, int K1,
   Plan p;
   p.bn = pick_bn(pairs, E, w_kind);
   p.slots = 2 * sm_count();
-  p.rule[0] = split_rule(pairs, E, p.bn, N1, K1);
-  p.rule[1] = N2 ? split_rule(pairs, E, p.bn, N2, K2) : SplitRule{1, 1, 1};
+  p.rule[0] = split_rule(pairs, E, p.bn, w_kind, N1, K1);
+  p.rule[1] = N2 ? split_rule(pairs, E, p.bn, w_kind, N2, K2) : SplitRule{1, 1, 1, false};
   p.counts = c.take<int>(4);
   p.tiles = c.take<int4>((size_t)max_tiles(pairs, E, p.bn));
   p.pos_of_pair = c.take<int>((size_t)pairs);
   p.pair_of_pos = c.take<int>((size_t)pairs);
+  for (int w = 0; w < 2; ++w) p.join[w] = p.rule[w].even ? c.take<int4>((size_t)p.slots) : nullptr;
+  p.part = p.rule[0].even || p.rule[1].even ? c.take<int32_t>((size_t)p.slots * 2 * p.bn * 128) : nullptr;
   return p;
 }
 
