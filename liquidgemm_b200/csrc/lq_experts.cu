@@ -18,6 +18,10 @@
 // tensor memory and warps 10..13 the epilogue, with INT8 weights warps 2..5 and 6..9 two epilogue groups.  The epilogue of an item
 // (3 us for 16 rows with the gated activation: one warp's chain of latencies) runs beside the next item's main loop; with
 // the sets doing it themselves the weight stream stood still meanwhile (28672 x 4096, eight experts: 4 of 14 us per item).
+// Bound by the weights' stream with few rows: one expert of 37888 x 8192 (two items' k-steps a SM at all times) 29 us for 165 MB, 5.7
+// TB/s with start and end, 7 TB/s between (362 ns a pair of k-steps); what is left is the start (2 us to the first sums' operands),
+// the last round and the join.  One token through two of eight experts' 28672 x 4096: 28 us with the pass before it; the floor is 19.
+// A CTA alone on its SM takes 178 ns a k-step (unpacking, and the chain of waits from copy to MMA).
 // The stage counts are even wherever two sets take turns, so that a set sees every use of its stages.  All waits are bounded;
 // status codes 161-166.
 #include <cuda.h>

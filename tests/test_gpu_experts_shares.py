@@ -93,3 +93,15 @@ def test_two_streams(moe, stack):
 def test_mlp(moe, T, how):
     # 2 x 160 blocks of 22 k-steps in the first product
     _check_mlp(moe, T, 2, 2, 2816, 10240, True, how, torch.bfloat16, T)
+
+
+def test_many_experts(moe):
+    """More pairs than the placing kernel sorts by itself; every tile is another expert's."""
+    T, k, E, K = 300, 8, 300, 3584
+    layer, q, s1 = _stack(moe, E, 128, K, True, 8)
+    x = _rows((T, K), torch.float16, 3)
+    xq, scale = _quantise(x)
+    ids = torch.stack([(torch.arange(E, device="cuda") * 7 + 41 * j) % E for j in range(k)], dim=1).to(torch.int32)   # eight rows each
+    want = _linear(xq, scale, ids, q, s1, False, torch.float16)
+    for _ in range(3):
+        assert torch.equal(moe.experts_linear(x, ids, layer), want)
