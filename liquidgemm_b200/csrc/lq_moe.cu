@@ -590,8 +590,9 @@ __device__ __forceinline__ void fetch_ids(const PlaceArgs& a, int* ids) {
   }
 }
 
-// Tiles and counts of the plan (one CTA of at least two warps).
+// Tiles and counts of the plan (one CTA, of a single warp where the rows are short).
 __device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
+  clear_joins(a.plan, threadIdx.x, blockDim.x);
   for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
   constexpr int kAhead = 8;   // ids of a thread in flight
@@ -604,10 +605,7 @@ __device__ __forceinline__ void make_tiles(const PlaceArgs& a, int* hist) {
       if (e[q] >= 0 && e[q] < a.E) atomicAdd(&hist[e[q]], 1);
   }
   __syncthreads();
-  if (threadIdx.x >= 32) {
-    clear_joins(a.plan, threadIdx.x - 32, blockDim.x - 32);
-    return;
-  }
+  if (threadIdx.x >= 32) return;
   const int per = (a.E + 31) / 32;   // neighbouring experts of a lane
   const int lane = threadIdx.x;
   int rows = 0, tiles = 0;
