@@ -320,7 +320,8 @@ LQ_API int lq_i8_gemm_scaled_ws(const int8_t* a, const int8_t* b, const float* a
  * only those of the topk_group best groups can be chosen; a group ranks by its largest key (group_score 0) or by the sum of
  * its two largest (1), the lowest index among equals.  weights [T, topk] are the chosen scores (without bias), divided by their sum
  * with `renormalize`, times `scale`.  A logit of -inf or NaN takes its expert out of the choice (and adds nothing to the softmax);
- * where fewer than topk experts are left the remaining slots hold id -1 and weight 0.
+ * where fewer than topk experts are left the remaining slots hold id -1 and weight 0.  Weights are those of 64-bit scores: the ratio of
+ * small ones is kept, and where none of the chosen has a score that 64 bits hold all weights are 0.
  * E <= 512, topk <= 32, E % n_group == 0, topk <= topk_group * (E / n_group). */
 LQ_API int lq_moe_route(const void* logits, int logits_dtype, const float* bias, float* weights, int32_t* ids, int T,
                         int E, int topk, int scoring, int n_group, int topk_group, int group_score, int renormalize,

@@ -116,32 +116,44 @@ __device__ __forceinline__ S softmax_terms(const float (&l)[PER], float& top, S 
   return sum > 0 ? sum : (S)1;
 }
 
-// sigmoid(l), for a token with a choice below -80 (`tiny`) times 2^100: the ratio of such scores to others would be lost in the
-// denormal range.
-__device__ __forceinline__ float sigmoid_score(float l, bool tiny) {
-  if (tiny) return (float)(0x1p100 / (1.0 + exp(-(double)l)));
-  return __fdividef(1.f, 1.f + expf(-l));
-}
-
-// Lane j has choice j (id -1: none left) and what its score comes from: the logit of a sigmoid, or the score itself.
-__device__ __forceinline__ void store_choice(const RouteArgs& a, long t, int id, float from) {
+// Lane j has choice j (id -1: none left) and its logit l; softmax: `top` is the row's largest logit and `sum` the sum of exp(l - top) over all
+// its experts (not used with renormalize).
+//
+// Renormalised softmax weights need the chosen logits alone: exp(l - m) over its sum, m the largest of the chosen.  A choice whose score (or,
+// renormalised, weight) may lie near the end of float32's range, and only a row that has one, is worked out in float64: the ratio
+// of such scores would be lost among float32's denormals.  What has no score in 64 bits (more than 745 below the top; a sigmoid below -709) has
+// the weight 0.
+__device__ __forceinline__ void store_choice(const RouteArgs& a, long t, int id, float l, float top, float sum) {
   const int lane = threadIdx.x & 31;
-  bool tiny = false;
-  float score = from;
-  if (a.sigmoid) {
-    tiny = __any_sync(0xffffffffu, id >= 0 && from < -80.f);
-    score = sigmoid_score(from, tiny);
-  }
-  if (id < 0) score = 0.f;
-  if (a.renormalize) {
-    float total = score;
-    for (int o = 1; o < a.topk; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);   // (lanes behind the last slot hold 0)
-    if (total > 0.f) score = __fdiv_rn(score, total);
-  } else if (tiny) {
-    score *= 0x1p-100f;
+  const bool some = id >= 0;
+  float ref = top;
+  if (!a.sigmoid && a.renormalize) ref = number(__reduce_max_sync(0xffffffffu, some ? ordered(l) : 0u));
+  const bool scored = some && (a.sigmoid || ref == top || ref - top > -745.f);
+  float w = 0.f;
+  if (__any_sync(0xffffffffu, some && (a.sigmoid ? l < -80.f : l - ref < -80.f))) {
+    double s = 0.0;
+    if (scored) s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)l)) : l == ref ? 1.0 : exp((double)l - (double)ref);
+    double total = 1.0;
+    if (a.renormalize) {
+      total = s;
+      for (int o = 1; o < a.topk; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);   // (lanes behind the last slot hold 0)
+      if (!(total > 0.0)) total = 1.0;
+    } else if (!a.sigmoid) {
+      total = sum;
+    }
+    w = (float)(s / total * a.scale);
+  } else {
+    if (scored) w = a.sigmoid ? __fdividef(1.f, 1.f + expf(-l)) : l == ref ? 1.f : expf(l - ref);
+    float total = sum;
+    if (a.renormalize) {
+      total = w;
+      for (int o = 1; o < a.topk; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if ((a.renormalize || !a.sigmoid) && total > 0.f) w = __fdiv_rn(w, total);
+    w *= a.scale;
   }
   if (lane < a.topk) {
-    a.weights[t * a.topk + lane] = score * a.scale;
+    a.weights[t * a.topk + lane] = w;
     a.ids[t * a.topk + lane] = id;
   }
 }
@@ -250,12 +262,12 @@ route_logits_kernel(const RouteArgs a) {
       else my_l = number(best);
     }
   }
-  if (!a.sigmoid) {
-    float top, s[PER];
-    const float sum = softmax_terms<PER, float>(l, top, s);
-    my_l = __fdiv_rn(my_l == top ? 1.f : expf(my_l - top), sum);
+  float top = __shfl_sync(0xffffffffu, my_l, 0), sum = 1.f;   // the first choice is the row's largest logit: its group is the best
+  if (!a.sigmoid && !a.renormalize) {
+    float s[PER];
+    sum = softmax_terms<PER, float>(l, top, s);
   }
-  store_choice(a, t, my_id, my_l);
+  store_choice(a, t, my_id, my_l, top, sum);
 }
 
 // The warp's buffers of the kernel below.
@@ -270,7 +282,8 @@ struct RouteBuffers {
 // used), a softmax score by 31 * 2^-24 (argument |x| e^x < 0.4, exponential 2 units, sum of 16 terms and over 32 lanes, quotient;
 // 2^-18 is used), the key by another |v| 2^-24; two keys by twice that, two sums of two by four times.
 template <int PER, typename S>
-__device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float (&l)[PER], RouteBuffers<PER>& buf, int& my_id, float& my_from) {
+__device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float (&l)[PER], RouteBuffers<PER>& buf, int& my_id, float& my_l,
+                                                float& top, float& sum) {
   using Key = typename KeyOf<S>::type;
   constexpr bool kFast = sizeof(S) == 4;
   const int lane = threadIdx.x & 31;
@@ -284,10 +297,10 @@ __device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float 
       else s[i] = l[i] > kNone ? 1.0 / (1.0 + exp(-(double)l[i])) : 0.0;
     }
   } else {
-    float top;
-    const S sum = softmax_terms<PER, S>(l, top, s);
+    const S all = softmax_terms<PER, S>(l, top, s);
+    sum = (float)all;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = s[i] / sum;
+    for (int i = 0; i < PER; ++i) s[i] = s[i] / all;
   }
   Key key[PER];
   S largest = 1;
@@ -320,10 +333,10 @@ __device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float 
       if (e < a.E && !buf.kept[group_of(a, e)]) key[i] = 0;
     }
   }
-  // what the chosen ones' scores are taken from: the logit (a sigmoid is worked out again, a lane each) or the score
+  // the chosen ones' weights are worked out from their logits, a lane each
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < PER; ++i) values[lane + 32 * i] = a.sigmoid ? (S)l[i] : s[i];
+  for (int i = 0; i < PER; ++i) values[lane + 32 * i] = (S)l[i];
   __syncwarp();
   uint32_t last = 0;   // the choice before
   const bool check = kFast && by_score;
@@ -348,7 +361,7 @@ __device__ __forceinline__ bool choose_by_score(const RouteArgs& a, const float 
       if (id == lane + 32 * i) key[i] = 0;
     if (lane == j) my_id = id;
   }
-  if (my_id >= 0) my_from = (float)values[my_id];
+  if (my_id >= 0) my_l = (float)values[my_id];
   return true;
 }
 
@@ -364,13 +377,13 @@ route_scores_kernel(const RouteArgs a) {
   float l[PER];
   load_logits<T, PER>(a, t, l);
   int id = -1;
-  float from = 0.f;
-  if (!choose_by_score<PER, float>(a, l, buffers[warp], id, from)) {
+  float my_l = 0.f, top = 0.f, sum = 1.f;
+  if (!choose_by_score<PER, float>(a, l, buffers[warp], id, my_l, top, sum)) {
     __syncwarp();
     id = -1;
-    choose_by_score<PER, double>(a, l, buffers[warp], id, from);
+    choose_by_score<PER, double>(a, l, buffers[warp], id, my_l, top, sum);
   }
-  store_choice(a, t, id, from);
+  store_choice(a, t, id, my_l, top, sum);
 }
 
 template <typename T, int PER>
