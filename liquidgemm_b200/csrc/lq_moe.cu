@@ -165,6 +165,7 @@ template <typename S>
 __device__ __forceinline__ bool rank_groups(const RouteArgs& a, bool top2, const S* v, S* rank, uint8_t* kept, S near) {
   const int lane = threadIdx.x & 31;
   const int G = a.n_group, size = (int)a.group_size, L = a.group_lanes, shift = __ffs(L) - 1;
+  bool clear = true;
   for (int base = 0; base < G; base += 32 >> shift) {
     const int g = base + (lane >> shift);
     S m1 = kNone, m2 = kNone;
@@ -182,10 +183,13 @@ __device__ __forceinline__ bool rank_groups(const RouteArgs& a, bool top2, const
       m2 = least > m2 ? least : m2;
       m1 = m1 > b1 ? m1 : b1;
     }
-    if (g < G && (lane & (L - 1)) == 0) rank[g] = top2 && m2 > (S)kNone ? m1 + m2 : m1;
+    if (g < G && (lane & (L - 1)) == 0) {
+      const bool two = top2 && m2 > (S)kNone;
+      rank[g] = two ? m1 + m2 : m1;
+      if (two && near >= 0 && fabs(m1 + m2) == (S)INFINITY) clear = false;   // a sum beyond float32, maybe
+    }
   }
   __syncwarp();
-  bool clear = true;
   for (int g = lane; g < G; g += 32) {
     const S mine = rank[g];
     int before = 0;

@@ -90,3 +90,16 @@ def test_scores_that_vanish_in_64_bits(moe):
     assert ids.tolist() == [[0, 1, 2]] and not w.any()
     w, ids = moe.route(torch.tensor([[INF, -5.0, -6.0]], device="cuda"), 2, bias=torch.tensor([-INF, 1.0, 0.0], device="cuda"))
     assert ids.tolist() == [[1, 2]] and not w.any()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_sums_of_two_keys_beyond_float32(moe, scoring, sign):
+    """Groups ranked by sums that only 64 bits hold: biases near float32's largest number."""
+    l = torch.linspace(-2, 2, 4 * 12, device="cuda").view(4, 12).contiguous()
+    apart = torch.linspace(1.0, 0.97, 4, device="cuda")      # no two keys of a group are close
+    bias = torch.cat([sign * v * apart for v in (1.8e38, 3.0e38, 2.5e38)])
+    for kept in (1, 2):
+        check(moe, l, 3 * kept, scoring=scoring, bias=bias, n_group=3, topk_group=kept, group_score="top2")
+    bias[4:8] = sign * INF            # groups that are infinite in 64 bits too
+    check(moe, l, 3, scoring=scoring, bias=bias, n_group=3, topk_group=1 if sign > 0 else 2, group_score="top2")
