@@ -105,12 +105,12 @@ def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
 
 
 def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, renormalize, scale):
-    _req(logits.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPE_CODES, "logits must be a 2-D CUDA tensor of bf16, fp16 or fp32")
+    logits.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPE_CODES or _refuse("logits must be a 2-D CUDA tensor of bf16, fp16 or fp32")
     T, E = logits.shape
     1 <= E <= MAX_EXPERTS or _refuse(f"1..{MAX_EXPERTS} experts")
-    _req(scoring in (0, 1) and group_score in (0, 1), "scoring and group_score must be 0 or 1")
-    _req(n_group >= 1 and E % n_group == 0, "n_group must divide the number of experts")
-    _req(1 <= topk_group <= n_group, "topk_group must be 1..n_group")
+    scoring in (0, 1) and group_score in (0, 1) or _refuse("scoring and group_score must be 0 or 1")
+    n_group >= 1 and E % n_group == 0 or _refuse("n_group must divide the number of experts")
+    1 <= topk_group <= n_group or _refuse("topk_group must be 1..n_group")
     1 <= topk <= min(MAX_TOPK, topk_group * (E // n_group)) or \
         _refuse(f"topk must be 1..{MAX_TOPK} and at most the experts of topk_group groups")
     if bias is not None:
@@ -183,12 +183,22 @@ def _experts_mlp(x, weights, ids, w13, s13, w2, s2, out_dtype):
     return y
 
 
-def _plain_call(t: torch.Tensor) -> bool:
-    """Whether an operator may be called without torch's dispatcher: an ordinary tensor, nothing that traces or intercepts.  The
-    dispatcher's way into a Python kernel costs 4.5 us of the host's 17 for a router call, which is all that a small one
-    takes."""
-    return type(t) is torch.Tensor and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0 and \
-        not torch.jit.is_tracing() and t.is_cuda
+_ORDINARY = (torch.Tensor, torch.nn.Parameter)
+_is_compiling, _dispatch_modes, _tracing_state, _transform = (torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack,
+                                                              torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack)
+_forward_ad = torch.autograd.forward_ad
+
+
+def _plain_call(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether an operator may be called without torch's dispatcher: ordinary CUDA tensors that no gradient is asked of, and nothing
+    that traces, transforms or intercepts (under ``vmap`` and its like a wrapped tensor looks ordinary).  The dispatcher's way into
+    a Python kernel costs 4.5 us of the host's 17 for a router call, which is all that a small one takes."""
+    if _is_compiling() or _dispatch_modes() or _tracing_state() is not None or _transform() is not None or _forward_ad._current_level >= 0:
+        return False
+    for t in tensors:
+        if t is not None and (type(t) not in _ORDINARY or (t.requires_grad and torch.is_grad_enabled())):
+            return False
+    return tensors[0].is_cuda
 
 
 _impl.impl("moe_route", _moe_route)
@@ -209,9 +219,9 @@ def route(logits: torch.Tensor, topk: int, scoring: str = "softmax", bias: Optio
     can be chosen; a group ranks by its largest key (``group_score="max"``) or the sum of its two largest (``"top2"``).
     Weights are the scores without the bias, divided by their sum with ``renormalize``, times ``scale``.  A logit of -inf or NaN takes
     its expert out; slots for which no expert is left have id -1 and weight 0 (the products skip them)."""
-    _req(scoring in _SCORING, "scoring must be 'softmax' or 'sigmoid'")
-    _req(group_score in _GROUP_SCORE, "group_score must be 'max' or 'top2'")
-    run = _moe_route if _plain_call(logits) else torch.ops.liquidgemm.moe_route
+    scoring in _SCORING or _refuse("scoring must be 'softmax' or 'sigmoid'")
+    group_score in _GROUP_SCORE or _refuse("group_score must be 'max' or 'top2'")
+    run = _moe_route if _plain_call(logits, bias) else torch.ops.liquidgemm.moe_route
     return run(logits, bias, int(topk), _SCORING[scoring], int(n_group), int(topk_group), _GROUP_SCORE[group_score], bool(renormalize),
                float(scale))
 
@@ -261,8 +271,9 @@ def experts_linear(x: torch.Tensor, ids: torch.Tensor, layer: dict, ascale: Opti
     _req(not layer["gated"], "a gated stack is stored for experts_mlp")
     out_dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.int8 else x.dtype)
     _req(out_dtype in _DTYPE_CODES, "out_dtype must be bfloat16, float16 or float32")
-    run = _experts_linear if _plain_call(x) else torch.ops.liquidgemm.experts_linear
-    return run(x, ascale, ids, layer["w"], layer["s1"], layer["N"], layer["K"], _DTYPE_CODES[out_dtype])
+    w, s1 = layer["w"], layer["s1"]
+    run = _experts_linear if _plain_call(x, ascale, ids, w, s1) else torch.ops.liquidgemm.experts_linear
+    return run(x, ascale, ids, w, s1, layer["N"], layer["K"], _DTYPE_CODES[out_dtype])
 
 
 def experts_mlp(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w13: dict, w2: dict,
@@ -276,5 +287,6 @@ def experts_mlp(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, w13: 
     _req(w13["gated"] and not w2["gated"], "w13 must be quantised with gated=True and w2 without")
     out_dtype = out_dtype or x.dtype
     _req(out_dtype in _DTYPE_CODES, "out_dtype must be bfloat16, float16 or float32")
-    run = _experts_mlp if _plain_call(x) else torch.ops.liquidgemm.experts_mlp
-    return run(x, weights, ids, w13["w"], w13["s1"], w2["w"], w2["s1"], _DTYPE_CODES[out_dtype])
+    args = (x, weights, ids, w13["w"], w13["s1"], w2["w"], w2["s1"])
+    run = _experts_mlp if _plain_call(*args) else torch.ops.liquidgemm.experts_mlp
+    return run(*args, _DTYPE_CODES[out_dtype])
