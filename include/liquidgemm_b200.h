@@ -334,7 +334,7 @@ LQ_API int lq_moe_route(const void* logits, int logits_dtype, const float* bias,
  * lq_quant_per_token.  x: [T, K], or [T, topk, K] with x_per_pair; x_dtype LQ_DT_* (each row is
  * quantised as by lq_quant_per_token) or 3 = INT8 with one scale per row in x_scale (null otherwise).  w_kind 0: E tile blobs one
  * behind the other (lq_tile_blob_bytes(N, K) each), 1: INT8 [E, N, K].  s1 [E, N].  y [T, topk, N].
- * K % 128 == 0, K < 131072 (int32 sums), E <= 512, topk <= 32, T * topk <= 2^24; x, w and scratch 16-byte aligned.
+ * N < 2^30, K % 128 == 0, K < 131072 (int32 sums), E <= 512, topk <= 32, T * topk <= 2^24; x, w and scratch 16-byte aligned.
  * `scratch`: lq_experts_linear_scratch_bytes() bytes, any content (0 from that function: sizes out of range). */
 LQ_API size_t lq_experts_linear_scratch_bytes(int T, int topk, int E, int N, int K, int w_kind);
 LQ_API int lq_experts_linear(const void* x, int x_dtype, const float* x_scale, int x_per_pair, const int32_t* ids,

@@ -1228,6 +1228,7 @@ static int check_sizes(long T, int topk, int E, int N, int K) {
   if (T < 1 || topk < 1 || E < 1 || N < 1 || K < 1) return LQ_ERR_BAD_ARG;
   if (topk > kMaxTopk || E > kMaxExperts || K % 128) return LQ_ERR_SHAPE;
   if (K >= 131072) return LQ_ERR_SHAPE;   // 2^17 products of -128 and -128 do not fit an int32 sum
+  if (N >= 1 << 30) return LQ_ERR_SHAPE;  // the bytes of a row of 32-bit outputs are a 32-bit number
   if (T * topk > (1L << 24) || (long)E * ((N + 127) / 128 * 128) > 0x7fffffffL) return LQ_ERR_SHAPE;
   return LQ_OK;
 }

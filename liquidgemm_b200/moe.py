@@ -89,7 +89,7 @@ def _weights(w: torch.Tensor, s1: torch.Tensor, N: int, K: int, name: str):
         _refuse(f"the scales of {name} must be CUDA float32 [E, {N}]")
     E = s1.shape[0]
     1 <= E <= MAX_EXPERTS or _refuse(f"1..{MAX_EXPERTS} experts")
-    N >= 1 and K >= 128 and K % 128 == 0 or _refuse(f"{name}: K % 128 == 0 required")
+    1 <= N < 1 << 30 and K >= 128 and K % 128 == 0 or _refuse(f"{name}: N below 2^30 and K % 128 == 0 required")
     K < 131072 or _refuse(f"{name}: K below 131072 required (int32 sums)")
     if dtype is torch.uint8:
         need = E * ((N + 127) // 128) * (K // 128) * TILE_BYTES
@@ -108,6 +108,7 @@ def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, re
     logits.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPE_CODES or _refuse("logits must be a 2-D CUDA tensor of bf16, fp16 or fp32")
     T, E = logits.shape
     1 <= E <= MAX_EXPERTS or _refuse(f"1..{MAX_EXPERTS} experts")
+    T < 1 << 31 or _refuse("fewer than 2^31 tokens required")   # (a C int, which ctypes would cut)
     scoring in (0, 1) and group_score in (0, 1) or _refuse("scoring and group_score must be 0 or 1")
     n_group >= 1 and E % n_group == 0 or _refuse("n_group must divide the number of experts")
     1 <= topk_group <= n_group or _refuse("topk_group must be 1..n_group")
