@@ -65,9 +65,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _same_device(first, **others):
-    for name, t in others.items():
-        t is None or t.device == first.device or _refuse(f"{name} must be on the device of the first argument")
+def _same_device(first, *others):
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            _refuse(f"every tensor must be on the device of the first argument, {first.device} (one is on {t.device})")
 
 
 def _ids(ids: torch.Tensor) -> torch.Tensor:
@@ -101,7 +103,7 @@ def _weights(w: torch.Tensor, s1: torch.Tensor, N: int, K: int, name: str):
 
 def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
     _req(nbytes > 0, "sizes out of range")
-    return torch.empty((nbytes,), dtype=torch.uint8, device=like.device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
 def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, renormalize, scale):
@@ -112,28 +114,31 @@ def _moe_route(logits, bias, topk, scoring, n_group, topk_group, group_score, re
     scoring in (0, 1) and group_score in (0, 1) or _refuse("scoring and group_score must be 0 or 1")
     n_group >= 1 and E % n_group == 0 or _refuse("n_group must divide the number of experts")
     1 <= topk_group <= n_group or _refuse("topk_group must be 1..n_group")
-    1 <= topk <= min(MAX_TOPK, topk_group * (E // n_group)) or \
+    1 <= topk <= MAX_TOPK and topk <= topk_group * (E // n_group) or \
         _refuse(f"topk must be 1..{MAX_TOPK} and at most the experts of topk_group groups")
     if bias is not None:
         _req(bias.is_cuda and bias.dtype == torch.float32 and bias.shape == (E,), "bias must be a CUDA float32 [E] tensor")
-        _same_device(logits, bias=bias)
+        _same_device(logits, bias)
         bias = bias.contiguous()
     logits = logits.contiguous()
-    weights = torch.empty(T, topk, dtype=torch.float32, device=logits.device)
-    ids = torch.empty(T, topk, dtype=torch.int32, device=logits.device)
+    device = logits.device
+    weights = torch.empty(T, topk, dtype=torch.float32, device=device)
+    ids = torch.empty(T, topk, dtype=torch.int32, device=device)
     if T:
         with _dev_ctx(logits):
-            check(lib.lq_moe_route(_ptr(logits), _DTYPE_CODES[logits.dtype], None if bias is None else _ptr(bias), _ptr(weights),
-                                   _ptr(ids), T, E, topk, scoring, n_group, topk_group, group_score, int(renormalize), scale,
-                                   _stream()), "moe_route")
+            check(lib.lq_moe_route(logits.data_ptr(), _DTYPE_CODES[logits.dtype], None if bias is None else bias.data_ptr(),
+                                   weights.data_ptr(), ids.data_ptr(), T, E, topk, scoring, n_group, topk_group, group_score,
+                                   int(renormalize), scale, torch._C._cuda_getCurrentRawStream(device.index)), "moe_route")
     return weights, ids
 
 
 def _experts_linear(x, ascale, ids, w, s1, N, K, out_dtype):
     ids = _ids(ids)
     T, topk = ids.shape
-    x.is_cuda and x.dim() in (2, 3) and x.shape[-1] == K or _refuse(f"x must be a CUDA [T, {K}] or [T, topk, {K}] tensor")
-    _req(tuple(x.shape[:-1]) in ((T,), (T, topk)), "x and ids must have the same tokens (and slots)")
+    shape = x.shape
+    per_pair = len(shape) == 3
+    x.is_cuda and (per_pair or len(shape) == 2) and shape[-1] == K or _refuse(f"x must be a CUDA [T, {K}] or [T, topk, {K}] tensor")
+    shape[0] == T and (not per_pair or shape[1] == topk) or _refuse("x and ids must have the same tokens (and slots)")
     _req(int(out_dtype) in _OUT_DTYPES, "out_dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)")
     if ascale is None:
         _req(x.dtype in _DTYPE_CODES, "x must be bfloat16, float16 or float32 (or int8 with ascale)")
@@ -144,11 +149,10 @@ def _experts_linear(x, ascale, ids, w, s1, N, K, out_dtype):
         ascale = ascale.contiguous()
         code = 3
     kind, w, s1, E = _weights(w, s1, N, K, "w")
-    _same_device(x, ids=ids, w=w, s1=s1, ascale=ascale)
-    y = torch.empty((T, topk, N), dtype=_OUT_DTYPES[int(out_dtype)], device=x.device)
+    _same_device(x, ids, w, s1, ascale)
+    y = torch.empty(T, topk, N, dtype=_OUT_DTYPES[int(out_dtype)], device=x.device)
     if T == 0:
         return y
-    per_pair = x.dim() == 3
     x = _aligned(x)
     with _dev_ctx(x):
         scratch = _scratch(lib.lq_experts_linear_scratch_bytes(T, topk, E, N, K, kind), x)
@@ -171,8 +175,8 @@ def _experts_mlp(x, weights, ids, w13, s13, w2, s2, out_dtype):
     kind, w13, s13, E = _weights(w13, s13, 2 * inner, H, "w13")
     kind2, w2, s2, E2 = _weights(w2, s2, H, inner, "w2")
     _req(kind == kind2 and E == E2, "w13 and w2 must be of the same kind and have the same experts")
-    _same_device(x, ids=ids, weights=weights, w13=w13, s13=s13, w2=w2, s2=s2)
-    y = torch.empty((T, H), dtype=_OUT_DTYPES[int(out_dtype)], device=x.device)
+    _same_device(x, ids, weights, w13, s13, w2, s2)
+    y = torch.empty(T, H, dtype=_OUT_DTYPES[int(out_dtype)], device=x.device)
     if T == 0:
         return y
     x, weights = _aligned(x), weights.contiguous()
@@ -184,10 +188,10 @@ def _experts_mlp(x, weights, ids, w13, s13, w2, s2, out_dtype):
     return y
 
 
-_ORDINARY = (torch.Tensor, torch.nn.Parameter)
+_ORDINARY = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 _is_compiling, _dispatch_modes, _tracing_state, _transform = (torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack,
                                                               torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack)
-_forward_ad = torch.autograd.forward_ad
+_any_requires_grad, _forward_ad = torch._C._any_requires_grad, torch.autograd.forward_ad
 
 
 def _plain_call(*tensors: Optional[torch.Tensor]) -> bool:
@@ -196,9 +200,8 @@ def _plain_call(*tensors: Optional[torch.Tensor]) -> bool:
     a Python kernel costs 4.5 us of the host's 17 for a router call, which is all that a small one takes."""
     if _is_compiling() or _dispatch_modes() or _tracing_state() is not None or _transform() is not None or _forward_ad._current_level >= 0:
         return False
-    for t in tensors:
-        if t is not None and (type(t) not in _ORDINARY or (t.requires_grad and torch.is_grad_enabled())):
-            return False
+    if not _ORDINARY.issuperset(map(type, tensors)) or (_any_requires_grad(*tensors) and torch.is_grad_enabled()):
+        return False
     return tensors[0].is_cuda
 
 
