@@ -1121,15 +1121,26 @@ static int run_weighted_sum(const float* rows, const float* weights, const int* 
 // ---------------------------------------------------------------------------------------------
 // sizes
 // ---------------------------------------------------------------------------------------------
-// Rows of a tile, by what an expert gets on average (the router's choice is uneven: a tile holds twice that and more).  Measured
-// on 8 x 28672 x 4096, 64 x 2048 x 2048 and 16 x 4096 x 4096 with uneven experts, tiles of 32 / 64 / 128 rows and the pair
-// kernel, us.  4-bit: 8 rows on average 82 / 85 / 92 / 101 (28672 x 4096), 24 rows 113 / 102 / 101 / 121, 40 rows 160 / 112 / 111 /
-// 133, 128 rows 410 / 246 / 167 / 180, 192 rows 620 / 381 / 279 / 229.  INT8, whose operands need no unpacking: 8 rows 170 / 155 /
-// 164 / 159, 32 rows 217 / 186 / 169 / 166, 48 rows 257 / 195 / 178 / 153, 192 rows 630 / 433 / 333 / 281.
+// Rows of a tile, by what an expert gets on average (the router's choice is uneven: a tile holds twice that and more; ids that are no
+// expert count too, since the host does not see them).  Measured with unevenly popular experts, tiles of 32 / 64 / 128 rows and the
+// pair kernel, us; L: one product of 8 x 28672 x 4096, M, F: MLPs of 8 experts (4096, 14336) and of 16 (5120, 1536).
+//   4-bit, rows:  8  L 89 / 88 / 100 / 122   M 129 / 131 / 148 / 183   F 54 / 56 / 62 / 67
+//                12  L 84 / 81 / 92 / 108    M 142 / 137 / 159 / 191   F 57 / 61 / 67 / 67
+//                32  L 129 / 111 / 114 / 148 M 214 / 188 / 187 / 220   F 70 / 65 / 69 / 70
+//                48  L 176 / 124 / 118 / 137 M 274 / 194 / 195 / 229   F 86 / 69 / 79 / 76
+//                64  L 216 / 146 / 137 / 154 M 337 / 256 / 215 / 233   F 103 / 74 / 83 / 80
+//               128  L 363 / 211 / 180 / 192 M 584 / 385 / 341 / 292   F 163 / 126 / 122 / 112
+//   INT8, whose operands need no unpacking:
+//                 8  L 121 / 119 / 121 / 122 M 201 / 199 / 208 / 211   F 72 / 73 / 75 / 75
+//                36  L 214 / 174 / 167 / 149 M 321 / 264 / 265 / 265   F 94 / 87 / 95 / 92
+//                44  L 239 / 183 / 174 / 172 M 347 / 309 / 265 / 267   F 93 / 88 / 97 / 95
+//                56  L 286 / 212 / 191 / 178 M 412 / 330 / 292 / 281   F 100 / 92 / 100 / 99
+//               128  L 476 / 333 / 262 / 226 M 698 / 511 / 418 / 329   F 158 / 136 / 127 / 128
+// The limits are where the medians over these, 64 x 2048 x 2048, 16 x 4096 x 4096 and four more layers cross.
 static int pick_bn(long pairs, int E, int w_kind) {
   const long mean = pairs / E;
-  if (mean >= (w_kind == kBlob ? 144 : 45)) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
-  return mean <= 10 ? 32 : mean <= 32 ? 64 : 128;
+  if (mean >= (w_kind == kBlob ? 96 : 56)) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
+  return mean <= 10 ? 32 : mean <= (w_kind == kBlob ? 48 : 40) ? 64 : 128;
 }
 
 // Whether a product's k may be cut, and into how many ranges at most, from the tiles that evenly chosen experts would make: where
