@@ -98,6 +98,7 @@ __device__ __forceinline__ Tile tile_at(const Args& a, int i, int row_tiles) {
 }
 __device__ __forceinline__ int width(int rows) { return (rows + 31) & ~31; }
 
+// MODE: kOutPairs or kOutGated (k is whole).
 template <bool W4, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<W4>::kThreads, 1)
 experts_pair_kernel(const __grid_constant__ Maps maps, const Args args) {
@@ -358,14 +359,11 @@ experts_pair_kernel(const __grid_constant__ Maps maps, const Args args) {
       // the slowest.
       float* sc = row_scale + (2 * g + slot) * kBN;
       int* to = row_pair + (2 * g + slot) * kBN;
-      float w_scale = 0.f;
-      if (MODE != kOutPlanes) {
-        if (n_ok) w_scale = args.s1[(size_t)t.expert * args.N + n];
-        for (int r = et; r < width(t.rows); r += 128) {
-          const bool in = r < t.rows;
-          sc[r] = in ? args.ascale[t.row0 + r] : 0.f;
-          if (MODE == kOutPairs) to[r] = in ? args.pair_of_pos[t.row0 + r] : 0;
-        }
+      const float w_scale = n_ok ? args.s1[(size_t)t.expert * args.N + n] : 0.f;
+      for (int r = et; r < width(t.rows); r += 128) {
+        const bool in = r < t.rows;
+        sc[r] = in ? args.ascale[t.row0 + r] : 0.f;
+        if (MODE == kOutPairs) to[r] = in ? args.pair_of_pos[t.row0 + r] : 0;
       }
       // One thread of the group performs the bounded wait and publishes the outcome, so that its 128 threads always agree
       // on it (they meet at a named barrier and must never split up).
