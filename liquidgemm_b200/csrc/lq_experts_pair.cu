@@ -19,10 +19,13 @@
 //            three, so a set sees every use of its stages; an operand stage is waited for by the set that fills it, and the
 //            MMAs of the set's own last step but one are then known to be done), then two epilogue groups
 //   INT8:    four epilogue groups
-// Bound by the tensor pipe under the part's power limit, and with 4-bit weights by the unpacking warps' issue slots: 8192 tokens x 2
-// experts through 4096 -> 14336 -> 4096, 5.8 TOP, 2.70 ms with all passes, 2.1 POPS (dense INT8 products hold about 3.05 here); INT8
-// weights, 4000 rows of 14336 to 4096, 0.47 TOP, 265 us with the rows' quantisation, 1.8 POPS.  Short k is bound by its outputs: 13332
-// rows of 1792 to 4096 in float32 write 218 MB, tensor pipe 43 %.
+// With 4-bit weights bound by the tensor pipe under the part's power limit and by the unpacking warps' issue slots: 8192 tokens x 2 experts through
+// 4096 -> 14336 -> 4096, 5.8 TOP, 2.60 to 2.75 ms with all passes, 2.1 POPS (dense INT8 products hold about 3.05 here); at 2048 tokens the pipe is
+// 66 and 71 % busy, the issue slots 62 and 50 %.  INT8 weights, 4000 rows of 14336 to 4096, 0.47 TOP, 250 to 270 us with the rows' quantisation,
+// 1.8 POPS: the pipe is 66 % busy, and the dense kernel (lq_i8_pair.cu) takes 158 us for the same product in one matrix, where this one with rows
+// that come in INT8 takes 218 to 225 with one expert, 230 to 255 with eight of 500 rows and 270 with uneven ones.  About 25 us of that are the plan
+// and the rows' copies, the ends of experts inside tiles are the step from one to eight; the rest is not explained.  Short k is bound by its
+// outputs: 13332 rows of 1792 to 4096 in float32 write 218 MB, tensor pipe 43 %.
 // Tensor memory (512 columns): two accumulators, and four 32-column operand stages with 4-bit weights.  No load uses cluster
 // multicast.  Every wait is bounded; status codes 171-177.
 #include <cuda.h>

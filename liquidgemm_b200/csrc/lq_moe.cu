@@ -24,11 +24,12 @@ namespace experts {
 // a choice is a whole number.  The choice is made in float32 first; a token where two numbers whose order matters are closer than
 // their errors together (about one in a thousand) is done again in float64.
 //
-// Bound by instruction issue (a token's row is a few hundred bytes).  A choice is one 32-bit warp reduction, of 16-bit logits with the
+// Bound by instruction issue and its latencies (a token's row is a few hundred bytes; with scores and groups 1390 instructions of a warp, the issue
+// slots 65 % busy, the rest waits of a fixed length and for loads).  A choice is one 32-bit warp reduction, of 16-bit logits with the
 // expert's index below them, or two, of the key and of the index; all lanes do the same throughout (the owner of a choice
 // looking for its next best alone, and handing its score out by shuffles, took as long as all the rest).
 // Groups are ranked from shared memory, 32 / G lanes to a group.  8192 tokens, 192 experts in 8 groups, sigmoid, bias: 64 us with
-// a reduction of the 64-bit key for every group and choice, 22 with all of it in float64, 19 now (without a bias and in one group 8).
+// a reduction of the 64-bit key for every group and choice, 22 with all of it in float64, 16 to 17 now.
 
 // Orders numbers like unsigned integers; every number's image is above 0, which stands for "not to be chosen".
 __device__ __forceinline__ uint32_t ordered(float v) {
