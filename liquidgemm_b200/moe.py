@@ -222,8 +222,8 @@ def route(logits: torch.Tensor, topk: int, scoring: str = "softmax", bias: Optio
     lowest index among equals.  With ``n_group`` > 1 only experts of the ``topk_group`` best groups of E / n_group neighbours
     can be chosen; a group ranks by its largest key (``group_score="max"``) or the sum of its two largest (``"top2"``).
     Weights are the scores without the bias, divided by their sum with ``renormalize``, times ``scale``: those of 64-bit scores, however
-    small, and 0 where none of the chosen has one.  A logit of -inf or NaN takes
-    its expert out; slots for which no expert is left have id -1 and weight 0 (the products skip them)."""
+    small, and 0 where none of the chosen has one.  A logit of -inf or NaN takes its expert out; slots for which no expert is left have
+    id -1 and weight 0 (the products skip them)."""
     scoring in _SCORING or _refuse("scoring must be 'softmax' or 'sigmoid'")
     group_score in _GROUP_SCORE or _refuse("group_score must be 'max' or 'top2'")
     run = _moe_route if _plain_call(logits, bias) else torch.ops.liquidgemm.moe_route
