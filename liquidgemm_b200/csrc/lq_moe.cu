@@ -1134,14 +1134,15 @@ static int run_weighted_sum(const float* rows, const float* weights, const int* 
 //   INT8, whose operands need no unpacking:
 //                 8  L 121 / 119 / 121 / 122 M 201 / 199 / 208 / 211   F 72 / 73 / 75 / 75
 //                36  L 214 / 174 / 167 / 149 M 321 / 264 / 265 / 265   F 94 / 87 / 95 / 92
-//                44  L 239 / 183 / 174 / 172 M 347 / 309 / 265 / 267   F 93 / 88 / 97 / 95
+//                48  L 253 / 209 / 180 / 176 M 377 / 319 / 278 / 277   F 94 / 90 / 97 / 95
 //                56  L 286 / 212 / 191 / 178 M 412 / 330 / 292 / 281   F 100 / 92 / 100 / 99
 //               128  L 476 / 333 / 262 / 226 M 698 / 511 / 418 / 329   F 158 / 136 / 127 / 128
 // The limits are where the forms cross on average over these, products of 64 x 2048 x 2048, 16 x 4096 x 4096, 32 x 4096 x 1792 and 64 x 1024 x
-// 4096 and MLPs of 32 experts (4096, 1792), 64 (2048, 1024) and 128 (2048, 768); single layers are up to 10 % faster on the other side.
+// 4096 and MLPs of 32 experts (4096, 1792), 64 (2048, 1024) and 128 (2048, 768); single layers are up to 10 % faster on the
+// other side (4-bit from 96 to 127 rows the pair kernel is ahead on average, but up to 13 % behind where weights are small or experts few).
 static int pick_bn(long pairs, int E, int w_kind) {
   const long mean = pairs / E;
-  if (mean >= (w_kind == kBlob ? 96 : 56)) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
+  if (mean >= (w_kind == kBlob ? 128 : 45)) return w_kind == kBlob ? kPairRowsBlob : kPairRowsInt8;
   return mean <= 10 ? 32 : mean <= (w_kind == kBlob ? 48 : 40) ? 64 : 128;
 }
 

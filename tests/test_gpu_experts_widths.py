@@ -16,7 +16,7 @@ def moe():
 
 
 @pytest.mark.parametrize("w4", [True, False], ids=["w4", "int8"])
-@pytest.mark.parametrize("mean", [10, 11, 40, 41, 48, 49, 55, 56, 95, 96, 144])
+@pytest.mark.parametrize("mean", [10, 11, 40, 41, 44, 45, 48, 49, 96, 127, 128])
 def test_both_sides_of_each_limit(moe, w4, mean):
     E, N, K = 5, 328, 384
     layer, q, s1 = _stack(moe, E, N, K, w4, mean)
