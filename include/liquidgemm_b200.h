@@ -352,6 +352,40 @@ LQ_API int lq_experts_mlp(const void* x, int x_dtype, const float* weights, cons
                           const float* s13, const void* w2, const float* s2, int w_kind, void* y, int out_dtype, int T,
                           int topk, int E, int H, int I, void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---- what stands around the linears of a layer (no counterpart in the reference) ----
+ *
+ * Low-rank adapters of many requests at once, added to a projection's output: for row t with slot l = ids[t]
+ *   out[t, n] = (type of y)(y[t, n] + scales[l] * sum_j b[l, n, j] * (sum_k a[l, s, j, k] * x[t, k])),  j < ranks[l, s],
+ * s the slice that column n belongs to; both sums in float32.  A row whose id is outside [0, L) is y's, and so is a slice with
+ * ranks[l, s] == 0.  ranks [L, n_slices].
+ * x [T, K] with rows `ldx` elements apart, a [L, n_slices, rank, K] and b [L, N, rank] in `dtype` (LQ_DT_BF16 or LQ_DT_F16); ranks beyond
+ * a slice's own (ranks[l, s] <= rank) are zero in b.  y and out [T, N], rows `ldy` and `ldo` elements apart, in `dtype` or, with
+ * y_f32, float32; out == y changes y in place, otherwise they must not overlap.  ids int32, or int64 with ids_64.  widths: a HOST
+ * array with the number of columns of each slice, N their sum.
+ * L <= 4096, rank <= 256, n_slices <= 8, T <= 2^24, K <= 2^20; rank, K, ldx and widths multiples of 8, x, a, b, y, out, rows of
+ * y and out, and scratch 16-byte aligned.  `scratch`: lq_adapters_scratch_bytes() bytes, any content (0 from that function: sizes out of
+ * range). */
+LQ_API size_t lq_adapters_scratch_bytes(int T, int K, int L, int rank, int n_slices);
+LQ_API int lq_adapters_add(const void* x, int dtype, long ldx, const void* a, const void* b, const int32_t* ranks,
+                           const float* scales, const void* ids, int ids_64, const void* y, long ldy, int y_f32, void* out,
+                           long ldo, int T, int K, int L, int rank, const int* widths, int n_slices, void* scratch,
+                           size_t scratch_bytes, void* stream);
+
+/* Norms around a block, in one pass over `rows` rows of H elements:
+ *   p = post ? x * (mean(x^2) + eps)^-1/2 * (post + offset) : x
+ *   h = (stream_dtype)(residual_scale * residual + scale * gate * p)
+ *   z = h * (mean(h^2) + eps)^-1/2 * (weight + offset)
+ * in float32, z rounded to x_dtype; or, with q and q_scale instead of z, INT8 rows and scales: with t = h * (weight + offset) in
+ * float32, q = round(127 t / max|t|) exactly (ties to even) and q_scale = max|t| * (mean(h^2) + eps)^-1/2 / 127.
+ * residual, gate, weight and post may be null (left out: no such term or factor), and so may h (not stored).  stream_dtype: that of residual and h,
+ * x_dtype or, with a residual, LQ_DT_F32.  gate, weight, post: x_dtype or LQ_DT_F32.  Row m of x, residual and gate lies
+ * (m / inner) * outer + (m % inner) * inner_stride elements behind the pointer (x_outer, x_inner, ...); gate_step 1: H gates a row, 0:
+ * one.  z, q and h are contiguous.  H <= 32768; eps >= 0.  Any alignment; 16-byte aligned rows of a multiple of 8 elements are faster. */
+LQ_API int lq_block_norm(const void* x, int x_dtype, long x_outer, long x_inner, const void* residual, int stream_dtype,
+                         long r_outer, long r_inner, const void* gate, int gate_dtype, long g_outer, long g_inner,
+                         int gate_step, const void* weight, int weight_dtype, const void* post, int post_dtype, void* z,
+                         int8_t* q, float* q_scale, void* h, int rows, int inner, int H, float eps, float scale,
+                         float residual_scale, float offset, void* stream);
 
 #ifdef __cplusplus
 }

@@ -73,6 +73,12 @@ _SIGNATURES = {
     "lq_experts_mlp_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "lq_experts_mlp": (c_int, [P, c_int, P, P, P, P, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, P,
                                c_size_t, P]),
+    "lq_adapters_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "lq_adapters_add": (c_int, [P, c_int, ctypes.c_long, P, P, P, P, P, c_int, P, ctypes.c_long, c_int, P, ctypes.c_long, c_int,
+                                c_int, c_int, c_int, P, c_int, P, c_size_t, P]),
+    "lq_block_norm": (c_int, [P, c_int, ctypes.c_long, ctypes.c_long, P, c_int, ctypes.c_long, ctypes.c_long, P, c_int,
+                              ctypes.c_long, ctypes.c_long, c_int, P, c_int, P, c_int, P, P, P, P, c_int, c_int, c_int,
+                              ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float, P]),
 }
 
 for _name, (_res, _args) in _SIGNATURES.items():

@@ -1,0 +1,225 @@
+"""Low-rank adapters of many requests at once beside a linear.
+
+A stack holds the adapters that a server keeps on the GPU, one per slot; every row of a batch names the slot of its request, or none:
+
+    ``y[t, n] + scale[l] * sum_j B[l, n, j] (sum_k A[l, s, j, k] x[t, k])``,  l = ids[t], s = the slice that column n belongs to.
+
+* :func:`make_stack`, :func:`load`, :func:`unload`   the stack and its slots;
+* :func:`add`      the adapters' part of a projection, added to its output ``y``;
+* :func:`linear`   a W4A8 or INT8 linear with the adapters beside it.
+
+A fused projection (q, k and v; gate and up) has one slice per part, each with matrices of its own.  The operators behind these are
+``torch.ops.liquidgemm.adapters_add`` and ``adapters_add_`` (in place), with fake kernels.  Like the dense operators they validate
+their arguments in Python, allocate outputs and scratch with torch, enqueue on the current stream of the tensors' device, synchronise
+nothing and can be captured into a CUDA graph; which slots a batch reaches is known on the device only, and nothing depends on it on the
+host, so a captured step may be replayed with other ids and after slots were loaded anew.  Inference only.
+
+The reference has no counterpart: its plugin quantises plain linears only (liquidgemm/vllm_plugin.py:101-108).
+Like :mod:`liquidgemm_b200.ops` this module is not imported by the package ``__init__``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import Optional, Sequence, Union
+
+import torch
+
+from ._lib import check, lib
+from .moe import _aligned, _plain_call, _refuse, _same_device
+from .ops import _DTYPE_CODES, _dev_ctx, _impl, _libdef, _req, _stream
+
+MAX_SLOTS = 4096
+MAX_RANK = 256
+MAX_SLICES = 8
+MAX_ROWS = 1 << 24
+MAX_K = 1 << 20
+
+_ARGS = "Tensor x, Tensor a, Tensor b, Tensor rank, Tensor scale, Tensor ids, int[] widths"
+_libdef.define(f"adapters_add(Tensor y, {_ARGS}) -> Tensor")
+_libdef.define(f"adapters_add_(Tensor(a!) y, {_ARGS}) -> ()")
+
+
+@torch.library.register_fake("liquidgemm::adapters_add")
+def _f_add(y, x, a, b, rank, scale, ids, widths):
+    return y.new_empty(y.shape)
+
+
+@torch.library.register_fake("liquidgemm::adapters_add_")
+def _f_add_(y, x, a, b, rank, scale, ids, widths):
+    return None
+
+
+@lru_cache(maxsize=256)
+def _c_widths(widths):
+    return (ctypes.c_int * len(widths))(*widths)
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from a row of ``t`` [T, n] to the next (of a single row: its own)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [T, n] with neighbours next to each other, rows and first element on 16-byte boundaries."""
+    pitch = _pitch(t)
+    if t.stride(1) == 1 and pitch >= t.shape[1] and pitch * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return _aligned(t)
+
+
+def _run(y, x, a, b, rank, scale, ids, widths, inplace):
+    dtype = x.dtype
+    dtype in (torch.bfloat16, torch.float16) and x.is_cuda and x.dim() == 2 or _refuse("x must be a 2-D CUDA tensor of bf16 or fp16")
+    a.dim() == 4 and b.dim() == 3 and a.dtype is dtype and b.dtype is dtype or \
+        _refuse("the stack's matrices must be [L, S, rank, K] and [L, N, rank] in the type of x")
+    L, S, r, K = a.shape
+    N = b.shape[1]
+    T = x.shape[0]
+    x.shape[1] == K or _refuse(f"x must be [T, {K}]")
+    1 <= L <= MAX_SLOTS and 1 <= S <= MAX_SLICES and 8 <= r <= MAX_RANK and r % 8 == 0 and 8 <= K <= MAX_K and K % 8 == 0 or \
+        _refuse(f"1..{MAX_SLOTS} slots, 1..{MAX_SLICES} slices, a rank of 8..{MAX_RANK} and K up to {MAX_K}, both multiples of 8, required")
+    b.shape[0] == L and b.shape[2] == r and a.is_contiguous() and b.is_contiguous() or _refuse("the stack's matrices do not fit each other")
+    widths = tuple(widths)
+    len(widths) == S and sum(widths) == N and all(w > 0 and w % 8 == 0 for w in widths) or \
+        _refuse(f"widths must be {S} multiples of 8 whose sum is {N}")
+    y.is_cuda and y.dim() == 2 and y.shape[0] == T and y.shape[1] == N and (y.dtype is dtype or y.dtype is torch.float32) or \
+        _refuse(f"y must be CUDA [{T}, {N}] in the type of x or float32")
+    rank.dtype is torch.int32 and scale.dtype is torch.float32 and rank.shape == (L, S) and scale.shape == (L,) or \
+        _refuse(f"rank must be int32 [{L}, {S}] and scale float32 [{L}]")
+    ids.is_cuda and ids.shape == (T,) and ids.dtype in (torch.int32, torch.int64) or _refuse(f"ids must be a CUDA [{T}] tensor of int32 or int64")
+    T <= MAX_ROWS or _refuse(f"at most {MAX_ROWS} rows")
+    _same_device(x, y, a, b, rank, scale, ids)
+    a.data_ptr() % 16 == 0 and b.data_ptr() % 16 == 0 or _refuse("the stack's matrices must start on 16-byte boundaries")
+    if inplace:
+        out = y
+        T == 0 or _rows(y) is y or _refuse("y is changed in place: neighbours next to each other, rows on 16-byte boundaries required")
+    else:
+        out = torch.empty((T, N), dtype=y.dtype, device=y.device)
+    if T == 0:
+        return out
+    x, ids = _rows(x), ids.contiguous()
+    y = out if inplace else _rows(y)
+    with _dev_ctx(x):
+        nbytes = lib.lq_adapters_scratch_bytes(T, K, L, r, S)
+        _req(nbytes > 0, "sizes out of range")
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        check(lib.lq_adapters_add(x.data_ptr(), _DTYPE_CODES[dtype], _pitch(x), a.data_ptr(), b.data_ptr(), rank.data_ptr(),
+                                  scale.data_ptr(), ids.data_ptr(), int(ids.dtype is torch.int64), y.data_ptr(), _pitch(y),
+                                  int(y.dtype is torch.float32), out.data_ptr(), _pitch(out), T, K, L, r, _c_widths(widths), S,
+                                  scratch.data_ptr(), nbytes, _stream()), "adapters_add")
+    return out
+
+
+def _add(y, x, a, b, rank, scale, ids, widths):
+    return _run(y, x, a, b, rank, scale, ids, widths, False)
+
+
+def _add_(y, x, a, b, rank, scale, ids, widths):
+    _run(y, x, a, b, rank, scale, ids, widths, True)
+
+
+_impl.impl("adapters_add", _add)
+_impl.impl("adapters_add_", _add_)
+
+
+# --------------------------------------------------------------------------------------
+# Python entry points
+# --------------------------------------------------------------------------------------
+
+def make_stack(slots: int, rank: int, K: int, widths: Union[int, Sequence[int]], dtype: torch.dtype = torch.bfloat16,
+               device="cuda") -> dict:
+    """An empty stack for adapters of a linear with inputs of ``K`` and slices of ``widths`` output channels (one number: one
+    slice): ``slots`` of them, of ranks up to ``rank`` (rounded up to a multiple of 8), in ``dtype`` (bf16 or fp16, the activations' type).
+
+    ``{"a" [slots, S, R, K], "b" [slots, N, R], "rank" [slots, S] int32, "scale" [slots] float32, "widths", "K", "N"}`` with R the rank
+    rounded up to a multiple of 8.  The tensors keep their addresses; an empty slot has ranks 0."""
+    widths = (int(widths),) if isinstance(widths, int) else tuple(int(w) for w in widths)
+    _req(1 <= slots <= MAX_SLOTS, f"1..{MAX_SLOTS} slots")
+    _req(1 <= rank <= MAX_RANK, f"rank must be 1..{MAX_RANK}")
+    _req(8 <= K <= MAX_K and K % 8 == 0, f"K must be a multiple of 8 up to {MAX_K}")
+    _req(1 <= len(widths) <= MAX_SLICES and all(w > 0 and w % 8 == 0 for w in widths) and sum(widths) < 1 << 24,
+         f"1..{MAX_SLICES} slices of widths that are multiples of 8 (fewer than 2^24 channels) required")
+    _req(dtype in (torch.bfloat16, torch.float16), "dtype must be bfloat16 or float16")
+    r = (rank + 7) // 8 * 8
+    N = sum(widths)
+    return {"a": torch.zeros((slots, len(widths), r, K), dtype=dtype, device=device),
+            "b": torch.zeros((slots, N, r), dtype=dtype, device=device),
+            "rank": torch.zeros((slots, len(widths)), dtype=torch.int32, device=device),
+            "scale": torch.zeros(slots, dtype=torch.float32, device=device), "widths": widths, "K": int(K), "N": N}
+
+
+def load(stack: dict, slot: int, a, b, scale: float = 1.0) -> None:
+    """Put an adapter into ``slot``: ``a`` [r, K] and ``b`` [N, r] (a list of such pairs' halves, one for each slice, for a fused
+    projection; ranks may differ, ``None`` for a slice without one), its part multiplied by ``scale`` (``alpha / r``).  Enqueued on the
+    current stream: work on other streams that reads the slot has to be ordered by the caller."""
+    widths = stack["widths"]
+    a, b = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (a, b))
+    _req(0 <= slot < stack["rank"].shape[0], f"slot must be 0..{stack['rank'].shape[0] - 1}")
+    _req(len(a) == len(widths) and len(b) == len(widths), f"{len(widths)} pairs of matrices required, one for each slice")
+    most, K = stack["a"].shape[2], stack["K"]
+    ranks = []
+    for s, w in enumerate(widths):
+        _req((a[s] is None) == (b[s] is None), "a slice has both matrices or none")
+        if a[s] is None:
+            ranks.append(0)
+            continue
+        _req(a[s].dim() == 2 and a[s].shape[1] == K and 1 <= a[s].shape[0] <= most, f"a must be [1..{most}, {K}]")
+        _req(tuple(b[s].shape) == (w, a[s].shape[0]), f"b must be [{w}, {a[s].shape[0]}]")
+        ranks.append(a[s].shape[0])
+    with torch.no_grad():
+        stack["a"][slot].zero_()
+        stack["b"][slot].zero_()
+        at = 0
+        for s, w in enumerate(widths):
+            if ranks[s]:
+                stack["a"][slot, s, :ranks[s]].copy_(a[s])
+                stack["b"][slot, at:at + w, :ranks[s]].copy_(b[s])
+            at += w
+        stack["scale"][slot] = float(scale)
+        for s, n in enumerate(ranks):
+            stack["rank"][slot, s] = n
+
+
+def unload(stack: dict, slot: int) -> None:
+    """Empty ``slot``: rows that name it are left as they are."""
+    _req(0 <= slot < stack["rank"].shape[0], f"slot must be 0..{stack['rank'].shape[0] - 1}")
+    stack["rank"][slot].zero_()
+
+
+def add(y: torch.Tensor, x: torch.Tensor, stack: dict, ids: torch.Tensor, inplace: bool = False) -> torch.Tensor:
+    """``y`` [T, N] plus what the adapters of its rows make of ``x`` [T, K] (bf16 or fp16), in the type of ``y`` (that of ``x``, or
+    float32): a new tensor, or ``y`` itself, changed, with ``inplace``.
+
+    ``ids`` [T] (int32 or int64) names the slot of every row; an id outside the slots, or an empty slot, leaves its row as it is.
+    Both products are summed in float32 and the result is rounded once."""
+    args = (y, x, stack["a"], stack["b"], stack["rank"], stack["scale"], ids)
+    if inplace:
+        (_add_ if _plain_call(*args) else torch.ops.liquidgemm.adapters_add_)(*args, stack["widths"])
+        return y
+    return (_add if _plain_call(*args) else torch.ops.liquidgemm.adapters_add)(*args, stack["widths"])
+
+
+def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A linear with the adapters of its rows beside it: [T, N] in ``out_dtype`` (default: that of ``x``).
+
+    ``layer`` holds a layer's device tensors: 4-bit weights as :func:`liquidgemm_b200.ops.w4a8_linear` takes them (``rs, s_u8, offset_a,
+    s1, N, K``), or ``w_i8`` [N, K] with ``s1`` in place of the first three.  The linear quantises ``x``, the adapters read it
+    as it is; their part joins the linear's rounded output (like a bias does), so the result is that of the linear and :func:`add`,
+    bit for bit."""
+    out_dtype = out_dtype or x.dtype
+    _req(x.dtype in (torch.bfloat16, torch.float16) and out_dtype in (x.dtype, torch.float32),
+         "x must be bf16 or fp16, out_dtype its type or float32")
+    _req(layer["N"] == stack["N"] and layer["K"] == stack["K"], "the stack is for another linear (N and K)")
+    code = _DTYPE_CODES[out_dtype]
+    if layer.get("rs") is not None:
+        y = torch.ops.liquidgemm.w4a8_linear(x, layer["rs"], layer["s_u8"], layer["offset_a"], layer["s1"], bias, layer["N"],
+                                             layer["K"], 64, code)
+    else:
+        rows, scales = torch.ops.liquidgemm.quant_per_token(x)
+        y = torch.ops.liquidgemm.i8_gemm_scaled(rows, layer["w_i8"], scales, layer["s1"], code)
+        if bias is not None:
+            y = y + bias
+    return add(y, x, stack, ids, inplace=True)
