@@ -377,15 +377,15 @@ LQ_API int lq_adapters_add(const void* x, int dtype, long ldx, const void* a, co
  *   z = h * (mean(h^2) + eps)^-1/2 * (weight + offset)
  * in float32, z rounded to x_dtype; or, with q and q_scale instead of z, INT8 rows and scales: with t = h * (weight + offset) in
  * float32, q = round(127 t / max|t|) exactly (ties to even) and q_scale = max|t| * (mean(h^2) + eps)^-1/2 / 127.
- * residual, gate, weight and post may be null (left out: no such term or factor), and so may h (not stored).  stream_dtype: that of residual and h,
+ * residual, gate, weight and post may be null (left out: no such term or factor), and, where nothing but x makes h, so may h.  stream_dtype: that of residual and h,
  * x_dtype or, with a residual, LQ_DT_F32.  gate, weight, post: x_dtype or LQ_DT_F32.  Row m of x, residual and gate lies
  * (m / inner) * outer + (m % inner) * inner_stride elements behind the pointer (x_outer, x_inner, ...); gate_step 1: H gates a row, 0:
  * one.  z, q and h are contiguous.  H <= 32768; eps >= 0.  Any alignment; 16-byte aligned rows of a multiple of 8 elements are faster. */
 LQ_API int lq_block_norm(const void* x, int x_dtype, long x_outer, long x_inner, const void* residual, int stream_dtype,
                          long r_outer, long r_inner, const void* gate, int gate_dtype, long g_outer, long g_inner,
                          int gate_step, const void* weight, int weight_dtype, const void* post, int post_dtype, void* z,
-                         int8_t* q, float* q_scale, void* h, int rows, int inner, int H, float eps, float scale,
-                         float residual_scale, float offset, void* stream);
+                         int8_t* q, float* q_scale, void* h, int rows, int inner, int H, double eps, double scale,
+                         double residual_scale, double offset, void* stream);
 
 #ifdef __cplusplus
 }

@@ -78,7 +78,7 @@ _SIGNATURES = {
                                 c_int, c_int, c_int, P, c_int, P, c_size_t, P]),
     "lq_block_norm": (c_int, [P, c_int, ctypes.c_long, ctypes.c_long, P, c_int, ctypes.c_long, ctypes.c_long, P, c_int,
                               ctypes.c_long, ctypes.c_long, c_int, P, c_int, P, c_int, P, P, P, P, c_int, c_int, c_int,
-                              ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float, P]),
+                              ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, P]),
 }
 
 for _name, (_res, _args) in _SIGNATURES.items():

@@ -95,6 +95,23 @@ def test_forms(H, stream, post, gate):
         _both(x, None, residual=residual, gate=None if shape is None else _randn(gen, *shape))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,H", [(9000, 40), (6000, 512), (5000, 1000), (3001, 4096), (1500, 8192), (700, 10240), (400, 16384), (3001, 1001)])
+def test_more_rows_than_the_gpu_holds(T, H, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    dtype = DTYPES[dtype]
+    x, weight = _randn(gen, T, H).to(dtype), (1 + 0.3 * _randn(gen, H)).to(dtype)
+    x[::7] *= 30.0
+    _both(x, weight)
+    _both(x, weight, residual=_randn(gen, T, H).to(dtype), gate=_randn(gen, T, 1).to(dtype))
+    _both(x, weight, residual=_randn(gen, T, H), post_weight=_randn(gen, H), gate=_randn(gen, T, H).to(dtype), scale=0.3, weight_offset=1.0)
+    if dtype != torch.float16:
+        x[T - 2] *= 1e30
+        _both(x, weight, gate=_randn(gen, H))
+    wide = torch.empty(T // 4, 4, H + 8, dtype=dtype, device="cuda").normal_(generator=gen)
+    _both(wide[:, 1:3, 8:], weight, residual=wide[:, :2, :H], gate=_randn(gen, T // 4, 1, H))
+
+
 def test_plain_norm_returns_its_rows():
     from liquidgemm_b200 import norms
     x = torch.randn(4, 64, device="cuda").to(torch.bfloat16)
