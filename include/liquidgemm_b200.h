@@ -362,7 +362,7 @@ LQ_API int lq_experts_mlp(const void* x, int x_dtype, const float* weights, cons
  * a slice's own (ranks[l, s] <= rank) are zero in b.  y and out [T, N], rows `ldy` and `ldo` elements apart, in `dtype` or, with
  * y_f32, float32; out == y changes y in place, otherwise they must not overlap.  ids int32, or int64 with ids_64.  widths: a HOST
  * array with the number of columns of each slice, N their sum.
- * L <= 4096, rank <= 256, n_slices <= 8, T <= 2^24, K <= 2^20; rank, K, ldx and widths multiples of 8, x, a, b, y, out, rows of
+ * L <= 4096, rank <= 256, n_slices <= 8, T <= 2^24, K <= 2^20, N <= 2^22; rank, K, ldx and widths multiples of 8, x, a, b, y, out, rows of
  * y and out, and scratch 16-byte aligned.  `scratch`: lq_adapters_scratch_bytes() bytes, any content (0 from that function: sizes out of
  * range). */
 LQ_API size_t lq_adapters_scratch_bytes(int T, int K, int L, int rank, int n_slices);

@@ -35,6 +35,7 @@ MAX_RANK = 256
 MAX_SLICES = 8
 MAX_ROWS = 1 << 24
 MAX_K = 1 << 20
+MAX_CHANNELS = 1 << 22
 
 _ARGS = "Tensor x, Tensor a, Tensor b, Tensor rank, Tensor scale, Tensor ids, int[] widths"
 _libdef.define(f"adapters_add(Tensor y, {_ARGS}) -> Tensor")
@@ -82,7 +83,7 @@ def _run(y, x, a, b, rank, scale, ids, widths, inplace):
         _refuse(f"1..{MAX_SLOTS} slots, 1..{MAX_SLICES} slices, a rank of 8..{MAX_RANK} and K up to {MAX_K}, both multiples of 8, required")
     b.shape[0] == L and b.shape[2] == r and a.is_contiguous() and b.is_contiguous() or _refuse("the stack's matrices do not fit each other")
     widths = tuple(widths)
-    len(widths) == S and sum(widths) == N and all(w > 0 and w % 8 == 0 for w in widths) or \
+    len(widths) == S and sum(widths) == N <= MAX_CHANNELS and all(w > 0 and w % 8 == 0 for w in widths) or \
         _refuse(f"widths must be {S} multiples of 8 whose sum is {N}")
     y.is_cuda and y.dim() == 2 and y.shape[0] == T and y.shape[1] == N and (y.dtype is dtype or y.dtype is torch.float32) or \
         _refuse(f"y must be CUDA [{T}, {N}] in the type of x or float32")
@@ -139,8 +140,8 @@ def make_stack(slots: int, rank: int, K: int, widths: Union[int, Sequence[int]],
     _req(1 <= slots <= MAX_SLOTS, f"1..{MAX_SLOTS} slots")
     _req(1 <= rank <= MAX_RANK, f"rank must be 1..{MAX_RANK}")
     _req(8 <= K <= MAX_K and K % 8 == 0, f"K must be a multiple of 8 up to {MAX_K}")
-    _req(1 <= len(widths) <= MAX_SLICES and all(w > 0 and w % 8 == 0 for w in widths) and sum(widths) < 1 << 24,
-         f"1..{MAX_SLICES} slices of widths that are multiples of 8 (fewer than 2^24 channels) required")
+    _req(1 <= len(widths) <= MAX_SLICES and all(w > 0 and w % 8 == 0 for w in widths) and sum(widths) <= MAX_CHANNELS,
+         f"1..{MAX_SLICES} slices of widths that are multiples of 8 (up to {MAX_CHANNELS} channels) required")
     _req(dtype in (torch.bfloat16, torch.float16), "dtype must be bfloat16 or float16")
     r = (rank + 7) // 8 * 8
     N = sum(widths)

@@ -1,9 +1,13 @@
 // Low-rank adapters of many requests at once, added to a projection's output:
 //   v[t, s, j] = sum_k A[l, s, j, k] x[t, k]                                 l = ids[t], float32
 //   out[t, n]  = (type of y)(y[t, n] + scale[l] * sum_j B[l, n, j] v[t, slice of n, j])
-// Three kernels: rows are put in the order of their adapters and cut into tiles of up to 64 rows of one adapter; a tile's rows
-// times A (K cut over warps and CTAs); the result times B, added to y.  The rows that a slot gets are known on the device only.
+// A few rows: one kernel, a cluster of CTAs for up to eight rows of one adapter.  More: rows are put in the order of their adapters and
+// cut into tiles of up to 64 rows of one adapter; a tile's rows times A (K cut over warps and CTAs); the result times B, added to y.
+// The rows that a slot gets are known on the device only.
+#include <type_traits>
+
 #include "lq_common.cuh"
+#include "lq_tc_ptx.cuh"
 
 namespace lq {
 namespace {
@@ -20,9 +24,9 @@ struct Tile {
 };
 
 struct Slices {
-  int n;
+  int n, N, parts;             // all columns, all parts
   int start[kMaxSlices + 1];   // first column of a slice
-  int block[kMaxSlices + 1];   // first column block of a slice (blocks end with their slice)
+  int part[kMaxSlices + 1];    // first part (the columns of a CTA, or of a warp) of a slice; parts end with their slice
 };
 
 template <typename T> struct Mma;
@@ -41,17 +45,22 @@ template <> struct Mma<__half> {
   }
 };
 
+// Two numbers rounded to a 16-bit type.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float2 v);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float2 v) {
+  const __half2 h = __float22half2_rn(v);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float2 v) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 
-// Coherent loads that may stay in L1 (other warps or tiles read the same weights).
-__device__ __forceinline__ uint4 ld_v4(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
-  return r;
-}
+// A coherent load that may stay in L1.
 __device__ __forceinline__ uint2 ld_v2(const void* p) {
   uint2 r;
   asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p) : "memory");
@@ -72,10 +81,10 @@ __device__ __forceinline__ int slot_of(const void* ids, bool wide, long t, int L
 // are its own wherever it lies in a tile.
 __global__ void __launch_bounds__(1024)
 adapter_plan_kernel(const void* ids, bool wide, const int* rank, int T, int L, int S, bool copy_rest, int* order, Tile* tiles,
-                    int max_tiles) {
-  extern __shared__ int smem[];
-  int* first = smem;                  // [L + 2] rows before a slot's
-  int* tile0 = smem + L + 2;          // [L + 2] tiles before a slot's
+                    int* done, int max_tiles) {
+  extern __shared__ int counts[];
+  int* first = counts;                // [L + 2] rows before a slot's
+  int* tile0 = counts + L + 2;          // [L + 2] tiles before a slot's
   int* next = tile0 + L + 2;          // [L + 1] counts, then the next free place
   __shared__ int warp_sum[2][32];
   allow_dependents();
@@ -127,6 +136,7 @@ adapter_plan_kernel(const void* ids, bool wide, const int* rank, int T, int L, i
       tile = {a == L ? -1 : a, at, min(kTile, first[a + 1] - at), 0};
     }
     tiles[i] = tile;
+    done[i] = 0;
   }
   for (int t0 = warp * 32; t0 < T; t0 += blockDim.x) {
     const int t = t0 + lane;
@@ -141,18 +151,74 @@ adapter_plan_kernel(const void* ids, bool wide, const int* rank, int T, int L, i
 }
 
 // ---------------------------------------------------------------------------------------------
-// v = A x for a tile's rows: ranks are the 16 rows of an MMA, eight tokens its columns, so that both operands come straight
-// from their row-major matrices into registers.  The order of k within a product is free: thread t of a quad takes the
-// eight neighbours 8 t .. 8 t + 7 of 32 k for both operands, one 16-byte load each.  A CTA's warps take turns at the 32-k
-// chunks of its range of K; their sums meet in shared memory and go to plane blockIdx.z of v [planes][T][R] (R = slices x stack
-// rank), in the order of the plan.
+// v = A x.  Ranks are the 16 rows of an MMA, eight tokens its columns, so that both operands come straight from their row-major
+// matrices into registers.  The order of k within a product is free: thread t of a quad takes the eight neighbours
+// 8 t .. 8 t + 7 of 32 k for both operands, one 16-byte load each.
+
+// A float32 sum goes into the second product as two 16-bit numbers whose sum carries 16 bits of it or more (22 in fp16), multiplied by
+// a power of two that keeps a row's sums of one slice in fp16's range.
+struct Power {
+  float down, up;
+};
+__device__ __forceinline__ Power power_of(float top) {   // of the largest magnitude: it goes to 2^13 .. 2^14
+  const int e = top > 0.f && top < 3.4e38f ? max(-100, min(100, 140 - (int)((__float_as_uint(top) >> 23) & 0xffu))) : 0;
+  return {__uint_as_float((uint32_t)(127 + e) << 23), __uint_as_float((uint32_t)(127 - e) << 23)};
+}
+template <typename T>
+__device__ __forceinline__ void halves(float v, T& hi, T& lo) {
+  hi = narrow<T>(v);
+  lo = narrow<T>(fabsf(v) < 3.4e38f ? v - to_f32<T>(hi) : 0.f);
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool on) {   // zeros where it is not on
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_but() {   // all copies but those of the last N groups are there
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void commit_stores() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void stores_read_but() {   // all bulk stores but those of the last N groups have read shared memory
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+constexpr uint64_t kWaitLimit = 2000000000ull;
+__device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, int* status, int site) {
+  const bool ok = ptx::mbar_wait_bounded(bar, parity, kWaitLimit);
+  if (!ok) atomicExch(status, site);
+  return ok;
+}
+__device__ __forceinline__ uint4 lds_v4(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+
+// A tile's rows, 16 RT ranks and one range of K.  Sixteen warps take turns at the 32-k chunks of the range, each thread's pieces on their
+// way into places of its own in shared memory a chunk ahead (nobody else reads them: no barrier).  The warps' sums meet in shared memory
+// and go to plane blockIdx.z of v [planes][T][R] (R = slices x stack rank), in the order of the plan; the last CTA of a tile adds up the
+// planes, in their order, and writes the sums' halves, vv [slices][T][stack rank / 4][2][4], and the power of two of each.
+// Bound by the stream of x: 8192 rows of 14336 at rank 16 235 MB.
+constexpr int kShrinkThreads = 512;
+template <int RT>
+struct Shrink {
+  static constexpr int kPieces = 8 + 2 * RT, kStage = kPieces * kShrinkThreads * 16, kStages = 2;
+  static constexpr int kSums = kShrinkThreads / 32 * RT * 16 * 66 * (int)sizeof(float);
+  static constexpr int kBytes = kStage * kStages > kSums ? kStage * kStages : kSums;
+};
+
 template <typename T, int RT>
-__global__ void __launch_bounds__(256, 1)
-adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const int* order, const Tile* tiles, float* v, int rows,
-                      int K, int R, int rp, int k_range) {
-  extern __shared__ float part[];   // [8 warps][RT * 16][66]
+__global__ void __launch_bounds__(kShrinkThreads, 1)
+adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const int* order, const Tile* tiles, int* done, float* v,
+                      T* vv, float* up, int rows, int K, int R, int rp, int k_range) {
+  extern __shared__ __align__(128) char smem[];   // [stages][pieces][threads] of 16 bytes; then float [warps][RT * 16][66]
   __shared__ int row_of[kTile];
-  constexpr int kPitch = 66;
+  __shared__ bool last;
+  constexpr int kPitch = 66, STAGES = Shrink<RT>::kStages, WARPS = kShrinkThreads / 32, kPiece = kShrinkThreads * 16;
   allow_dependents();
   dependency_wait();
   const Tile tile = tiles[blockIdx.x];
@@ -161,7 +227,6 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
   if (tid < kTile) row_of[tid] = order[tile.start + min(tid, tile.count - 1)];
   const int r0 = blockIdx.y * (RT * 16), S = R / rp;
   const int k0 = blockIdx.z * k_range, k1 = min(K, k0 + k_range);
-  const T* al = a + (long)tile.slot * R * K;
   bool live[RT][2];   // the eight-row halves of the rank tiles that the slices' ranks reach (rp % 8 == 0)
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -177,31 +242,56 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
   __syncthreads();
-  for (int k = k0 + warp * 32; k < k1; k += 256) {
-    const int kk = k + 8 * t;
-    const bool in = kk < k1;
-    uint4 xa[8], aa[RT][2];
+  const int first = k0 + warp * 32;
+  const T* xr[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      xa[j] = in && j < tokens8 ? ld_stream_v4(x + (long)row_of[j * 8 + g] * ldx + kk) : make_uint4(0, 0, 0, 0);
+  for (int j = 0; j < 8; ++j) xr[j] = x + (long)row_of[j * 8 + g] * ldx + 8 * t;
+  const T* ar = a + ((long)tile.slot * R + r0 + g) * K + 8 * t;
+  const uint32_t places = smem_u32(smem) + tid * 16;
+  auto ask = [&](int k, int stage) {
+    if (k < k1) {
+      const bool in = k + 8 * t < k1;
+      const uint32_t to = places + stage * Shrink<RT>::kStage;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < tokens8) copy16(to + j * kPiece, in ? xr[j] + k : x, in);
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (live[i][h]) copy16(to + (8 + 2 * i + h) * kPiece, in ? ar + (long)(i * 16 + h * 8) * K + k : a, in);
+    }
+    commit_copies();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) ask(first + i * (32 * WARPS), i);
+  int stage = 0;
+  for (int k = first; k < k1; k += 32 * WARPS) {
+    copies_but<STAGES - 2>();
+    const uint32_t from = places + stage * Shrink<RT>::kStage;
+    ask(k + (STAGES - 1) * (32 * WARPS), stage == 0 ? STAGES - 1 : stage - 1);   // (where this thread read the chunk before)
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    uint4 aa[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        aa[i][h] = in && live[i][h] ? ld_v4(al + (long)(r0 + i * 16 + h * 8 + g) * K + kk) : make_uint4(0, 0, 0, 0);
+      for (int h = 0; h < 2; ++h) aa[i][h] = live[i][h] ? lds_v4(from + (8 + 2 * i + h) * kPiece) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      if (!live[i][0] && !live[i][1]) continue;
-      const uint32_t lo[4] = {aa[i][0].x, aa[i][1].x, aa[i][0].y, aa[i][1].y};
-      const uint32_t hi[4] = {aa[i][0].z, aa[i][1].z, aa[i][0].w, aa[i][1].w};
+    for (int j = 0; j < 8; ++j) {
+      if (j >= tokens8) break;
+      const uint4 xa = lds_v4(from + j * kPiece);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < tokens8) {
-          Mma<T>::run(acc[i][j], lo, xa[j].x, xa[j].y);
-          Mma<T>::run(acc[i][j], hi, xa[j].z, xa[j].w);
-        }
+      for (int i = 0; i < RT; ++i) {
+        const uint32_t lo[4] = {aa[i][0].x, aa[i][1].x, aa[i][0].y, aa[i][1].y};
+        const uint32_t hi[4] = {aa[i][0].z, aa[i][1].z, aa[i][0].w, aa[i][1].w};
+        Mma<T>::run(acc[i][j], lo, xa.x, xa.y);
+        Mma<T>::run(acc[i][j], hi, xa.z, xa.w);
+      }
     }
   }
+  copies_but<0>();
+  __syncthreads();   // every place has been read: they take the sums
+  float* part = reinterpret_cast<float*>(smem);
   float* mine_part = part + warp * (RT * 16 * kPitch);
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -213,182 +303,277 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
       }
   __syncthreads();
   float* vp = v + ((long)blockIdx.z * rows + tile.start) * R + r0;
-  for (int i = tid; i < tile.count * (RT * 16); i += 256) {
+  for (int i = tid; i < tile.count * (RT * 16); i += kShrinkThreads) {
     const int token = i / (RT * 16), r = i % (RT * 16);
     if (r0 + r >= R) continue;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += part[(w * RT * 16 + r) * kPitch + token];
+    for (int w = 0; w < WARPS; ++w) s += part[(w * RT * 16 + r) * kPitch + token];
     vp[(long)token * R + r] = s;
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(done + blockIdx.x, 1) == (int)(gridDim.y * gridDim.z) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  // a row's sums of one slice: four threads, four neighbouring ranks of 16 each, four planes on their way at a time
+  for (int item = tid >> 2; item - (tid >> 2) < tile.count * S; item += kShrinkThreads / 4) {
+    const int q = tid & 3, token = min(item, tile.count * S - 1) / S, s = min(item, tile.count * S - 1) % S;
+    const long row = (long)tile.start + token;
+    const int mine = rank[tile.slot * S + s], planes = gridDim.z;
+    const float* from = v + row * R + s * rp + q * 4;
+    const long plane = (long)rows * R;
+    auto sum4 = [&](int j) {   // (ranks past the slice's own are none, whatever the row holds)
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j + q * 4 < mine)
+        for (int p = 0; p < planes; p += 4) {
+          uint4 w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = p + e < planes ? __ldcg(reinterpret_cast<const uint4*>(from + (p + e) * plane + j)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f.x += __uint_as_float(w[e].x), f.y += __uint_as_float(w[e].y);
+            f.z += __uint_as_float(w[e].z), f.w += __uint_as_float(w[e].w);
+          }
+        }
+      const int j0 = j + q * 4;
+      return make_float4(f.x, j0 + 1 < mine ? f.y : 0.f, j0 + 2 < mine ? f.z : 0.f, j0 + 3 < mine ? f.w : 0.f);
+    };
+    float4 keep[4];   // the first 64 ranks stay in registers
+    float top = 0.f;
+    auto take = [&](const float4& f) {
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      keep[i] = sum4(i * 16);
+      take(keep[i]);
+    }
+    for (int j = 64; j < mine; j += 16) take(sum4(j));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const Power power = power_of(top);
+    if (item >= tile.count * S) continue;
+    if (q == 0) up[(long)s * rows + row] = power.up;
+    T* to = vv + (((long)s * rows + row) * rp + q * 4) * 2;
+    auto write = [&](int j, const float4& f) {
+      if (j + q * 4 >= rp) return;
+      __align__(16) T e[8];   // the first halves of four ranks, then the second
+      halves<T>(f.x * power.down, e[0], e[4]);
+      halves<T>(f.y * power.down, e[1], e[5]);
+      halves<T>(f.z * power.down, e[2], e[6]);
+      halves<T>(f.w * power.down, e[3], e[7]);
+      *reinterpret_cast<uint4*>(to + j * 2) = *reinterpret_cast<uint4*>(e);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) write(i * 16, keep[i]);
+    for (int j = 64; j < rp; j += 16) write(j, sum4(j));
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// out = y + scale * B v for a tile's rows and 512 columns of one slice, 64 a warp.  Output columns are the 16 rows of an MMA, tokens its
-// columns; row g of product i of four stands for column 8 g + 2 i, row g + 8 for the next one, so that a thread ends with eight
-// neighbouring columns of two tokens: one 16-byte access of y each (two in float32), a warp's accesses whole 128-byte lines.
-// v is a float32 sum and stays one: it goes into the product as two 16-bit numbers whose sum carries 16 bits of it or more (22 in
-// fp16), each row of it multiplied by a power of two that keeps it in fp16's range.
-template <typename T, typename Y, int KT, bool ONE>
-__global__ void __launch_bounds__(256, 1)
-adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const int* rank, const float* scale, const int* order,
-                      const Tile* tiles, const float* v, int rows, int R, int rp, int planes, const Slices slices) {
-  extern __shared__ char raw[];
-  const int pitch = (rp + 15) / 16 * 16 + 8;              // 16-bit numbers of a token; rows 16 bytes apart in the banks
-  T* hi = reinterpret_cast<T*>(raw);                      // [64][pitch]
-  T* lo = hi + kTile * pitch;
-  __shared__ float up[kTile];                             // a token's power of two, undone
-  __shared__ int row_of[kTile];
-  allow_dependents();
-  dependency_wait();
-  const Tile tile = tiles[blockIdx.x];
-  if (tile.count == 0) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  int s = 0;
+// out = y + scale * B v.  Output columns are the 16 rows of an MMA, eight tokens its columns; row g of product i of MT stands for column
+// 2 MT g + 2 i of a warp's 16 MT, row g + 8 for the next one, so that a thread ends with 2 MT neighbouring columns of two tokens: whole
+// 16-byte accesses of y (8 with MT = 2), a warp's in whole lines.
+
+// This thread's part of B's 16 MT columns from column `col` on (that thread's own first), KT * 16 ranks.
+template <int KT, int MT>
+__device__ __forceinline__ void fetch_columns(uint32_t (&w)[MT][KT][4], const void* b, bool in, int steps, int rp, int t) {
+  const char* p = static_cast<const char*>(b) + 8 * t;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      const bool on = in && k < steps && k * 16 + 4 * t < rp;
+      const uint2 p0 = on ? ld_v2(p + (2 * i) * rp * 2 + k * 32) : make_uint2(0u, 0u);
+      const uint2 p1 = on ? ld_v2(p + (2 * i + 1) * rp * 2 + k * 32) : make_uint2(0u, 0u);
+      w[i][k][0] = p0.x, w[i][k][2] = p0.y, w[i][k][1] = p1.x, w[i][k][3] = p1.y;
+    }
+}
+
+// Which slice a part of `columns` columns belongs to, its first column and the slice's end.
+struct Where {
+  int s, col, end;
+};
+__device__ __forceinline__ Where where_is(const Slices& slices, int part, int columns) {
+  int s = 0, start = slices.start[0], end = slices.start[1], first = 0;
 #pragma unroll
   for (int i = 1; i < kMaxSlices; ++i)
-    if (i < slices.n && (int)blockIdx.y >= slices.block[i]) s = i;
-  int c0 = 0, c1 = 0, b0 = 0;
+    if (i < slices.n && part >= slices.part[i]) s = i, start = slices.start[i], end = slices.start[i + 1], first = slices.part[i];
+  return {s, start + (part - first) * columns, end};
+}
+
+// A CTA has 128 MT columns of one slice, 16 MT a warp, and walks over a range of tiles, up to 32 rows (half a tile) at a time; B's part
+// stays in registers as long as the slot does.  Rows of y come by bulk copies, four a warp, with their halves of v, and results go back
+// the same way; what lies between is shared memory and MMAs.  Bound by y, read and written: 8192 rows of 28672 940 MB.
+template <typename Y, int KT, int MT>
+struct Expand {
+  static constexpr int kRowY = 128 * MT * (int)sizeof(Y) + 16;   // (16 apart in the banks: a quad's rows without conflicts)
+  static constexpr int kV = 32 * KT * 64, kUp = 128, kStage = 32 * kRowY + kV + kUp;
+  static constexpr int kFit = (KT <= 1 ? 72 : KT <= 4 ? 108 : 216) * 1024 / kStage, kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
+};
+
+template <typename T, typename Y, int KT, int MT>
+__global__ void __launch_bounds__(256, KT <= 1 ? 3 : KT <= 4 ? 2 : 1)
+adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const int* rank, const float* scale, const int* order,
+                      const Tile* tiles, const T* vv, const float* up, int rows, int rp, int max_tiles, int tiles_each,
+                      const Slices slices, int* status) {
+  extern __shared__ __align__(128) char smem[];   // stages of: y [32][kRowY], v [32][rp / 4][2][4], powers [32]
+  using E = Expand<Y, KT, MT>;
+  constexpr int COLS = 2 * MT, STAGES = E::kStages, BYTES = COLS * (int)sizeof(Y), PB = BYTES < 16 ? BYTES : 16, PIECES = BYTES / PB;
+  __shared__ __align__(8) uint64_t bars[STAGES];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t full = smem_u32(bars), ring = smem_u32(smem);
+  if (tid == 0) {
 #pragma unroll
-  for (int i = 0; i < kMaxSlices; ++i)
-    if (i == s) c0 = slices.start[i], c1 = slices.start[i + 1], b0 = slices.block[i];
-  const int col = c0 + ((int)blockIdx.y - b0) * 512 + warp * 64 + g * 8;   // this thread's eight columns
-  const bool in = col < c1;                                                // (slices are multiples of eight columns)
-  if (tid < kTile) row_of[tid] = order[tile.start + min(tid, tile.count - 1)];
-  const int mine = tile.slot < 0 ? 0 : rank[tile.slot * slices.n + s];
-  if (mine == 0 && y == out) return;
-  const float times = tile.slot < 0 ? 0.f : scale[tile.slot];
-  const int steps = (mine + 15) / 16;
-  if (mine > 0) {
-    // four threads a token
-    const int token = tid >> 2, q = tid & 3;
-    const float* vr = v + ((long)tile.start + token) * R + s * rp;
-    constexpr int NF = (ONE ? KT : kMaxRank / 16) * 4;
-    float f[NF];
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < NF / 4; ++i) {
-      const int j = i * 16 + q * 4;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (token < tile.count && j < mine) {   // (rp % 8 == 0: a group of four that starts inside the rank ends inside rp)
-        for (int p = 0; p < planes; ++p) {
-          const uint4 w = ld_stream_v4(vr + (long)p * rows * R + j);
-          sum.x += __uint_as_float(w.x), sum.y += __uint_as_float(w.y);
-          sum.z += __uint_as_float(w.z), sum.w += __uint_as_float(w.w);
-        }
-      }
-      f[4 * i] = sum.x;
-      f[4 * i + 1] = j + 1 < mine ? sum.y : 0.f;   // ranks past the slot's own are none, whatever the row holds
-      f[4 * i + 2] = j + 2 < mine ? sum.z : 0.f;
-      f[4 * i + 3] = j + 3 < mine ? sum.w : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(f[4 * i + e]));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the largest magnitude goes to 2^13 .. 2^14 (2^100 and 2^-100 at most: beyond that it is 0 or no number for fp16 either way)
-    const int e = top > 0.f && top < 3.4e38f ? max(-100, min(100, 13 - (int)((__float_as_uint(top) >> 23) & 0xffu) + 127)) : 0;
-    const float down = __uint_as_float((uint32_t)(127 + e) << 23);
-    if (q == 0) up[token] = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int i = 0; i < NF / 4; ++i) {
-      const int j = i * 16 + q * 4;
-      if (i < steps) {
-        T h4[4], l4[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float w = f[4 * i + k] * down;
-          h4[k] = narrow<T>(w);
-          const float rest = w - to_f32<T>(h4[k]);
-          l4[k] = narrow<T>(fabsf(w) < 3.4e38f ? rest : 0.f);
-        }
-        *reinterpret_cast<uint2*>(hi + token * pitch + j) = *reinterpret_cast<uint2*>(h4);
-        *reinterpret_cast<uint2*>(lo + token * pitch + j) = *reinterpret_cast<uint2*>(l4);
-      }
-    }
+    for (int i = 0; i < STAGES; ++i) ptx::mbar_init(full + 8 * i, 32);
+    ptx::fence_mbar_init();
   }
+  allow_dependents();
+  dependency_wait();
   __syncthreads();
-  const int passes = ONE ? 1 : (steps + KT - 1) / KT;
-  const T* bl = b + ((long)max(tile.slot, 0) * slices.start[slices.n] + col) * rp + 4 * t;
-  uint32_t w[4][KT][4];
-  auto fetch = [&](int pass) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const int step = pass * KT + k;
-        const bool on = in && step < steps && step * 16 + 4 * t < rp;
-        const uint2 p0 = on ? ld_v2(bl + (2 * i) * rp + step * 16) : make_uint2(0u, 0u);
-        const uint2 p1 = on ? ld_v2(bl + (2 * i + 1) * rp + step * 16) : make_uint2(0u, 0u);
-        w[i][k][0] = p0.x, w[i][k][2] = p0.y, w[i][k][1] = p1.x, w[i][k][3] = p1.y;
-      }
-  };
-  if (ONE) fetch(0);
-  constexpr int YV = sizeof(Y) / 2;   // 16-byte pieces of eight columns
-#pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    const int token0 = half * 32;
-    if (token0 >= tile.count) break;
-    uint4 old[4][2][YV];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int token = token0 + j * 8 + 2 * t + e;
-#pragma unroll
-        for (int p = 0; p < YV; ++p)
-          if (in && token < tile.count) old[j][e][p] = ld_stream_v4(y + (long)row_of[token] * ldy + col + p * 4);
-      }
-    float acc[4][4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.f;
-    for (int pass = 0; pass < passes; ++pass) {
-      if (!ONE) fetch(pass);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (token0 + j * 8 >= tile.count) break;
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          const int step = pass * KT + k;
-          if (step >= steps) break;
-          const int at = (token0 + j * 8 + g) * pitch + step * 16 + 4 * t;
-          const uint2 h = *reinterpret_cast<const uint2*>(hi + at), l = *reinterpret_cast<const uint2*>(lo + at);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            Mma<T>::run(acc[j][i], w[i][k], l.x, l.y);
-            Mma<T>::run(acc[j][i], w[i][k], h.x, h.y);
-          }
-        }
-      }
+  const Where at = where_is(slices, blockIdx.x, 128 * MT);
+  const int tile0 = (int)blockIdx.y * tiles_each, tile_end = min(max_tiles, tile0 + tiles_each);
+  const Tile none = {-1, 0, 0, 0};
+  const bool in_place = y == out;
+  auto tile_at = [&](int i) { return i < tile_end ? tiles[i] : none; };
+  auto rank_at = [&](const Tile& tile) { return tile.slot < 0 ? 0 : rank[tile.slot * slices.n + at.s]; };
+
+  // What the first four lanes of a warp ask for: row 4 warp + lane of part `ap` of tile `asked`, the row's index and power known a part ahead.
+  const bool copies = lane < 4;
+  const int mine_token = warp * 4 + lane;
+  const uint32_t row_bytes = min(128 * MT, at.end - at.col) * (int)sizeof(Y);
+  int ai = tile0, ap = 0, arow = 0;
+  float apower = 0.f;
+  Tile asked = tile_at(ai);
+  int arank = rank_at(asked);
+  auto look = [&]() {
+    if (copies && ap * 32 + mine_token < asked.count) {
+      arow = order[asked.start + ap * 32 + mine_token];
+      if (arank > 0) apower = up[(long)at.s * rows + asked.start + ap * 32 + mine_token];
     }
+  };
+  look();
+  auto ask = [&](int stage) {   // the row that this lane will write back from there, -1: none
+    int held = -1;
+    if (asked.count == 0) return held;
+    if (copies) {
+      const uint32_t to = ring + stage * E::kStage, bar = full + 8 * stage;
+      const int left = min(32, asked.count - ap * 32);
+      const bool on = mine_token < left && !(in_place && arank == 0), first = tid == 0 && arank > 0;
+      if (on) held = arow;
+      if (arank > 0 && mine_token < left)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 32 * E::kRowY + E::kV + mine_token * 4), "f"(apower) : "memory");
+      ptx::mbar_expect_tx(bar, (on ? row_bytes : 0) + (first ? left * rp * 4 : 0));
+      if (on) ptx::bulk_load(to + mine_token * E::kRowY, y + (long)arow * ldy + at.col, row_bytes, bar);
+      if (first)
+        ptx::bulk_load(to + 32 * E::kRowY, vv + ((long)at.s * rows + asked.start + ap * 32) * rp * 2, left * rp * 4, bar);
+    }
+    if (++ap * 32 >= asked.count) {
+      ap = 0;
+      asked = tile_at(++ai);
+      arank = rank_at(asked);
+    }
+    look();
+    return held;
+  };
+  int held[STAGES];   // by parts, the one in hand first
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+  for (int i = 0; i < STAGES - 1; ++i) held[i] = ask(i);
+
+  const int col = at.col + warp * (16 * MT) + g * COLS;
+  const bool in = col < at.end;
+  int turn = 0, stage = 0, slot = -2, mine = 0, steps = 0;
+  float times = 0.f;
+  uint32_t w[MT][KT][4];
+  Tile tile = tile_at(tile0);
+  for (int i = tile0; tile.count > 0; ++i) {
+    const Tile after = tile_at(i + 1);
+    if (tile.slot != slot) {
+      slot = tile.slot;
+      mine = rank_at(tile);
+      times = slot < 0 ? 0.f : scale[slot];
+      steps = (mine + 15) / 16;
+      fetch_columns<KT, MT>(w, b + ((long)max(slot, 0) * slices.N + col) * rp, in, steps, rp, t);
+    }
+    for (int part = 0; part * 32 < tile.count; ++part, ++turn) {
+      const int left = min(32, tile.count - part * 32);
+      await(full + 8 * stage, (turn / STAGES) & 1, status, 181);   // (where it gives up, the rows are wrong and reported as such)
+      const uint32_t from = ring + stage * E::kStage, fv = from + 32 * E::kRowY;
+      if (mine > 0 && warp * (16 * MT) < at.end - at.col) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int token = token0 + j * 8 + 2 * t + e;
-        if (!in || token >= tile.count) continue;
-        if (mine > 0) {
-          const float undo = up[token];
-          Y* old8 = reinterpret_cast<Y*>(old[j][e]);
+        for (int j = 0; j < 4; ++j) {
+          if (j * 8 >= left) break;
+          float acc[MT][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            old8[2 * i] = narrow<Y>(__fmaf_rn(times, acc[j][i][e] * undo, to_f32<Y>(old8[2 * i])));
-            old8[2 * i + 1] = narrow<Y>(__fmaf_rn(times, acc[j][i][2 + e] * undo, to_f32<Y>(old8[2 * i + 1])));
+          for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+          const uint32_t va = fv + (min(j * 8 + g, left - 1) * rp + 4 * t) * 4;
+#pragma unroll
+          for (int k = 0; k < KT; ++k) {
+            if (k >= steps) break;
+            const uint4 v = k * 16 + 4 * t < rp ? lds_v4(va + k * 64) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) Mma<T>::run(acc[m], w[m][k], v.z, v.w);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) Mma<T>::run(acc[m], w[m][k], v.x, v.y);
+          }
+          float undo[2];
+          asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(undo[0]), "=f"(undo[1]) : "r"(fv + E::kV + (j * 8 + 2 * t) * 4) : "memory");
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int token = j * 8 + 2 * t + e;
+            if (!in || token >= left) continue;
+            const uint32_t piece = from + token * E::kRowY + (warp * (16 * MT) + g * COLS) * (int)sizeof(Y);
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+              constexpr int EACH = PB / (int)sizeof(Y);   // columns of a piece
+              uint32_t o[4];
+              if constexpr (PB == 16) {
+                const uint4 q = lds_v4(piece + p * 16);
+                o[0] = q.x, o[1] = q.y, o[2] = q.z, o[3] = q.w;
+              } else {
+                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(o[0]), "=r"(o[1]) : "r"(piece) : "memory");
+              }
+#pragma unroll
+              for (int c = 0; c < EACH; c += 2) {
+                const int m = (p * EACH + c) / 2;   // the MMA row pair of columns c and c + 1
+                const float f0 = acc[m][e] * undo[e], f1 = acc[m][2 + e] * undo[e];
+                if constexpr (sizeof(Y) == 2) {
+                  const float2 old = unpack2<Y>(o[c / 2]);
+                  o[c / 2] = pack2<Y>(make_float2(__fmaf_rn(times, f0, old.x), __fmaf_rn(times, f1, old.y)));
+                } else {
+                  o[c] = __float_as_uint(__fmaf_rn(times, f0, __uint_as_float(o[c])));
+                  o[c + 1] = __float_as_uint(__fmaf_rn(times, f1, __uint_as_float(o[c + 1])));
+                }
+              }
+              if constexpr (PB == 16)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(piece + p * 16), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+              else
+                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(piece), "r"(o[0]), "r"(o[1]) : "memory");
+            }
           }
         }
-#pragma unroll
-        for (int p = 0; p < YV; ++p)
-          *reinterpret_cast<uint4*>(out + (long)row_of[token] * ldo + col + p * 4) = old[j][e][p];
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // what this thread wrote and read, ahead of the bulk copies
+      __syncthreads();
+      if (held[0] >= 0) bulk_store(out + (long)held[0] * ldo + at.col, from + mine_token * E::kRowY, row_bytes);
+      commit_stores();
+#pragma unroll
+      for (int h = 0; h + 2 < STAGES; ++h) held[h] = held[h + 1];
+      stores_read_but<1>();   // the part before this one has left its stage
+      held[STAGES - 2] = ask(stage == 0 ? STAGES - 1 : stage - 1);
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+    tile = after;
   }
+  stores_read_but<0>();
 }
 
 // ---------------------------------------------------------------------------------------------
 struct Plan {
   int R, rp, max_tiles, planes, k_range;
-  size_t order_at, tiles_at, bytes;   // v lies at the scratch's start
+  size_t vv_at, up_at, order_at, tiles_at, done_at, bytes;   // v lies at the scratch's start
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -402,21 +587,54 @@ int make_plan(int T, int K, int L, int rank, int S, Plan* p) {
   p->R = S * rank;
   const int full = T / kTile, most = full + (T < L + 1 ? T : L + 1);
   p->max_tiles = most;
-  // ranges of K: about two CTAs for every SM if tiles were full, at least 256 k each (a chunk of 32 for every warp)
-  const int tiles = (T + kTile - 1) / kTile, chunks = (p->R + 63) / 64;
-  int planes = 2 * sm_count() / (tiles * chunks);
+  // ranges of K: about one CTA for every SM if tiles were full, at least 512 k each
+  const int tiles = (T + kTile - 1) / kTile, chunks = (p->R + 31) / 32;
+  int planes = sm_count() / (tiles * chunks);
   planes = planes < 1 ? 1 : planes > kMaxSplits ? kMaxSplits : planes;
-  const int longest = (K + 255) / 256;
+  const int longest = (K + 511) / 512;
   if (planes > longest) planes = longest;
   p->k_range = ((K + planes - 1) / planes + 255) / 256 * 256;
   p->planes = (K + p->k_range - 1) / p->k_range;
-  size_t at = up256((size_t)p->planes * T * p->R * sizeof(float));
-  p->order_at = at;
-  at += up256((size_t)T * sizeof(int));
-  p->tiles_at = at;
-  at += up256((size_t)p->max_tiles * sizeof(Tile));
+  const size_t cells = (size_t)T * p->R;
+  size_t at = up256(p->planes * cells * sizeof(float));
+  p->vv_at = at, at += up256(cells * 4);
+  p->up_at = at, at += up256((size_t)T * S * sizeof(float));
+  p->order_at = at, at += up256((size_t)T * sizeof(int));
+  p->tiles_at = at, at += up256((size_t)p->max_tiles * sizeof(Tile));
+  p->done_at = at, at += up256((size_t)p->max_tiles * sizeof(int));
   p->bytes = at;
   return LQ_OK;
+}
+
+// The arguments of a call.
+struct Call {
+  const void *x, *a, *b, *ids, *y;
+  void *out, *scratch;
+  const int* ranks;
+  const float* scales;
+  long ldx, ldy, ldo;
+  int T, K, L, ids_64;
+  const int* widths;
+  int n_slices;
+  cudaStream_t st;
+  int* status;
+  int* order(const Plan& p) const { return reinterpret_cast<int*>(static_cast<char*>(scratch) + p.order_at); }
+  Tile* tiles(const Plan& p) const { return reinterpret_cast<Tile*>(static_cast<char*>(scratch) + p.tiles_at); }
+  int* done(const Plan& p) const { return reinterpret_cast<int*>(static_cast<char*>(scratch) + p.done_at); }
+  float* up(const Plan& p) const { return reinterpret_cast<float*>(static_cast<char*>(scratch) + p.up_at); }
+  template <typename T> T* vv(const Plan& p) const { return reinterpret_cast<T*>(static_cast<char*>(scratch) + p.vv_at); }
+};
+
+// Slices cut into parts of `columns`.
+Slices slices_of(const Call& c, int columns) {
+  Slices s = {};
+  s.n = c.n_slices;
+  for (int i = 0; i < c.n_slices; ++i) {
+    s.start[i + 1] = s.start[i] + c.widths[i];
+    s.part[i + 1] = s.part[i] + (c.widths[i] + columns - 1) / columns;
+  }
+  s.N = s.start[s.n], s.parts = s.part[s.n];
+  return s;
 }
 
 template <typename F>
@@ -425,52 +643,54 @@ cudaError_t allow_smem(F* kernel, size_t bytes) {
 }
 
 template <typename T, int RT>
-cudaError_t launch_shrink(const Plan& p, const T* x, long ldx, const T* a, const int* rank, const int* order, const Tile* tiles,
-                          float* v, int rows, int K, cudaStream_t st) {
-  const size_t smem = (size_t)8 * RT * 16 * 66 * sizeof(float);
+cudaError_t launch_shrink(const Plan& p, const Call& c) {
+  const size_t smem = Shrink<RT>::kBytes;
   cudaError_t e = allow_smem(adapter_shrink_kernel<T, RT>, smem);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(adapter_shrink_kernel<T, RT>, dim3(p.max_tiles, (p.R + RT * 16 - 1) / (RT * 16), p.planes), dim3(256),
-                           smem, st, x, ldx, a, rank, order, tiles, v, rows, K, p.R, p.rp, p.k_range);
+  return launch_overlapped(adapter_shrink_kernel<T, RT>, dim3(p.max_tiles, (p.R + RT * 16 - 1) / (RT * 16), p.planes),
+                           dim3(kShrinkThreads), smem, c.st, static_cast<const T*>(c.x), c.ldx, static_cast<const T*>(c.a), c.ranks,
+                           static_cast<const int*>(c.order(p)), static_cast<const Tile*>(c.tiles(p)), c.done(p),
+                           static_cast<float*>(c.scratch), c.vv<T>(p), c.up(p), c.T, c.K, p.R, p.rp, p.k_range);
 }
 
-template <typename T, typename Y, int KT, bool ONE>
-cudaError_t launch_expand(const Plan& p, const Y* y, long ldy, Y* out, long ldo, const T* b, const int* rank, const float* scale,
-                          const int* order, const Tile* tiles, const float* v, int rows, const Slices& slices, cudaStream_t st) {
-  const size_t smem = (size_t)2 * kTile * ((p.rp + 15) / 16 * 16 + 8) * sizeof(T);
-  cudaError_t e = allow_smem(adapter_expand_kernel<T, Y, KT, ONE>, smem);
+template <typename T, typename Y, int KT, int MT>
+cudaError_t launch_expand(const Plan& p, const Call& c) {
+  using E = Expand<Y, KT, MT>;
+  const Slices slices = slices_of(c, 128 * MT);
+  const size_t smem = (size_t)E::kStages * E::kStage;
+  cudaError_t e = allow_smem(adapter_expand_kernel<T, Y, KT, MT>, smem);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(adapter_expand_kernel<T, Y, KT, ONE>, dim3(p.max_tiles, slices.block[slices.n]), dim3(256), smem, st, y,
-                           ldy, out, ldo, b, rank, scale, order, tiles, v, rows, p.R, p.rp, p.planes, slices);
+  // as many tiles for a CTA as leave a few CTAs for every SM
+  const long work = (long)p.max_tiles * slices.parts, slots = (long)sm_count() * 4;
+  const int each = work < slots ? 1 : (int)(work / slots);
+  return launch_overlapped(adapter_expand_kernel<T, Y, KT, MT>, dim3(slices.parts, (p.max_tiles + each - 1) / each), dim3(256), smem,
+                           c.st, static_cast<const Y*>(c.y), c.ldy, static_cast<Y*>(c.out), c.ldo, static_cast<const T*>(c.b),
+                           c.ranks, c.scales, static_cast<const int*>(c.order(p)), static_cast<const Tile*>(c.tiles(p)),
+                           static_cast<const T*>(c.vv<T>(p)), static_cast<const float*>(c.up(p)), c.T, p.rp, p.max_tiles, each,
+                           slices, c.status);
 }
 
 template <typename T, typename Y>
-cudaError_t run_expand(const Plan& p, const void* y, long ldy, void* out, long ldo, const void* b, const int* rank,
-                       const float* scale, const int* order, const Tile* tiles, const float* v, int rows, const Slices& slices,
-                       cudaStream_t st) {
-  auto go = [&](auto launch) {
-    return launch(p, static_cast<const Y*>(y), ldy, static_cast<Y*>(out), ldo, static_cast<const T*>(b), rank, scale, order, tiles, v,
-                  rows, slices, st);
-  };
-  if (p.rp <= 16) return go(launch_expand<T, Y, 1, true>);
-  if (p.rp <= 32) return go(launch_expand<T, Y, 2, true>);
-  if (p.rp <= 64) return go(launch_expand<T, Y, 4, true>);
-  return go(launch_expand<T, Y, 4, false>);
+cudaError_t run_expand(const Plan& p, const Call& c) {
+  if (p.rp <= 16) return launch_expand<T, Y, 1, 4>(p, c);
+  if (p.rp <= 32) return launch_expand<T, Y, 2, 4>(p, c);
+  if (p.rp <= 64) return launch_expand<T, Y, 4, 4>(p, c);
+  if (p.rp <= 128) return launch_expand<T, Y, 8, 4>(p, c);
+  return launch_expand<T, Y, 16, 2>(p, c);
 }
 
 template <typename T>
-cudaError_t run_add(const Plan& p, const void* x, long ldx, const void* a, const void* b, const int* rank, const float* scale,
-                    const void* y, long ldy, int y_f32, void* out, long ldo, int rows, int K, const Slices& slices, int* order,
-                    Tile* tiles, float* v, cudaStream_t st) {
-  const T* xt = static_cast<const T*>(x);
-  const T* at = static_cast<const T*>(a);
-  cudaError_t e;
-  if (p.R <= 16) e = launch_shrink<T, 1>(p, xt, ldx, at, rank, order, tiles, v, rows, K, st);
-  else if (p.R <= 32) e = launch_shrink<T, 2>(p, xt, ldx, at, rank, order, tiles, v, rows, K, st);
-  else e = launch_shrink<T, 4>(p, xt, ldx, at, rank, order, tiles, v, rows, K, st);
+cudaError_t run_add(const Plan& p, const Call& c, int y_f32) {
+  const size_t smem = (size_t)(3 * c.L + 5) * sizeof(int);
+  cudaError_t e = allow_smem(adapter_plan_kernel, smem);
   if (e != cudaSuccess) return e;
-  return y_f32 ? run_expand<T, float>(p, y, ldy, out, ldo, b, rank, scale, order, tiles, v, rows, slices, st)
-               : run_expand<T, T>(p, y, ldy, out, ldo, b, rank, scale, order, tiles, v, rows, slices, st);
+  e = launch_overlapped(adapter_plan_kernel, dim3(1), dim3(1024), smem, c.st, c.ids, c.ids_64 != 0, c.ranks, c.T, c.L, c.n_slices,
+                        c.y != c.out, c.order(p), c.tiles(p), c.done(p), p.max_tiles);
+  if (e != cudaSuccess) return e;
+  if (p.R <= 16) e = launch_shrink<T, 1>(p, c);
+  else e = launch_shrink<T, 2>(p, c);
+  if (e != cudaSuccess) return e;
+  return y_f32 ? run_expand<T, float>(p, c) : run_expand<T, T>(p, c);
 }
 
 }  // namespace
@@ -491,37 +711,21 @@ extern "C" int lq_adapters_add(const void* x, int dtype, long ldx, const void* a
   Plan p;
   const int bad = make_plan(T, K, L, rank, n_slices, &p);
   if (bad) return bad;
-  Slices slices = {};
-  slices.n = n_slices;
   long N = 0;
   for (int s = 0; s < n_slices; ++s) {
     if (widths[s] <= 0) return LQ_ERR_BAD_ARG;
-    if (widths[s] % 8 || widths[s] > (1 << 24)) return LQ_ERR_SHAPE;
-    slices.start[s] = (int)N;
+    if (widths[s] % 8 || widths[s] > (1 << 22)) return LQ_ERR_SHAPE;
     N += widths[s];
-    slices.block[s + 1] = slices.block[s] + (widths[s] + 511) / 512;
   }
-  slices.start[n_slices] = (int)N;
   const int wide = y_f32 ? 4 : 2;
   auto odd = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) != 0; };
   if (odd(x) || odd(a) || odd(b) || odd(y) || odd(out) || ldx % 8 || ldx < 0 || (ldy * wide) % 16 || (ldo * wide) % 16 ||
-      (T > 1 && (ldy < N || ldo < N)) || slices.block[n_slices] > 65535)
+      (T > 1 && (ldy < N || ldo < N)) || N > 1 << 22)
     return LQ_ERR_SHAPE;
   if (!scratch || odd(scratch) || scratch_bytes < p.bytes) return LQ_ERR_WORKSPACE;
-  float* v = static_cast<float*>(scratch);
-  int* order = reinterpret_cast<int*>(static_cast<char*>(scratch) + p.order_at);
-  Tile* tiles = reinterpret_cast<Tile*>(static_cast<char*>(scratch) + p.tiles_at);
-  cudaStream_t st = as_stream(stream);
-  const size_t smem = (size_t)(3 * L + 5) * sizeof(int);
-  cudaError_t e = allow_smem(adapter_plan_kernel, smem);
-  if (e == cudaSuccess)
-    e = launch_overlapped(adapter_plan_kernel, dim3(1), dim3(1024), smem, st, ids, ids_64 != 0, ranks, T, L, n_slices, y != out, order,
-                          tiles, p.max_tiles);
-  if (e == cudaSuccess)
-    e = dtype == LQ_DT_BF16 ? run_add<__nv_bfloat16>(p, x, ldx, a, b, ranks, scales, y, ldy, y_f32, out, ldo, T, K, slices, order,
-                                                     tiles, v, st)
-                            : run_add<__half>(p, x, ldx, a, b, ranks, scales, y, ldy, y_f32, out, ldo, T, K, slices, order, tiles,
-                                              v, st);
+  const Call c = {x, a, b, ids, y, out, scratch, ranks, scales, ldx, ldy, ldo, T, K, L, ids_64, widths, n_slices, as_stream(stream), status_word()};
+  if (!c.status) return LQ_ERR_CUDA;
+  const cudaError_t e = dtype == LQ_DT_BF16 ? run_add<__nv_bfloat16>(p, c, y_f32) : run_add<__half>(p, c, y_f32);
   if (e != cudaSuccess) {
     record_cuda_error(e, "adapters_add");
     return LQ_ERR_CUDA;
