@@ -67,20 +67,17 @@ __device__ __forceinline__ uint2 ld_v2(const void* p) {
   return r;
 }
 
-// The slot of a row, L where it has none (an id outside the slots, a slot without any slice's matrices).
-__device__ __forceinline__ int slot_of(const void* ids, bool wide, long t, int L, int S, const int* rank) {
+// The slot of a row, L where it has none.
+__device__ __forceinline__ int slot_of(const void* ids, bool wide, long t, int L) {
   const long id = wide ? static_cast<const long long*>(ids)[t] : static_cast<const int*>(ids)[t];
-  bool any = false;
-  if (id >= 0 && id < L)
-    for (int s = 0; s < S; ++s) any |= rank[id * S + s] > 0;
-  return any ? (int)id : L;
+  return id >= 0 && id < L ? (int)id : L;
 }
 
 // ---------------------------------------------------------------------------------------------
 // Rows in the order of their slots, tiles.  One CTA.  The order within a slot hangs on atomics; no result does, since a row's sums
 // are its own wherever it lies in a tile.
 __global__ void __launch_bounds__(1024)
-adapter_plan_kernel(const void* ids, bool wide, const int* rank, int T, int L, int S, bool copy_rest, int* order, Tile* tiles,
+adapter_plan_kernel(const void* ids, bool wide, int T, int L, bool copy_rest, int* order, Tile* tiles,
                     int* done, int max_tiles) {
   extern __shared__ int counts[];
   int* first = counts;                // [L + 2] rows before a slot's
@@ -92,11 +89,23 @@ adapter_plan_kernel(const void* ids, bool wide, const int* rank, int T, int L, i
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i <= L; i += blockDim.x) next[i] = 0;
   __syncthreads();
-  for (int t0 = warp * 32; t0 < T; t0 += blockDim.x) {
-    const int t = t0 + lane;
-    const int b = t < T ? slot_of(ids, wide, t, L, S, rank) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, b);
-    if (b >= 0 && lane == __ffs(same) - 1) atomicAdd(&next[b], __popc(same));
+  constexpr int B = 8;   // ids of a thread that are on their way together
+  int slot[B];
+  auto take = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int t = t0 + i * 1024 + tid;
+      slot[i] = t < T ? slot_of(ids, wide, t, L) : -1;
+    }
+  };
+  for (int t0 = 0; t0 < T; t0 += B * 1024) {
+    take(t0);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (t0 + i * 1024 >= T) break;
+      const unsigned same = __match_any_sync(0xffffffffu, slot[i]);
+      if (slot[i] >= 0 && lane == __ffs(same) - 1) atomicAdd(&next[slot[i]], __popc(same));
+    }
   }
   __syncthreads();
   // exclusive sums over the slots, a run of neighbours per thread
@@ -138,15 +147,18 @@ adapter_plan_kernel(const void* ids, bool wide, const int* rank, int T, int L, i
     tiles[i] = tile;
     done[i] = 0;
   }
-  for (int t0 = warp * 32; t0 < T; t0 += blockDim.x) {
-    const int t = t0 + lane;
-    const int b = t < T ? slot_of(ids, wide, t, L, S, rank) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, b);
-    const int leader = __ffs(same) - 1;
-    int at = 0;
-    if (b >= 0 && lane == leader) at = atomicAdd(&next[b], __popc(same));
-    at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1));
-    if (b >= 0) order[at] = t;
+  for (int t0 = 0; t0 < T; t0 += B * 1024) {
+    if (T > B * 1024) take(t0);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (t0 + i * 1024 >= T) break;
+      const unsigned same = __match_any_sync(0xffffffffu, slot[i]);
+      const int leader = __ffs(same) - 1;
+      int at = 0;
+      if (slot[i] >= 0 && lane == leader) at = atomicAdd(&next[slot[i]], __popc(same));
+      at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1));
+      if (slot[i] >= 0) order[at] = t0 + i * 1024 + tid;
+    }
   }
 }
 
@@ -226,7 +238,8 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   if (tid < kTile) row_of[tid] = order[tile.start + min(tid, tile.count - 1)];
   const int r0 = blockIdx.y * (RT * 16), S = R / rp;
-  const int k0 = blockIdx.z * k_range, k1 = min(K, k0 + k_range);
+  const int k0 = blockIdx.z * k_range;
+  int k1 = k0;        // (nothing to sum where no rank is reached)
   bool live[RT][2];   // the eight-row halves of the rank tiles that the slices' ranks reach (rp % 8 == 0)
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -234,6 +247,7 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
     for (int h = 0; h < 2; ++h) {
       const int r = r0 + i * 16 + h * 8;
       live[i][h] = r < R && r % rp < rank[tile.slot * S + r / rp];
+      if (live[i][h]) k1 = min(K, k0 + k_range);
     }
   const int tokens8 = (tile.count + 7) / 8;
   float acc[RT][8][4];
@@ -377,15 +391,15 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
 // 2 MT g + 2 i of a warp's 16 MT, row g + 8 for the next one, so that a thread ends with 2 MT neighbouring columns of two tokens: whole
 // 16-byte accesses of y (8 with MT = 2), a warp's in whole lines.
 
-// This thread's part of B's 16 MT columns from column `col` on (that thread's own first), KT * 16 ranks.
+// This thread's part of 16 MT columns of B (`b`: its own first), KT * 16 ranks of the `left` that their rows still hold.
 template <int KT, int MT>
-__device__ __forceinline__ void fetch_columns(uint32_t (&w)[MT][KT][4], const void* b, bool in, int steps, int rp, int t) {
+__device__ __forceinline__ void fetch_columns(uint32_t (&w)[MT][KT][4], const void* b, bool in, int steps, int rp, int left, int t) {
   const char* p = static_cast<const char*>(b) + 8 * t;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
-      const bool on = in && k < steps && k * 16 + 4 * t < rp;
+      const bool on = in && k < steps && k * 16 + 4 * t < left;
       const uint2 p0 = on ? ld_v2(p + (2 * i) * rp * 2 + k * 32) : make_uint2(0u, 0u);
       const uint2 p1 = on ? ld_v2(p + (2 * i + 1) * rp * 2 + k * 32) : make_uint2(0u, 0u);
       w[i][k][0] = p0.x, w[i][k][2] = p0.y, w[i][k][1] = p1.x, w[i][k][3] = p1.y;
@@ -404,13 +418,14 @@ __device__ __forceinline__ Where where_is(const Slices& slices, int part, int co
   return {s, start + (part - first) * columns, end};
 }
 
-// A CTA has 128 MT columns of one slice, 16 MT a warp, and walks over a range of tiles, up to 32 rows (half a tile) at a time; B's part
-// stays in registers as long as the slot does.  Rows of y come by bulk copies, four a warp, with their halves of v, and results go back
-// the same way; what lies between is shared memory and MMAs.  Bound by y, read and written: 8192 rows of 28672 940 MB.
+// A CTA has 128 MT columns of one slice, 16 MT a warp, and walks over a range of tiles, up to 16 rows at a time; B's part stays in
+// registers as long as the slot does.  Rows of y come by bulk copies, two a warp, with their halves of v, and results go back the same
+// way; what lies between is shared memory and MMAs.  Bound by y, read and written: 8192 rows of 28672 940 MB.
+constexpr int kPart = 16;
 template <typename Y, int KT, int MT>
 struct Expand {
   static constexpr int kRowY = 128 * MT * (int)sizeof(Y) + 16;   // (16 apart in the banks: a quad's rows without conflicts)
-  static constexpr int kV = 32 * KT * 64, kUp = 128, kStage = 32 * kRowY + kV + kUp;
+  static constexpr int kV = kPart * KT * 64, kUp = 128, kStage = kPart * kRowY + kV + kUp;
   static constexpr int kFit = (KT <= 1 ? 72 : KT <= 4 ? 108 : 216) * 1024 / kStage, kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
 };
 
@@ -419,7 +434,7 @@ __global__ void __launch_bounds__(256, KT <= 1 ? 3 : KT <= 4 ? 2 : 1)
 adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const int* rank, const float* scale, const int* order,
                       const Tile* tiles, const T* vv, const float* up, int rows, int rp, int max_tiles, int tiles_each,
                       const Slices slices, int* status) {
-  extern __shared__ __align__(128) char smem[];   // stages of: y [32][kRowY], v [32][rp / 4][2][4], powers [32]
+  extern __shared__ __align__(128) char smem[];   // stages of: y [kPart][kRowY], v [kPart][rp / 4][2][4], powers [kPart]
   using E = Expand<Y, KT, MT>;
   constexpr int COLS = 2 * MT, STAGES = E::kStages, BYTES = COLS * (int)sizeof(Y), PB = BYTES < 16 ? BYTES : 16, PIECES = BYTES / PB;
   __shared__ __align__(8) uint64_t bars[STAGES];
@@ -427,7 +442,7 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
   const uint32_t full = smem_u32(bars), ring = smem_u32(smem);
   if (tid == 0) {
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i) ptx::mbar_init(full + 8 * i, 32);
+    for (int i = 0; i < STAGES; ++i) ptx::mbar_init(full + 8 * i, kPart);
     ptx::fence_mbar_init();
   }
   allow_dependents();
@@ -440,18 +455,18 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
   auto tile_at = [&](int i) { return i < tile_end ? tiles[i] : none; };
   auto rank_at = [&](const Tile& tile) { return tile.slot < 0 ? 0 : rank[tile.slot * slices.n + at.s]; };
 
-  // What the first four lanes of a warp ask for: row 4 warp + lane of part `ap` of tile `asked`, the row's index and power known a part ahead.
-  const bool copies = lane < 4;
-  const int mine_token = warp * 4 + lane;
+  // What the first two lanes of a warp ask for: row 2 warp + lane of part `ap` of tile `asked`, the row's index and power known a part ahead.
+  const bool copies = lane < kPart / 8;
+  const int mine_token = warp * (kPart / 8) + lane;
   const uint32_t row_bytes = min(128 * MT, at.end - at.col) * (int)sizeof(Y);
   int ai = tile0, ap = 0, arow = 0;
   float apower = 0.f;
   Tile asked = tile_at(ai);
   int arank = rank_at(asked);
   auto look = [&]() {
-    if (copies && ap * 32 + mine_token < asked.count) {
-      arow = order[asked.start + ap * 32 + mine_token];
-      if (arank > 0) apower = up[(long)at.s * rows + asked.start + ap * 32 + mine_token];
+    if (copies && ap * kPart + mine_token < asked.count) {
+      arow = order[asked.start + ap * kPart + mine_token];
+      if (arank > 0) apower = up[(long)at.s * rows + asked.start + ap * kPart + mine_token];
     }
   };
   look();
@@ -460,17 +475,17 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
     if (asked.count == 0) return held;
     if (copies) {
       const uint32_t to = ring + stage * E::kStage, bar = full + 8 * stage;
-      const int left = min(32, asked.count - ap * 32);
+      const int left = min(kPart, asked.count - ap * kPart);
       const bool on = mine_token < left && !(in_place && arank == 0), first = tid == 0 && arank > 0;
       if (on) held = arow;
       if (arank > 0 && mine_token < left)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 32 * E::kRowY + E::kV + mine_token * 4), "f"(apower) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + kPart * E::kRowY + E::kV + mine_token * 4), "f"(apower) : "memory");
       ptx::mbar_expect_tx(bar, (on ? row_bytes : 0) + (first ? left * rp * 4 : 0));
       if (on) ptx::bulk_load(to + mine_token * E::kRowY, y + (long)arow * ldy + at.col, row_bytes, bar);
       if (first)
-        ptx::bulk_load(to + 32 * E::kRowY, vv + ((long)at.s * rows + asked.start + ap * 32) * rp * 2, left * rp * 4, bar);
+        ptx::bulk_load(to + kPart * E::kRowY, vv + ((long)at.s * rows + asked.start + ap * kPart) * rp * 2, left * rp * 4, bar);
     }
-    if (++ap * 32 >= asked.count) {
+    if (++ap * kPart >= asked.count) {
       ap = 0;
       asked = tile_at(++ai);
       arank = rank_at(asked);
@@ -495,15 +510,15 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
       mine = rank_at(tile);
       times = slot < 0 ? 0.f : scale[slot];
       steps = (mine + 15) / 16;
-      fetch_columns<KT, MT>(w, b + ((long)max(slot, 0) * slices.N + col) * rp, in, steps, rp, t);
+      fetch_columns<KT, MT>(w, b + ((long)max(slot, 0) * slices.N + col) * rp, in, steps, rp, rp, t);
     }
-    for (int part = 0; part * 32 < tile.count; ++part, ++turn) {
-      const int left = min(32, tile.count - part * 32);
+    for (int part = 0; part * kPart < tile.count; ++part, ++turn) {
+      const int left = min(kPart, tile.count - part * kPart);
       await(full + 8 * stage, (turn / STAGES) & 1, status, 181);   // (where it gives up, the rows are wrong and reported as such)
-      const uint32_t from = ring + stage * E::kStage, fv = from + 32 * E::kRowY;
+      const uint32_t from = ring + stage * E::kStage, fv = from + kPart * E::kRowY;
       if (mine > 0 && warp * (16 * MT) < at.end - at.col) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kPart / 8; ++j) {
           if (j * 8 >= left) break;
           float acc[MT][4];
 #pragma unroll
@@ -568,6 +583,213 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
     tile = after;
   }
   stores_read_but<0>();
+}
+
+// ---------------------------------------------------------------------------------------------
+// A few rows, in one launch.  A cluster for up to eight rows of one adapter (the cluster of the first of them; the others' end at
+// once): its CTAs share out K for the first product, exchange their sums through distributed shared memory, and share out
+// the columns for the second.  A's and B's rows are read from memory straight into MMA operands, B's lines asked for into L2 at the start.
+// Bound by the chain of latencies: ids, rows and weights, the exchange, y.
+constexpr int kFewRanks = 512;    // slices x stack rank
+
+__device__ __forceinline__ float4 peer_v4(uint32_t at, int cta) {
+  uint32_t there;
+  float4 f;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(there) : "memory");
+  return f;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// RT tiles of 16 ranks at a time in the first product, KT steps of 16 in the second.  The code is kept short: a launch that
+// takes a few us waits for its instructions as well (four groups of columns unrolled: one token 9.6 us instead of 7.5).
+template <typename T, typename Y, int RT, int KT>
+__global__ void __launch_bounds__(256, 2)
+adapter_few_kernel(const T* x, long ldx, const Y* y, long ldy, Y* out, long ldo, const T* a, const T* b, const int* rank,
+                   const float* scale, const void* ids, bool wide, int rows, int K, int L, int R, int rp, const Slices slices) {
+  extern __shared__ __align__(128) char smem[];
+  float* mine_v = reinterpret_cast<float*>(smem);               // [R][8] this CTA's sums, which its peers read
+  float* all_v = mine_v + R * 8;                                // [R][8]
+  float* part_v = all_v + R * 8;                                  // [8 warps][16 RT][8]; then the halves: [8 tokens][R / 4 + 1] of 16 bytes
+  __shared__ unsigned same_of[8];
+  __shared__ int row_of[8];
+  __shared__ float up_of[8][kMaxSlices];
+  __shared__ int rank_of[kMaxSlices];
+  allow_dependents();
+  dependency_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int cta = blockIdx.x, ctas = gridDim.x, m = blockIdx.y, S = slices.n, N = slices.N;
+  const int slot = slot_of(ids, wide, m, L);
+  const bool in_place = y == out;
+  if (slot == L) {
+    if (!in_place) {
+      constexpr int EACH = 16 / (int)sizeof(Y);
+      for (int n = (cta * 256 + tid) * EACH; n < N; n += ctas * 256 * EACH)
+        *reinterpret_cast<uint4*>(out + m * ldo + n) = ld_stream_v4(y + m * ldy + n);
+    }
+    return;
+  }
+  const float times = scale[slot];
+  if (tid < S) rank_of[tid] = rank[slot * S + tid];
+  const bool like = tid < rows && slot_of(ids, wide, tid, L) == slot;
+  const unsigned same = __ballot_sync(0xffffffffu, like);
+  if (lane == 0) same_of[warp] = same;
+  __syncthreads();
+  int before = 0, ahead = 0, total = 0;   // rows of the slot ahead of this thread's, of this cluster's, and all
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const unsigned s = same_of[w];
+    total += __popc(s);
+    before += w < warp ? __popc(s) : w == warp ? __popc(s & ((1u << lane) - 1)) : 0;
+    ahead += w < m / 32 ? __popc(s) : w == m / 32 ? __popc(s & ((1u << (m & 31)) - 1)) : 0;
+  }
+  if (ahead % 8) return;
+  const int count = min(8, total - ahead);
+  if (like && before >= ahead && before < ahead + 8) row_of[before - ahead] = tid;
+  const T* al = a + (long)slot * R * K;
+  const T* bl = b + (long)slot * N * rp;
+  const int group0 = cta * 8 + warp, groups = ctas * 8;
+  for (int i = group0; i < slices.parts; i += groups) {   // 64 rows of B are 64 rp neighbours
+    const Where at = where_is(slices, i, 64);
+    for (int line = lane; line < rp; line += 32)
+      if (at.col + line * 64 / rp < at.end)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(bl + (long)at.col * rp) + line * 128));
+  }
+  __syncthreads();
+  const T* xr = x + (long)row_of[min(g, count - 1)] * ldx + 8 * t;
+  const int chunks = (K + 31) / 32;
+  for (int p = 0; p < R; p += 16 * RT) {
+    float acc[RT][4];
+    bool live[RT][2];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = p + i * 16 + h * 8;
+        live[i][h] = r < R && r % rp < rank_of[min(r, R - 1) / rp];
+      }
+    }
+    const T* ar = al + (long)(p + g) * K + 8 * t;
+    for (int c = group0; c < chunks; c += 2 * groups) {   // two chunks of 32 k on their way
+      uint4 xa[2], aa[2][RT][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k = (c + u * groups) * 32;
+        const bool in = k + 8 * t < K;
+        xa[u] = in ? ld_stream_v4(xr + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            aa[u][i][h] = in && live[i][h] ? ld_stream_v4(ar + (long)(i * 16 + h * 8) * K + k) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const uint32_t lo[4] = {aa[u][i][0].x, aa[u][i][1].x, aa[u][i][0].y, aa[u][i][1].y};
+          const uint32_t hi[4] = {aa[u][i][0].z, aa[u][i][1].z, aa[u][i][0].w, aa[u][i][1].w};
+          Mma<T>::run(acc[i], lo, xa[u].x, xa[u].y);
+          Mma<T>::run(acc[i], hi, xa[u].z, xa[u].w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(part_v + (warp * (16 * RT) + i * 16 + h * 8 + g) * 8 + 2 * t) = make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+    __syncthreads();
+    for (int i = tid; i < min(16 * RT, R - p) * 8; i += 256) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += part_v[w * (128 * RT) + i];
+      mine_v[p * 8 + i] = s;
+    }
+    __syncthreads();
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int i = tid; i < R * 2; i += 256) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < ctas; ++c) {
+      const float4 f = peer_v4(smem_u32(mine_v) + i * 16, c);
+      s.x += f.x, s.y += f.y, s.z += f.z, s.w += f.w;
+    }
+    reinterpret_cast<float4*>(all_v)[i] = s;
+  }
+  __syncthreads();
+  cluster_arrive();   // (waited for at the end: peers may be reading this CTA's sums)
+  T* halves_of = reinterpret_cast<T*>(part_v) + warp * (R / 4 + 1) * 8;   // a warp for a token
+  for (int s = 0; s < S; ++s) {
+    const int mine = rank_of[s];
+    float top = 0.f;   // (ranks past the slice's own are none, whatever the row holds)
+    for (int j = lane; j < mine; j += 32) top = fmaxf(top, fabsf(all_v[(s * rp + j) * 8 + warp]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const Power power = power_of(top);
+    if (lane == 0) up_of[warp][s] = power.up;
+    for (int j = lane; j < rp; j += 32) {
+      T h, l;
+      halves<T>(j < mine ? all_v[(s * rp + j) * 8 + warp] * power.down : 0.f, h, l);
+      T* to = halves_of + (s * rp + j) / 4 * 8 + j % 4;
+      to[0] = h, to[4] = l;
+    }
+  }
+  __syncthreads();
+  constexpr int YV = sizeof(Y) / 2;   // 16-byte pieces of eight columns
+  for (int i = group0; i < slices.parts; i += groups) {
+    const Where at = where_is(slices, i, 64);
+    const int mine = rank_of[at.s], steps = (mine + 15) / 16, col = at.col + g * 8;
+    if (mine == 0 && in_place) continue;
+    const bool in = col < at.end;
+    uint4 old[2][YV];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int p = 0; p < YV; ++p)
+        if (in && 2 * t + e < count) old[e][p] = ld_stream_v4(y + row_of[2 * t + e] * ldy + col + p * 4);
+    float acc[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
+    const uint32_t va = smem_u32(part_v) + (g * (R / 4 + 1) + (at.s * rp) / 4 + t) * 16;
+    for (int k0 = 0; k0 < steps; k0 += KT) {
+      uint32_t w[4][KT][4];
+      fetch_columns<KT, 4>(w, bl + (long)col * rp + k0 * 16, in, steps - k0, rp, rp - k0 * 16, t);
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        if (k0 + k >= steps) break;
+        const uint4 v = (k0 + k) * 16 + 4 * t < rp ? lds_v4(va + (k0 + k) * 64) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) Mma<T>::run(acc[q], w[q][k], v.z, v.w);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) Mma<T>::run(acc[q], w[q][k], v.x, v.y);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (!in || 2 * t + e >= count) continue;
+      if (mine > 0) {
+        const float undo = up_of[2 * t + e][at.s];
+        uint32_t* o = reinterpret_cast<uint32_t*>(old[e]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float f0 = acc[q][e] * undo, f1 = acc[q][2 + e] * undo;
+          if constexpr (sizeof(Y) == 2) {
+            const float2 before = unpack2<Y>(o[q]);
+            o[q] = pack2<Y>(make_float2(__fmaf_rn(times, f0, before.x), __fmaf_rn(times, f1, before.y)));
+          } else {
+            o[2 * q] = __float_as_uint(__fmaf_rn(times, f0, __uint_as_float(o[2 * q])));
+            o[2 * q + 1] = __float_as_uint(__fmaf_rn(times, f1, __uint_as_float(o[2 * q + 1])));
+          }
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < YV; ++p) *reinterpret_cast<uint4*>(out + row_of[2 * t + e] * ldo + col + p * 4) = old[e][p];
+    }
+  }
+  cluster_wait();
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -679,13 +901,49 @@ cudaError_t run_expand(const Plan& p, const Call& c) {
   return launch_expand<T, Y, 16, 2>(p, c);
 }
 
+template <typename T, typename Y, int RT, int KT>
+cudaError_t launch_few(const Plan& p, const Call& c) {
+  const size_t halves = (size_t)8 * (p.R / 4 + 1) * 16, sums = (size_t)8 * 16 * RT * 8 * sizeof(float);
+  const size_t smem = (size_t)2 * p.R * 8 * sizeof(float) + (halves > sums ? halves : sums);
+  auto kernel = adapter_few_kernel<T, Y, RT, KT>;
+  cudaError_t e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
+  // as many CTAs for a row as all of them together fit on the SMs, two each
+  int ctas = 8;
+  while (ctas > 1 && (long)ctas * c.T > 2 * sm_count()) ctas /= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, c.T);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = c.st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(c.x), c.ldx, static_cast<const Y*>(c.y), c.ldy, static_cast<Y*>(c.out),
+                            c.ldo, static_cast<const T*>(c.a), static_cast<const T*>(c.b), c.ranks, c.scales, c.ids, c.ids_64 != 0,
+                            c.T, c.K, c.L, p.R, p.rp, slices_of(c, 64));
+}
+
 template <typename T>
 cudaError_t run_add(const Plan& p, const Call& c, int y_f32) {
+  // One launch for few rows.  At 4096 -> 6144 and rank 16 (rows of one adapter / of as many as there are rows), against the three
+  // kernels: 1 row 10 us (13), 32 rows 11 / 14 (17 / 26), 64 rows 14 / 16 (25 / 43), 128 rows 20 / 23 (25 / 44).  Every cluster goes over all
+  // columns, so with 28672 of them 64 rows take 29 / 33 (22 / 54) and 128 rows 52 / 57 (27 / 57).
+  long N = 0;
+  for (int i = 0; i < c.n_slices; ++i) N += c.widths[i];
+  if ((c.T <= 64 || (c.T <= 128 && N <= 8192)) && p.R <= kFewRanks) {
+    if (p.R <= 16) return y_f32 ? launch_few<T, float, 1, 1>(p, c) : launch_few<T, T, 1, 1>(p, c);
+    if (p.rp <= 16) return y_f32 ? launch_few<T, float, 4, 1>(p, c) : launch_few<T, T, 4, 1>(p, c);
+    return y_f32 ? launch_few<T, float, 4, 4>(p, c) : launch_few<T, T, 4, 4>(p, c);
+  }
   const size_t smem = (size_t)(3 * c.L + 5) * sizeof(int);
   cudaError_t e = allow_smem(adapter_plan_kernel, smem);
   if (e != cudaSuccess) return e;
-  e = launch_overlapped(adapter_plan_kernel, dim3(1), dim3(1024), smem, c.st, c.ids, c.ids_64 != 0, c.ranks, c.T, c.L, c.n_slices,
-                        c.y != c.out, c.order(p), c.tiles(p), c.done(p), p.max_tiles);
+  e = launch_overlapped(adapter_plan_kernel, dim3(1), dim3(1024), smem, c.st, c.ids, c.ids_64 != 0, c.T, c.L, c.y != c.out, c.order(p), c.tiles(p), c.done(p), p.max_tiles);
   if (e != cudaSuccess) return e;
   if (p.R <= 16) e = launch_shrink<T, 1>(p, c);
   else e = launch_shrink<T, 2>(p, c);
