@@ -32,14 +32,14 @@ struct Slices {
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 template <> struct Mma<__half> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
@@ -420,7 +420,8 @@ __device__ __forceinline__ Where where_is(const Slices& slices, int part, int co
 
 // A CTA has 128 MT columns of one slice, 16 MT a warp, and walks over a range of tiles, up to 16 rows at a time; B's part stays in
 // registers as long as the slot does.  Rows of y come by bulk copies, two a warp, with their halves of v, and results go back the same
-// way; what lies between is shared memory and MMAs.  Bound by y, read and written: 8192 rows of 28672 940 MB.
+// way; what lies between is shared memory and MMAs.  The copies alone take 23 us for 8192 rows of 4096 and 178 for 28672 (floors 21 and
+// 144); with the products (rank 16, and 64) it is 31 and 357: issue of instructions and copies.  All copying by one warp: 39 and 438.
 constexpr int kPart = 16;
 template <typename Y, int KT, int MT>
 struct Expand {
@@ -524,14 +525,21 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
 #pragma unroll
           for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
           const uint32_t va = fv + (min(j * 8 + g, left - 1) * rp + 4 * t) * 4;
+          constexpr int V = KT < 4 ? KT : 4;   // steps whose halves are read ahead of their products
 #pragma unroll
-          for (int k = 0; k < KT; ++k) {
-            if (k >= steps) break;
-            const uint4 v = k * 16 + 4 * t < rp ? lds_v4(va + k * 64) : make_uint4(0, 0, 0, 0);
+          for (int k0 = 0; k0 < KT; k0 += V) {
+            uint4 v[V];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) Mma<T>::run(acc[m], w[m][k], v.z, v.w);
+            for (int k = 0; k < V; ++k)
+              v[k] = k0 + k < steps && (k0 + k) * 16 + 4 * t < rp ? lds_v4(va + (k0 + k) * 64) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) Mma<T>::run(acc[m], w[m][k], v.x, v.y);
+            for (int k = 0; k < V; ++k) {
+              if (k0 + k >= steps) break;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) Mma<T>::run(acc[m], w[m][k0 + k], v[k].z, v[k].w);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) Mma<T>::run(acc[m], w[m][k0 + k], v[k].x, v[k].y);
+            }
           }
           float undo[2];
           asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(undo[0]), "=f"(undo[1]) : "r"(fv + E::kV + (j * 8 + 2 * t) * 4) : "memory");
