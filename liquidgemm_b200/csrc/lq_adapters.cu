@@ -32,14 +32,14 @@ struct Slices {
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 template <> struct Mma<__half> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
@@ -81,7 +81,7 @@ adapter_plan_kernel(const void* ids, bool wide, int T, int L, bool copy_rest, in
                     int* done, int max_tiles) {
   extern __shared__ int counts[];
   int* first = counts;                // [L + 2] rows before a slot's
-  int* tile0 = counts + L + 2;          // [L + 2] tiles before a slot's
+  int* tile0 = counts + L + 2;        // [L + 2] tiles before a slot's
   int* next = tile0 + L + 2;          // [L + 1] counts, then the next free place
   __shared__ int warp_sum[2][32];
   allow_dependents();
@@ -257,6 +257,7 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
     for (int j = 0; j < 8; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
   __syncthreads();
   const int first = k0 + warp * 32;
+  // (volatile products: a thread's next copies into a place are behind those that used what it held)
   const T* xr[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) xr[j] = x + (long)row_of[j * 8 + g] * ldx + 8 * t;
@@ -502,6 +503,7 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
   const bool in = col < at.end;
   int turn = 0, stage = 0, slot = -2, mine = 0, steps = 0;
   float times = 0.f;
+  bool lost = false;
   uint32_t w[MT][KT][4];
   Tile tile = tile_at(tile0);
   for (int i = tile0; tile.count > 0; ++i) {
@@ -515,7 +517,7 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
     }
     for (int part = 0; part * kPart < tile.count; ++part, ++turn) {
       const int left = min(kPart, tile.count - part * kPart);
-      await(full + 8 * stage, (turn / STAGES) & 1, status, 181);   // (where it gives up, the rows are wrong and reported as such)
+      if (!lost) lost = !await(full + 8 * stage, (turn / STAGES) & 1, status, 181);   // (reported: no more waiting, wrong rows)
       const uint32_t from = ring + stage * E::kStage, fv = from + kPart * E::kRowY;
       if (mine > 0 && warp * (16 * MT) < at.end - at.col) {
 #pragma unroll
@@ -590,6 +592,9 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
     }
     tile = after;
   }
+  if (lost)   // what may still be on its way ends before the CTA does
+    for (int i = 1; i <= STAGES; ++i)
+      if (turn >= i) ptx::mbar_wait_bounded(full + 8 * ((turn - i) % STAGES), ((turn - i) / STAGES) & 1, kWaitLimit);
   stores_read_but<0>();
 }
 

@@ -69,7 +69,8 @@ def _inputs(T, K, N, dtype, seed, y_dtype=None):
     (1, 128, 64, 1, 8), (1, 4096, (512, 128, 128), 5, 16), (2, 8, 8, 3, 1), (7, 264, (72, 24), 4, 5), (32, 1024, 520, 40, 16),
     (63, 520, 136, 3, 12), (64, 512, 256, 2, 32), (65, 512, 256, 1, 24), (200, 2048, (64, 1000, 8), 9, 64),
     (333, 1000, 328, 16, 40), (1000, 640, 1032, 300, 16), (700, 768, (128, 256), 4, 128), (130, 384, 512, 2, 256),
-    (129, 256, (512,) * 8, 3, 72), (4096, 256, 512, 8, 16),
+    (129, 256, (512,) * 8, 3, 72), (4096, 256, 512, 8, 16), (20, 128, (64,) * 8, 4, 72), (100, 64, 8200, 7, 16), (10, 384, 512, 3, 256),
+    (128, 4096, 8192, 128, 16), (65, 256, 8192, 1, 48), (3, 14336, (128, 64, 8), 2, 33), (9000, 64, 72, 500, 8),
 ])
 def test_add(T, K, widths, L, rank, dtype):
     from liquidgemm_b200 import adapters
@@ -89,7 +90,7 @@ def test_add(T, K, widths, L, rank, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-@pytest.mark.parametrize("T,rank", [(3, 16), (90, 32), (300, 64), (65, 200)])
+@pytest.mark.parametrize("T,rank", [(3, 16), (90, 32), (300, 64), (65, 200), (131, 8), (200, 32), (140, 120), (150, 250)])
 def test_float32_outputs(T, rank, dtype):
     from liquidgemm_b200 import adapters
     stack = _stack(4, rank, 512, (136, 72), DTYPES[dtype], 3)
@@ -134,17 +135,18 @@ def test_batches(order):
         assert torch.equal(got.view(torch.int16), y.view(torch.int16))
 
 
-def test_strides():
+@pytest.mark.parametrize("T", [40, 160])
+def test_strides(T):
     from liquidgemm_b200 import adapters
     stack = _stack(3, 16, 256, 64, torch.bfloat16, 1)
-    ids = torch.arange(40, device="cuda") % 3
-    wide_x, wide_y, _ = _inputs(40, 512, 200, torch.bfloat16, 2)
+    ids = torch.arange(T, device="cuda") % 3
+    wide_x, wide_y, _ = _inputs(T, 512, 200, torch.bfloat16, 2)
     x, y = wide_x[:, 128:384], wide_y[:, 8:72]
     want = adapters.add(y.contiguous(), x.contiguous(), stack, ids)
     rest = wide_y.clone()
     assert torch.equal(adapters.add(y, x, stack, ids), want)
     assert torch.equal(adapters.add(wide_y[:, 8:72].t().contiguous().t(), wide_x[:, 128:384].t().contiguous().t(), stack, ids), want)
-    odd = torch.zeros(40 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(40, 64)
+    odd = torch.zeros(T * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(T, 64)
     odd.copy_(y)
     assert torch.equal(adapters.add(odd, x, stack, torch.stack([ids, ids], 1)[:, 0]), want)
     adapters.add(y, x, stack, ids, inplace=True)   # a part of a larger tensor: what stands beside it stays
@@ -165,21 +167,22 @@ def test_no_rows():
                         torch.empty(0, dtype=torch.int64, device="cuda")).shape == (0, 64)
 
 
+@pytest.mark.parametrize("T", [70, 200])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-def test_special_values_stay_in_their_rows(dtype):
+def test_special_values_stay_in_their_rows(dtype, T):
     """Infinities and NaN in x or y reach their own row alone; large and small rows keep their precision."""
     from liquidgemm_b200 import adapters
     dtype = DTYPES[dtype]
     stack = _stack(2, 12, 128, (64, 64), dtype, 4)
     stack["rank"][1, 1] = 0                     # a slice without matrices: not touched by what x holds
-    x, y, _ = _inputs(70, 128, 128, dtype, 5)
+    x, y, _ = _inputs(T, 128, 128, dtype, 5)
     x[3, 5], x[9, 0], y[11, 2] = float("inf"), float("nan"), float("-inf")
     x[20] *= 100.0
     x[21] *= 1e-4
     x[22] = 0.0
-    ids = torch.arange(70, device="cuda") % 2
+    ids = torch.arange(T, device="cuda") % 2
     got = adapters.add(y, x, stack, ids)
-    plain = torch.ones(70, dtype=torch.bool, device="cuda")
+    plain = torch.ones(T, dtype=torch.bool, device="cuda")
     plain[[3, 9, 11]] = False
     _check(got[plain], y[plain], x[plain], stack, ids[plain])
     assert torch.equal(got[22], y[22])
@@ -188,13 +191,14 @@ def test_special_values_stay_in_their_rows(dtype):
     assert got[11, 2] == float("-inf") and torch.isfinite(got[11, 3:]).all()
 
 
-def test_fp16_intermediate_beyond_its_range():
+@pytest.mark.parametrize("T", [5, 150])
+def test_fp16_intermediate_beyond_its_range(T):
     from liquidgemm_b200 import adapters
     stack = adapters.make_stack(1, 8, 1024, 64, dtype=torch.float16)
     adapters.load(stack, 0, torch.full((8, 1024), 30.0), torch.full((64, 8), 2.0 ** -14), 1.0)
-    x = torch.full((5, 1024), 60.0, dtype=torch.float16, device="cuda")   # A x = 1 843 200
-    y = torch.zeros(5, 64, dtype=torch.float16, device="cuda")
-    got = adapters.add(y, x, stack, torch.zeros(5, dtype=torch.int32, device="cuda"))
+    x = torch.full((T, 1024), 60.0, dtype=torch.float16, device="cuda")   # A x = 1 843 200
+    y = torch.zeros(T, 64, dtype=torch.float16, device="cuda")
+    got = adapters.add(y, x, stack, torch.zeros(T, dtype=torch.int32, device="cuda"))
     assert torch.equal(got, torch.full_like(got, 900.0))
 
 
@@ -224,11 +228,12 @@ def test_linear_is_the_linear_and_add(T, w4):
     _check(wide, torch.ops.liquidgemm.w4a8_linear_bias(rows, blob, scales, q.s1, None, N, K, 2), x, stack, ids)
 
 
-def test_graph_replayed_with_other_ids_and_slots():
+@pytest.mark.parametrize("T", [1, 100, 300])
+def test_graph_replayed_with_other_ids_and_slots(T):
     from liquidgemm_b200 import adapters
     stack = _stack(4, 16, 256, 128, torch.bfloat16, 1)
-    x, y, gen = _inputs(100, 256, 128, torch.bfloat16, 2)
-    ids = torch.randint(-1, 4, (100,), device="cuda", generator=gen)
+    x, y, gen = _inputs(T, 256, 128, torch.bfloat16, 2)
+    ids = torch.randint(-1, 4, (T,), device="cuda", generator=gen)
     adapters.add(y, x, stack, ids)
     torch.cuda.synchronize()
     first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
@@ -238,8 +243,8 @@ def test_graph_replayed_with_other_ids_and_slots():
         b = adapters.add(y, x, stack, ids)
     for seed in (3, 4):
         gen.manual_seed(seed)
-        ids.copy_(torch.randint(-1, 4, (100,), device="cuda", generator=gen))
-        x.copy_(torch.randn(100, 256, device="cuda", generator=gen))
+        ids.copy_(torch.randint(-1, 4, (T,), device="cuda", generator=gen))
+        x.copy_(torch.randn(T, 256, device="cuda", generator=gen))
         adapters.load(stack, 1, torch.randn(5, 256, device="cuda", generator=gen) * 0.1, torch.randn(128, 5, device="cuda", generator=gen))
         a.zero_(), b.zero_()
         first.replay()
