@@ -28,7 +28,7 @@ import torch
 
 from ._lib import check, lib
 from .moe import _aligned, _plain_call, _refuse, _same_device
-from .ops import _DTYPE_CODES, _dev_ctx, _impl, _libdef, _req, _stream
+from .ops import _DTYPE_CODES, _dev_ctx, _i8_gemm_scaled, _impl, _libdef, _linear, _quant_per_token, _req
 
 MAX_SLOTS = 4096
 MAX_RANK = 256
@@ -57,59 +57,77 @@ def _c_widths(widths):
     return (ctypes.c_int * len(widths))(*widths)
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Elements from a row of ``t`` [T, n] to the next (of a single row: its own)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+@lru_cache(maxsize=1024)
+def _scratch_bytes(device, T, K, L, r, S):   # (of the current device, whose number keeps devices apart)
+    return lib.lq_adapters_scratch_bytes(T, K, L, r, S)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [T, n] with neighbours next to each other, rows and first element on 16-byte boundaries."""
-    pitch = _pitch(t)
-    if t.stride(1) == 1 and pitch >= t.shape[1] and pitch * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return _aligned(t)
+@lru_cache(maxsize=256)
+def _stack_sizes(a_shape, b_shape, widths):
+    """(L, S, r, K, N) of a stack's matrices; refused where they do not fit each other."""
+    len(a_shape) == 4 and len(b_shape) == 3 or _refuse("the stack's matrices must be [L, S, rank, K] and [L, N, rank]")
+    L, S, r, K = a_shape
+    N = b_shape[1]
+    1 <= L <= MAX_SLOTS and 1 <= S <= MAX_SLICES and 8 <= r <= MAX_RANK and r % 8 == 0 and 8 <= K <= MAX_K and K % 8 == 0 or \
+        _refuse(f"1..{MAX_SLOTS} slots, 1..{MAX_SLICES} slices, a rank of 8..{MAX_RANK} and K up to {MAX_K}, both multiples of 8, required")
+    b_shape[0] == L and b_shape[2] == r or _refuse("the stack's matrices do not fit each other")
+    len(widths) == S and sum(widths) == N <= MAX_CHANNELS and all(w > 0 and w % 8 == 0 for w in widths) or \
+        _refuse(f"widths must be {S} multiples of 8 whose sum is {N}")
+    return L, S, r, K, N
+
+
+def _rows(t: torch.Tensor, size: int):
+    """(t, pitch) of ``t`` [T, n] with neighbours next to each other, rows and first element on 16-byte boundaries (copied where it is not)."""
+    T, n = t.shape
+    pitch, step = t.stride()
+    if T == 1:
+        pitch = n   # a single row has no next
+    if step == 1 and pitch >= n and pitch * size % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, pitch
+    return _aligned(t), n
 
 
 def _run(y, x, a, b, rank, scale, ids, widths, inplace):
-    dtype = x.dtype
-    dtype in (torch.bfloat16, torch.float16) and x.is_cuda and x.dim() == 2 or _refuse("x must be a 2-D CUDA tensor of bf16 or fp16")
-    a.dim() == 4 and b.dim() == 3 and a.dtype is dtype and b.dtype is dtype or \
-        _refuse("the stack's matrices must be [L, S, rank, K] and [L, N, rank] in the type of x")
-    L, S, r, K = a.shape
-    N = b.shape[1]
+    dtype, device = x.dtype, x.device
+    (dtype is torch.bfloat16 or dtype is torch.float16) and x.is_cuda and x.dim() == 2 or _refuse("x must be a 2-D CUDA tensor of bf16 or fp16")
+    a.dtype is dtype and b.dtype is dtype and a.is_contiguous() and b.is_contiguous() or \
+        _refuse("the stack's matrices must be contiguous and in the type of x")
+    widths = tuple(widths)
+    L, S, r, K, N = _stack_sizes(a.shape, b.shape, widths)
     T = x.shape[0]
     x.shape[1] == K or _refuse(f"x must be [T, {K}]")
-    1 <= L <= MAX_SLOTS and 1 <= S <= MAX_SLICES and 8 <= r <= MAX_RANK and r % 8 == 0 and 8 <= K <= MAX_K and K % 8 == 0 or \
-        _refuse(f"1..{MAX_SLOTS} slots, 1..{MAX_SLICES} slices, a rank of 8..{MAX_RANK} and K up to {MAX_K}, both multiples of 8, required")
-    b.shape[0] == L and b.shape[2] == r and a.is_contiguous() and b.is_contiguous() or _refuse("the stack's matrices do not fit each other")
-    widths = tuple(widths)
-    len(widths) == S and sum(widths) == N <= MAX_CHANNELS and all(w > 0 and w % 8 == 0 for w in widths) or \
-        _refuse(f"widths must be {S} multiples of 8 whose sum is {N}")
-    y.is_cuda and y.dim() == 2 and y.shape[0] == T and y.shape[1] == N and (y.dtype is dtype or y.dtype is torch.float32) or \
+    y_f32 = y.dtype is torch.float32
+    y.is_cuda and y.dim() == 2 and y.shape[0] == T and y.shape[1] == N and (y_f32 or y.dtype is dtype) or \
         _refuse(f"y must be CUDA [{T}, {N}] in the type of x or float32")
-    rank.dtype is torch.int32 and scale.dtype is torch.float32 and rank.shape == (L, S) and scale.shape == (L,) or \
-        _refuse(f"rank must be int32 [{L}, {S}] and scale float32 [{L}]")
-    ids.is_cuda and ids.shape == (T,) and ids.dtype in (torch.int32, torch.int64) or _refuse(f"ids must be a CUDA [{T}] tensor of int32 or int64")
+    rank.dtype is torch.int32 and scale.dtype is torch.float32 and rank.shape == (L, S) and scale.shape == (L,) and \
+        rank.is_contiguous() and scale.is_contiguous() or _refuse(f"rank must be int32 [{L}, {S}] and scale float32 [{L}]")
+    wide = ids.dtype is torch.int64
+    ids.is_cuda and ids.dim() == 1 and ids.shape[0] == T and (wide or ids.dtype is torch.int32) or \
+        _refuse(f"ids must be a CUDA [{T}] tensor of int32 or int64")
     T <= MAX_ROWS or _refuse(f"at most {MAX_ROWS} rows")
     _same_device(x, y, a, b, rank, scale, ids)
-    a.data_ptr() % 16 == 0 and b.data_ptr() % 16 == 0 or _refuse("the stack's matrices must start on 16-byte boundaries")
-    if inplace:
-        out = y
-        T == 0 or _rows(y) is y or _refuse("y is changed in place: neighbours next to each other, rows on 16-byte boundaries required")
-    else:
-        out = torch.empty((T, N), dtype=y.dtype, device=y.device)
+    pa, pb = a.data_ptr(), b.data_ptr()
+    (pa | pb) % 16 == 0 or _refuse("the stack's matrices must start on 16-byte boundaries")
     if T == 0:
-        return out
-    x, ids = _rows(x), ids.contiguous()
-    y = out if inplace else _rows(y)
+        return y if inplace else torch.empty_like(y, memory_format=torch.contiguous_format)
+    yr, ldy = _rows(y, 4 if y_f32 else 2)
+    if inplace:
+        yr is y or _refuse("y is changed in place: neighbours next to each other, rows on 16-byte boundaries required")
+        out, ldo = y, ldy
+    else:
+        out, ldo = torch.empty((T, N), dtype=y.dtype, device=device), N
+    x, ldx = _rows(x, 2)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     with _dev_ctx(x):
-        nbytes = lib.lq_adapters_scratch_bytes(T, K, L, r, S)
-        _req(nbytes > 0, "sizes out of range")
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(lib.lq_adapters_add(x.data_ptr(), _DTYPE_CODES[dtype], _pitch(x), a.data_ptr(), b.data_ptr(), rank.data_ptr(),
-                                  scale.data_ptr(), ids.data_ptr(), int(ids.dtype is torch.int64), y.data_ptr(), _pitch(y),
-                                  int(y.dtype is torch.float32), out.data_ptr(), _pitch(out), T, K, L, r, _c_widths(widths), S,
-                                  scratch.data_ptr(), nbytes, _stream()), "adapters_add")
+        nbytes = _scratch_bytes(device.index, T, K, L, r, S)
+        nbytes > 0 or _refuse("sizes out of range")
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        code = lib.lq_adapters_add(x.data_ptr(), _DTYPE_CODES[dtype], ldx, pa, pb, rank.data_ptr(), scale.data_ptr(), ids.data_ptr(), wide,
+                                   yr.data_ptr(), ldy, y_f32, out.data_ptr(), ldo, T, K, L, r, _c_widths(widths), S, scratch.data_ptr(),
+                                   nbytes, torch._C._cuda_getCurrentRawStream(device.index))
+    if code:
+        check(code, "adapters_add")
     return out
 
 
@@ -215,12 +233,16 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
          "x must be bf16 or fp16, out_dtype its type or float32")
     _req(layer["N"] == stack["N"] and layer["K"] == stack["K"], "the stack is for another linear (N and K)")
     code = _DTYPE_CODES[out_dtype]
-    if layer.get("rs") is not None:
-        y = torch.ops.liquidgemm.w4a8_linear(x, layer["rs"], layer["s_u8"], layer["offset_a"], layer["s1"], bias, layer["N"],
-                                             layer["K"], 64, code)
+    blob = layer.get("rs")
+    plain = _plain_call(x, blob if blob is not None else layer["w_i8"], layer["s1"], bias)
+    if blob is not None:
+        run = _linear if plain else torch.ops.liquidgemm.w4a8_linear
+        y = run(x, blob, layer["s_u8"], layer["offset_a"], layer["s1"], bias, layer["N"], layer["K"], 64, code)
     else:
-        rows, scales = torch.ops.liquidgemm.quant_per_token(x)
-        y = torch.ops.liquidgemm.i8_gemm_scaled(rows, layer["w_i8"], scales, layer["s1"], code)
+        quantise, product = (_quant_per_token, _i8_gemm_scaled) if plain else \
+            (torch.ops.liquidgemm.quant_per_token, torch.ops.liquidgemm.i8_gemm_scaled)
+        rows, scales = quantise(x)
+        y = product(rows, layer["w_i8"], scales, layer["s1"], code)
         if bias is not None:
             y = y + bias
     return add(y, x, stack, ids, inplace=True)

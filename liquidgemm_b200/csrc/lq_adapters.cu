@@ -214,7 +214,8 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t at) {
 // way into places of its own in shared memory a chunk ahead (nobody else reads them: no barrier).  The warps' sums meet in shared memory
 // and go to plane blockIdx.z of v [planes][T][R] (R = slices x stack rank), in the order of the plan; the last CTA of a tile adds up the
 // planes, in their order, and writes the sums' halves, vv [slices][T][stack rank / 4][2][4], and the power of two of each.
-// Bound by the stream of x: 8192 rows of 14336 at rank 16 235 MB.
+// Bound by the stream of x and its latencies: 8192 rows of 14336 at rank 16 57 us (235 MB, 4.1 TB/s); eight warps 74, rows by bulk
+// copies of 512 bytes 150.
 constexpr int kShrinkThreads = 512;
 template <int RT>
 struct Shrink {
@@ -336,7 +337,7 @@ adapter_shrink_kernel(const T* x, long ldx, const T* a, const int* rank, const i
   for (int item = tid >> 2; item - (tid >> 2) < tile.count * S; item += kShrinkThreads / 4) {
     const int q = tid & 3, token = min(item, tile.count * S - 1) / S, s = min(item, tile.count * S - 1) % S;
     const long row = (long)tile.start + token;
-    const int mine = rank[tile.slot * S + s], planes = gridDim.z;
+    const int mine = min(rank[tile.slot * S + s], rp), planes = gridDim.z;
     const float* from = v + row * R + s * rp + q * 4;
     const long plane = (long)rows * R;
     auto sum4 = [&](int j) {   // (ranks past the slice's own are none, whatever the row holds)
@@ -422,7 +423,7 @@ __device__ __forceinline__ Where where_is(const Slices& slices, int part, int co
 // A CTA has 128 MT columns of one slice, 16 MT a warp, and walks over a range of tiles, up to 16 rows at a time; B's part stays in
 // registers as long as the slot does.  Rows of y come by bulk copies, two a warp, with their halves of v, and results go back the same
 // way; what lies between is shared memory and MMAs.  The copies alone take 23 us for 8192 rows of 4096 and 178 for 28672 (floors 21 and
-// 144); with the products (rank 16, and 64) it is 31 and 357: issue of instructions and copies.  All copying by one warp: 39 and 438.
+// 144); with the products (rank 16, and 64) it is 32 and 365: issue of instructions and copies.  All copying by one warp: 39 and 438.
 constexpr int kPart = 16;
 template <typename Y, int KT, int MT>
 struct Expand {
@@ -455,7 +456,7 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
   const Tile none = {-1, 0, 0, 0};
   const bool in_place = y == out;
   auto tile_at = [&](int i) { return i < tile_end ? tiles[i] : none; };
-  auto rank_at = [&](const Tile& tile) { return tile.slot < 0 ? 0 : rank[tile.slot * slices.n + at.s]; };
+  auto rank_at = [&](const Tile& tile) { return tile.slot < 0 ? 0 : min(rank[tile.slot * slices.n + at.s], rp); };
 
   // What the first two lanes of a warp ask for: row 2 warp + lane of part `ap` of tile `asked`, the row's index and power known a part ahead.
   const bool copies = lane < kPart / 8;
@@ -602,7 +603,8 @@ adapter_expand_kernel(const Y* y, long ldy, Y* out, long ldo, const T* b, const 
 // A few rows, in one launch.  A cluster for up to eight rows of one adapter (the cluster of the first of them; the others' end at
 // once): its CTAs share out K for the first product, exchange their sums through distributed shared memory, and share out
 // the columns for the second.  A's and B's rows are read from memory straight into MMA operands, B's lines asked for into L2 at the start.
-// Bound by the chain of latencies: ids, rows and weights, the exchange, y.
+// Bound by the chain of latencies (ids, rows and weights, the exchange, y): 6.2 us for one row of 4096 to 4096, 16 for 32 rows with adapters of
+// their own to 6144 (three launches: 12 and 26).
 constexpr int kFewRanks = 512;    // slices x stack rank
 
 __device__ __forceinline__ float4 peer_v4(uint32_t at, int cta) {
@@ -644,7 +646,7 @@ adapter_few_kernel(const T* x, long ldx, const Y* y, long ldy, Y* out, long ldo,
     return;
   }
   const float times = scale[slot];
-  if (tid < S) rank_of[tid] = rank[slot * S + tid];
+  if (tid < S) rank_of[tid] = min(rank[slot * S + tid], rp);
   const bool like = tid < rows && slot_of(ids, wide, tid, L) == slot;
   const unsigned same = __ballot_sync(0xffffffffu, like);
   if (lane == 0) same_of[warp] = same;

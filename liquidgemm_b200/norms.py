@@ -26,7 +26,7 @@ import torch
 
 from ._lib import check, lib
 from .moe import _plain_call, _refuse, _same_device
-from .ops import _DTYPE_CODES, _dev_ctx, _impl, _libdef, _stream
+from .ops import _DTYPE_CODES, _dev_ctx, _impl, _libdef
 
 MAX_WIDTH = 32768
 
@@ -46,72 +46,86 @@ def _f_norm(x, weight, residual, post_weight, gate, eps, scale, residual_scale, 
     return z, q_scale, stream.new_empty(x.shape if _joins(residual, post_weight, gate, scale) else (0,))
 
 
-def _strides(t: torch.Tensor):
+def _strides(t: torch.Tensor, nd: int):
     """(t, outer, inner) of [T, H] or [B, S, H] rows whose elements are neighbours."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] != 1:
         t = t.contiguous()
-    return (t, t.stride(0), t.stride(1)) if t.dim() == 3 else (t, 0, t.stride(0))
+        strides = t.stride()
+    return (t, 0, strides[0]) if nd == 2 else (t, strides[0], strides[1])
 
 
-def _vector(w, name, H, dtype):
-    w.is_cuda and w.shape == (H,) and (w.dtype is dtype or w.dtype is torch.float32) or \
+def _vector(w, name, H, dtype, device):
+    w.is_cuda and w.dim() == 1 and w.shape[0] == H and (w.dtype is dtype or w.dtype is torch.float32) or \
         _refuse(f"{name} must be a CUDA [{H}] tensor in the type of x or float32")
-    return w.contiguous()
+    w.device == device or _refuse(f"{name} must be on the device of x, {device}")
+    return w if w.is_contiguous() else w.contiguous()
+
+
+def _run(x, weight, residual, post_weight, gate, eps, scale, residual_scale, weight_offset, quantize):
+    """(z, scales or None, h or None): the checks of a call cost the host more than a small one's kernel takes, so each value is asked for once."""
+    dtype, shape, device = x.dtype, x.shape, x.device
+    code = _DTYPE_CODES.get(dtype)
+    nd = len(shape)
+    code is not None and (nd == 2 or nd == 3) and x.is_cuda or _refuse("x must be a CUDA [T, H] or [B, S, H] tensor of bf16, fp16 or fp32")
+    H = shape[-1]
+    1 <= H <= MAX_WIDTH or _refuse(f"H must be 1..{MAX_WIDTH}")
+    rows = shape[0] if nd == 2 else shape[0] * shape[1]
+    rows < 1 << 31 or _refuse("fewer than 2^31 rows required")
+    eps >= 0.0 or _refuse("eps must not be negative")
+    joins = scale != 1.0
+    stream, stream_code = dtype, code
+    r = g = w = p = None
+    ro = ri = go = gi = step = g_code = w_code = p_code = 0
+    if residual is not None:
+        joins, stream = True, residual.dtype
+        residual.is_cuda and residual.shape == shape and (stream is dtype or stream is torch.float32) or \
+            _refuse("residual must be a CUDA tensor of x's shape, in the type of x or float32")
+        residual.device == device or _same_device(x, residual)
+        stream_code = _DTYPE_CODES[stream]
+        residual, ro, ri = _strides(residual, nd)
+        r = residual.data_ptr()
+    if weight is not None:
+        weight = _vector(weight, "weight", H, dtype, device)
+        w, w_code = weight.data_ptr(), _DTYPE_CODES[weight.dtype]
+    if post_weight is not None:
+        joins = True
+        post_weight = _vector(post_weight, "post_weight", H, dtype, device)
+        p, p_code = post_weight.data_ptr(), _DTYPE_CODES[post_weight.dtype]
+    if gate is not None:
+        joins = True
+        gate.is_cuda and (gate.dtype is dtype or gate.dtype is torch.float32) or \
+            _refuse("gate must be a CUDA tensor in the type of x or float32")
+        gate.dim() <= nd and all(a == 1 or a == n for a, n in zip(reversed(gate.shape), reversed(shape))) or \
+            _refuse(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+        gate.device == device or _same_device(x, gate)
+        per_row = gate.dim() == 0 or (gate.shape[-1] == 1 and H > 1)
+        if not per_row and H > 1 and gate.stride(-1) != 1:
+            gate = gate.contiguous()
+        wide = gate.expand(shape)
+        go, gi = (wide.stride(0), wide.stride(1)) if nd == 3 else (0, wide.stride(0))
+        g, g_code, step = gate.data_ptr(), _DTYPE_CODES[gate.dtype], 0 if per_row else 1
+    z = torch.empty(shape, dtype=torch.int8 if quantize else dtype, device=device)
+    q_scale = torch.empty(shape[:-1], dtype=torch.float32, device=device) if quantize else None
+    h = torch.empty(shape, dtype=stream, device=device) if joins else None
+    if rows == 0:
+        return z, q_scale, h
+    x, xo, xi = _strides(x, nd)
+    pz = z.data_ptr()
+    with _dev_ctx(x):
+        code = lib.lq_block_norm(x.data_ptr(), code, xo, xi, r, stream_code, ro, ri, g, g_code, go, gi, step, w, w_code, p, p_code,
+                                 None if quantize else pz, pz if quantize else None, q_scale.data_ptr() if quantize else None,
+                                 h.data_ptr() if joins else None, rows, rows if nd == 2 else shape[1], H, eps, scale,
+                                 residual_scale, weight_offset, torch._C._cuda_getCurrentRawStream(device.index))
+    if code:
+        check(code, "block_norm")
+    return z, q_scale, h
 
 
 def _block_norm(x, weight, residual, post_weight, gate, eps, scale, residual_scale, weight_offset, quantize):
-    dtype = x.dtype
-    x.is_cuda and x.dim() in (2, 3) and dtype in _DTYPE_CODES or _refuse("x must be a CUDA [T, H] or [B, S, H] tensor of bf16, fp16 or fp32")
-    shape = x.shape
-    H = shape[-1]
-    rows = x.numel() // H if H else 0
-    1 <= H <= MAX_WIDTH or _refuse(f"H must be 1..{MAX_WIDTH}")
-    rows < 1 << 31 or _refuse("fewer than 2^31 rows required")
-    eps >= 0.0 or _refuse("eps must not be negative")
-    if residual is not None:
-        residual.is_cuda and residual.shape == shape and (residual.dtype is dtype or residual.dtype is torch.float32) or \
-            _refuse("residual must be a CUDA tensor of x's shape, in the type of x or float32")
-    if weight is not None:
-        weight = _vector(weight, "weight", H, dtype)
-    if post_weight is not None:
-        post_weight = _vector(post_weight, "post_weight", H, dtype)
-    if gate is not None:
-        gate.is_cuda and (gate.dtype is dtype or gate.dtype is torch.float32) or \
-            _refuse("gate must be a CUDA tensor in the type of x or float32")
-        gate.dim() <= len(shape) and all(g in (1, n) for g, n in zip(reversed(gate.shape), reversed(shape))) or \
-            _refuse(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
-    _same_device(x, residual, weight, post_weight, gate)
+    z, q_scale, h = _run(x, weight, residual, post_weight, gate, eps, scale, residual_scale, weight_offset, quantize)
     stream = x if residual is None else residual
-    joins = _joins(residual, post_weight, gate, scale)
-    device = x.device
-    z = torch.empty(shape, dtype=torch.int8 if quantize else dtype, device=device)
-    q_scale = torch.empty(shape[:-1] if quantize else (0,), dtype=torch.float32, device=device)
-    h = torch.empty(shape if joins else (0,), dtype=stream.dtype, device=device)
-    if rows == 0:
-        return z, q_scale, h
-    inner = shape[1] if len(shape) == 3 else rows
-    x, xo, xi = _strides(x)
-    r, ro, ri, g, go, gi, step = None, 0, 0, None, 0, 0, 0
-    if residual is not None:
-        residual, ro, ri = _strides(residual)
-        r = residual.data_ptr()
-    if gate is not None:
-        per_row = gate.dim() == 0 or (gate.shape[-1] == 1 and H > 1)
-        if not per_row and gate.stride(-1) != 1 and H > 1:
-            gate = gate.contiguous()
-        wide = gate.expand(shape)
-        go, gi = (wide.stride(0), wide.stride(1)) if len(shape) == 3 else (0, wide.stride(0))
-        g, step = gate.data_ptr(), 0 if per_row else 1
-    with _dev_ctx(x):
-        check(lib.lq_block_norm(x.data_ptr(), _DTYPE_CODES[dtype], xo, xi, r, _DTYPE_CODES[stream.dtype], ro, ri, g,
-                                0 if gate is None else _DTYPE_CODES[gate.dtype], go, gi, step,
-                                None if weight is None else weight.data_ptr(), 0 if weight is None else _DTYPE_CODES[weight.dtype],
-                                None if post_weight is None else post_weight.data_ptr(),
-                                0 if post_weight is None else _DTYPE_CODES[post_weight.dtype],
-                                None if quantize else z.data_ptr(), z.data_ptr() if quantize else None,
-                                q_scale.data_ptr() if quantize else None, h.data_ptr() if joins else None, rows, inner, H,
-                                eps, scale, residual_scale, weight_offset, _stream()), "block_norm")
-    return z, q_scale, h
+    return z, x.new_empty(0, dtype=torch.float32) if q_scale is None else q_scale, stream.new_empty(0) if h is None else h
 
 
 _impl.impl("block_norm", _block_norm)
@@ -122,9 +136,11 @@ _impl.impl("block_norm", _block_norm)
 # --------------------------------------------------------------------------------------
 
 def _call(x, weight, residual, post_weight, gate, eps, scale, residual_scale, weight_offset, quantize):
-    run = _block_norm if _plain_call(x, weight, residual, post_weight, gate) else torch.ops.liquidgemm.block_norm
-    z, q_scale, h = run(x, weight, residual, post_weight, gate, float(eps), float(scale), float(residual_scale),
-                        float(weight_offset), quantize)
+    args = (x, weight, residual, post_weight, gate, float(eps), float(scale), float(residual_scale), float(weight_offset), quantize)
+    if _plain_call(x, weight, residual, post_weight, gate):
+        z, q_scale, h = _run(*args)
+        return z, q_scale, x if h is None else h
+    z, q_scale, h = torch.ops.liquidgemm.block_norm(*args)
     return z, q_scale, h if _joins(residual, post_weight, gate, scale) else x
 
 
