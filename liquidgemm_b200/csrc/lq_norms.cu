@@ -417,8 +417,8 @@ block_norm_kernel(const NormArgs a) {
 // As many CTAs as the GPU holds at once (64 registers a thread), or fewer where all of them then take as many rows.
 template <typename K>
 static cudaError_t launch_rows(K* kernel, const NormArgs& a, int threads, cudaStream_t st) {
-  const int most = 1024 / threads * sm_count(), turns = (a.rows + most - 1) / most;
-  return launch_overlapped(kernel, dim3((a.rows + turns - 1) / turns), dim3(threads), 0, st, a);
+  const long most = 1024 / threads * sm_count(), turns = (a.rows + most - 1) / most;
+  return launch_overlapped(kernel, dim3((unsigned)((a.rows + turns - 1) / turns)), dim3(threads), 0, st, a);
 }
 
 template <typename T, typename R, int NV, bool QUANT>
