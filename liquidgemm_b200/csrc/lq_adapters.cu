@@ -874,15 +874,18 @@ Slices slices_of(const Call& c, int columns) {
   return s;
 }
 
+// A launch of `bytes` of dynamic shared memory.  Up to 48 KB, static shared memory with it (these kernels have less than 1 KB), needs no leave;
+// above, the kernel's limit goes to `most`, what its largest call takes: the limit is the kernel's, so a smaller one, set for
+// another host thread's call, could come between a call's own and its launch.
 template <typename F>
-cudaError_t allow_smem(F* kernel, size_t bytes) {
-  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+cudaError_t allow_smem(F* kernel, size_t bytes, size_t most) {
+  return bytes > 47 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) : cudaSuccess;
 }
 
 template <typename T, int RT>
 cudaError_t launch_shrink(const Plan& p, const Call& c) {
   const size_t smem = Shrink<RT>::kBytes;
-  cudaError_t e = allow_smem(adapter_shrink_kernel<T, RT>, smem);
+  cudaError_t e = allow_smem(adapter_shrink_kernel<T, RT>, smem, smem);
   if (e != cudaSuccess) return e;
   return launch_overlapped(adapter_shrink_kernel<T, RT>, dim3(p.max_tiles, (p.R + RT * 16 - 1) / (RT * 16), p.planes),
                            dim3(kShrinkThreads), smem, c.st, static_cast<const T*>(c.x), c.ldx, static_cast<const T*>(c.a), c.ranks,
@@ -895,7 +898,7 @@ cudaError_t launch_expand(const Plan& p, const Call& c) {
   using E = Expand<Y, KT, MT>;
   const Slices slices = slices_of(c, 128 * MT);
   const size_t smem = (size_t)E::kStages * E::kStage;
-  cudaError_t e = allow_smem(adapter_expand_kernel<T, Y, KT, MT>, smem);
+  cudaError_t e = allow_smem(adapter_expand_kernel<T, Y, KT, MT>, smem, smem);
   if (e != cudaSuccess) return e;
   // as many tiles for a CTA as leave a few CTAs for every SM
   const long work = (long)p.max_tiles * slices.parts, slots = (long)sm_count() * 4;
@@ -918,10 +921,13 @@ cudaError_t run_expand(const Plan& p, const Call& c) {
 
 template <typename T, typename Y, int RT, int KT>
 cudaError_t launch_few(const Plan& p, const Call& c) {
-  const size_t halves = (size_t)8 * (p.R / 4 + 1) * 16, sums = (size_t)8 * 16 * RT * 8 * sizeof(float);
-  const size_t smem = (size_t)2 * p.R * 8 * sizeof(float) + (halves > sums ? halves : sums);
+  auto bytes = [](size_t R) {
+    const size_t halves = 8 * (R / 4 + 1) * 16, sums = (size_t)8 * 16 * RT * 8 * sizeof(float);
+    return 2 * R * 8 * sizeof(float) + (halves > sums ? halves : sums);
+  };
+  const size_t smem = bytes(p.R);
   auto kernel = adapter_few_kernel<T, Y, RT, KT>;
-  cudaError_t e = allow_smem(kernel, smem);
+  cudaError_t e = allow_smem(kernel, smem, bytes(kFewRanks));
   if (e != cudaSuccess) return e;
   // as many CTAs for a row as all of them together fit on the SMs, two each
   int ctas = 8;
@@ -956,7 +962,7 @@ cudaError_t run_add(const Plan& p, const Call& c, int y_f32) {
     return y_f32 ? launch_few<T, float, 4, 4>(p, c) : launch_few<T, T, 4, 4>(p, c);
   }
   const size_t smem = (size_t)(3 * c.L + 5) * sizeof(int);
-  cudaError_t e = allow_smem(adapter_plan_kernel, smem);
+  cudaError_t e = allow_smem(adapter_plan_kernel, smem, (size_t)(3 * kMaxSlots + 5) * sizeof(int));
   if (e != cudaSuccess) return e;
   e = launch_overlapped(adapter_plan_kernel, dim3(1), dim3(1024), smem, c.st, c.ids, c.ids_64 != 0, c.T, c.L, c.y != c.out, c.order(p), c.tiles(p), c.done(p), p.max_tiles);
   if (e != cudaSuccess) return e;
