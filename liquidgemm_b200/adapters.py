@@ -232,6 +232,11 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
     _req(x.dtype in (torch.bfloat16, torch.float16) and out_dtype in (x.dtype, torch.float32),
          "x must be bf16 or fp16, out_dtype its type or float32")
     _req(layer["N"] == stack["N"] and layer["K"] == stack["K"], "the stack is for another linear (N and K)")
+    if bias is not None:   # (one contract for both weight kinds: no broadcast, no promotion of the result)
+        bias.is_cuda and bias.dtype == out_dtype and bias.numel() == layer["N"] or \
+            _refuse(f"bias must be a CUDA [{layer['N']}] tensor of the output type, {out_dtype}")
+        _same_device(x, bias)
+        bias = bias.reshape(-1)
     code = _DTYPE_CODES[out_dtype]
     blob = layer.get("rs")
     plain = _plain_call(x, blob if blob is not None else layer["w_i8"], layer["s1"], bias)
@@ -244,5 +249,5 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
         rows, scales = quantise(x)
         y = product(rows, layer["w_i8"], scales, layer["s1"], code)
         if bias is not None:
-            y = y + bias
+            y = y.add_(bias) if plain else y + bias
     return add(y, x, stack, ids, inplace=True)
