@@ -222,6 +222,72 @@ __device__ __noinline__ int code_exact(float t, float top) {
   return q == q ? max(-127, min(127, __double2int_rn(q))) : 0;
 }
 
+template <typename T> __device__ __forceinline__ T rounded(double v);
+template <> __device__ __forceinline__ float rounded<float>(double v) { return (float)v; }
+template <> __device__ __forceinline__ __half rounded<__half>(double v) { return __float2half_rn((float)v); }
+template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(double v) { return __float2bfloat16_rn((float)v); }
+
+__device__ __forceinline__ long row_start(const RowStrides& s, unsigned m, const NormArgs& a) {
+  if (a.inner == a.rows) return (long)m * s.inner;
+  const unsigned outer = m / (unsigned)a.inner;
+  return (long)outer * s.outer + (long)(m - outer * a.inner) * s.inner;
+}
+
+// A row whose sum of squares float32 does not hold, element by element in 64 bits, from its operands in memory.  A function
+// of its own that ends the row: what hardly any row takes then costs the others no registers (the elements taken again inside the kernel's
+// own code: 7 to 24 % of all rows' time where 16-byte accesses do not go).  `sums`: 32 doubles, the maxima behind them.
+template <typename T, typename R, bool QUANT>
+__device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, double* sums) {
+  const int H = a.H, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  float* tops = reinterpret_cast<float*>(sums + 32);
+  auto sum_max = [&](double s, float& top) {
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    __syncthreads();   // (what was read from there before)
+    if ((threadIdx.x & 31) == 0) sums[warp] = s, tops[warp] = top;
+    __syncthreads();
+    s = 0.0;
+    for (int w = 0; w < warps; ++w) s += sums[w], top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(tops[w])));
+    return s;
+  };
+  auto weight = [&](const void* p, bool f32, int e) {
+    return (f32 ? static_cast<const float*>(p)[e] : to_f32<T>(static_cast<const T*>(p)[e])) + a.offset;
+  };
+  auto root_of = [&](double s) { return rsqrt(s * a.inv_h + a.eps); };
+  const T* x = static_cast<const T*>(a.x) + row_start(a.xs, m, a);
+  R* h = static_cast<R*>(a.h) + (long)m * H;
+  double s = 0.0, root = 1.0;
+  float top = 0.f;
+  if (a.post) {
+#pragma unroll 1
+    for (int e = threadIdx.x; e < H; e += blockDim.x) s = fma((double)to_f32<T>(x[e]), (double)to_f32<T>(x[e]), s);
+    root = root_of(sum_max(s, top));
+  }
+  s = 0.0;
+#pragma unroll 1
+  for (int e = threadIdx.x; e < H; e += blockDim.x) {
+    double p = a.scale * root * to_f32<T>(x[e]);
+    if (a.post) p *= weight(a.post, a.post_f32, e);
+    if (a.gate) {
+      const long at = row_start(a.gs, m, a) + (a.gate_step ? e : 0);
+      p *= a.gate_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
+    }
+    if (a.residual) p = fma(a.residual_scale, (double)to_f32<R>((static_cast<const R*>(a.residual) + row_start(a.rs, m, a))[e]), p);
+    h[e] = rounded<R>(p);
+    const float v = to_f32<R>(h[e]), t = a.weight ? v * weight(a.weight, a.weight_f32, e) : v;
+    s = fma((double)v, (double)v, s);
+    top = max_abs_nan(top, t, t);
+  }
+  root = root_of(sum_max(s, top));
+  if (QUANT && threadIdx.x == 0) a.q_scale[m] = (float)(top * root / 127.0);
+#pragma unroll 1
+  for (int e = threadIdx.x; e < H; e += blockDim.x) {   // (this thread's own elements of h)
+    const float v = to_f32<R>(h[e]), w = a.weight ? weight(a.weight, a.weight_f32, e) : 1.f;
+    if constexpr (QUANT) a.q[(long)m * H + e] = (int8_t)code_exact(v * w, top);
+    else static_cast<T*>(a.z)[(long)m * H + e] = rounded<T>(v * root * w);
+  }
+}
+
 // A CTA takes row after row, each in registers (NV units of eight elements a thread), so that everything is read once:
 //   p = x * (mean(x^2) + eps)^-1/2 * (post + offset)        (with `post`; x otherwise)
 //   h = residual_scale * residual + scale * gate * p         rounded to the stream's type R, and stored
@@ -241,8 +307,9 @@ __device__ __noinline__ int code_exact(float t, float top) {
 // of 58 at 4096 x 8192).  Rows that 16-byte accesses cannot take (8192 x 5001: 114 us, 2.9 TB/s) are bound by instruction issue too.
 template <typename T, typename R, int NV, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(VEC ? 1024 : 512, VEC ? 1 : 2)
-block_norm_kernel(const NormArgs a) {
+block_norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ __align__(16) float red[2][3][64];
+  __shared__ double outlying[48];
   constexpr bool HOLD = VEC && NV == 1 && !QUANT;
   for (int i = threadIdx.x; i < 2 * 3 * 64; i += blockDim.x) (&red[0][0][0])[i] = 0.f;
   __syncthreads();
@@ -250,11 +317,7 @@ block_norm_kernel(const NormArgs a) {
   dependency_wait();
   const int H = a.H;
   const bool gate16 = a.gate && a.gate_step && !a.gate_f32;
-  auto row_at = [&](const RowStrides& s, unsigned m) {
-    if (a.inner == a.rows) return (long)m * s.inner;
-    const unsigned outer = m / (unsigned)a.inner;
-    return (long)outer * s.outer + (long)(m - outer * a.inner) * s.inner;
-  };
+  auto row_at = [&](const RowStrides& s, unsigned m) { return row_start(s, m, a); };
   const Factor rs = split(a.residual_scale);
   const bool sum = a.residual && !a.post && a.scale == 1.0 && a.residual_scale == 1.0;   // h = residual + gate * x
   const Factor scale = split(a.scale);
@@ -299,7 +362,11 @@ block_norm_kernel(const NormArgs a) {
       }
       // (every thread takes the same way: the sum has the same bits everywhere)
       const float ss = block_sum_max<false>(s.x + s.y, 0.f, red[parity][0]).x;
-      by = split((ss < 3e38f ? exact_root(ss, a) : root_of_large<T, NV, VEC>(x, H, a.inv_h, red[parity][0])) * a.scale);
+      if (!(ss < 3e38f)) {   // (float32 may not hold such elements times a weight and a gate either)
+        outlying_row<T, R, QUANT>(a, m, outlying);
+        continue;
+      }
+      by = split(exact_root(ss, a) * a.scale);
     }
     if (a.gate) {
 #pragma unroll
