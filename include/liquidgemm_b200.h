@@ -380,7 +380,9 @@ LQ_API int lq_adapters_add(const void* x, int dtype, long ldx, const void* a, co
  * residual, gate, weight and post may be null (left out: no such term or factor), and, where nothing but x makes h, so may h.  stream_dtype: that of residual and h,
  * x_dtype or, with a residual, LQ_DT_F32.  gate, weight, post: x_dtype or LQ_DT_F32.  Row m of x, residual and gate lies
  * (m / inner) * outer + (m % inner) * inner_stride elements behind the pointer (x_outer, x_inner, ...); gate_step 1: H gates a row, 0:
- * one.  z, q and h are contiguous.  H <= 32768; eps >= 0.  Any alignment; 16-byte aligned rows of a multiple of 8 elements are faster. */
+ * one.  z, q and h are contiguous.  H <= 32768; eps >= 0.  Any alignment; 16-byte aligned rows of a multiple of 8 elements are faster.
+ * Rows with a sum of squares that float32 does not hold, too large or (beside eps) too small, are taken in 64 bits; rows of zeros stay zeros
+ * with eps 0 as well (q_scale 0). */
 LQ_API int lq_block_norm(const void* x, int x_dtype, long x_outer, long x_inner, const void* residual, int stream_dtype,
                          long r_outer, long r_inner, const void* gate, int gate_dtype, long g_outer, long g_inner,
                          int gate_step, const void* weight, int weight_dtype, const void* post, int post_dtype, void* z,

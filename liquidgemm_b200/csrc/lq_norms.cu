@@ -196,24 +196,6 @@ __device__ __forceinline__ double exact_root(float ss, const NormArgs& a) {
   return r < INFINITY ? fma(0.5 * r, fma(-m * r, (double)r, 1.0), (double)r) : (double)r;
 }
 
-// The same of a row whose squares float32 does not hold (`ss` says so): those of the row times 2^-80 are summed instead, which neither exceed nor
-// fall below that and beside which eps does not count.  Each thread reads its own elements of `row` again.
-template <typename T, int NV, bool VEC>
-__device__ __noinline__ double root_of_large(const T* row, int H, double inv_h, float* red) {
-  float s = 0.f;
-#pragma unroll 1
-  for (int i = 0; i < NV; ++i)
-#pragma unroll 1
-    for (int j = 0; j < 8; ++j) {
-      const int e = unit_at<VEC>(i) + (VEC ? j : j * 32);
-      const float v = e < H ? to_f32<T>(row[e]) * 0x1p-80f : 0.f;
-      s = __fmaf_rn(v, v, s);
-    }
-  __syncthreads();
-  s = block_sum_max<false>(s, 0.f, red).x;
-  return 0x1p-80 * rsqrt((double)s * inv_h);
-}
-
 // round(127 t / top) of an element that lies next to a border between two codes, or whose factor 127 / top float32 does not
 // hold.  The product by 127 is exact and the quotient of two float32 numbers is never nearer to a half-integer than 64 bits can
 // tell, unless it is one.
@@ -233,11 +215,14 @@ __device__ __forceinline__ long row_start(const RowStrides& s, unsigned m, const
   return (long)outer * s.outer + (long)(m - outer * a.inner) * s.inner;
 }
 
-// A row whose sum of squares float32 does not hold, element by element in 64 bits, from its operands in memory.  A function
-// of its own that ends the row: what hardly any row takes then costs the others no registers (the elements taken again inside the kernel's
-// own code: 7 to 24 % of all rows' time where 16-byte accesses do not go).  `sums`: 32 doubles, the maxima behind them.
+// Whether float32 holds a row's sum of squares, and the `mean` of them and eps: each square may be off by 2^-150, 2^-30 of the least mean here.
+__device__ __forceinline__ bool holds(float ss, float mean) { return ss < 3e38f && mean >= 0x1p-120f; }
+
+// A row of which it does not, element by element in 64 bits: from its operands in memory, or, where that is `formed` already, from its
+// stream.  A function of its own that ends the row: what hardly any row takes then costs the others no registers (the elements taken again
+// inside the kernel's own code: 7 to 24 % of all rows' time where 16-byte accesses do not go).  `sums`: 32 doubles, the maxima behind them.
 template <typename T, typename R, bool QUANT>
-__device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, double* sums) {
+__device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, bool formed, double* sums) {
   const int H = a.H, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   float* tops = reinterpret_cast<float*>(sums + 32);
   auto sum_max = [&](double s, float& top) {
@@ -253,12 +238,14 @@ __device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, double*
   auto weight = [&](const void* p, bool f32, int e) {
     return (f32 ? static_cast<const float*>(p)[e] : to_f32<T>(static_cast<const T*>(p)[e])) + a.offset;
   };
-  auto root_of = [&](double s) { return rsqrt(s * a.inv_h + a.eps); };
+  auto root_of = [&](double s) { return s == 0.0 ? 0.0 : rsqrt(s * a.inv_h + a.eps); };   // (zeros stay zeros, whatever eps)
   const T* x = static_cast<const T*>(a.x) + row_start(a.xs, m, a);
   R* h = static_cast<R*>(a.h) + (long)m * H;
+  const R* row = a.h ? h : reinterpret_cast<const R*>(x);
   double s = 0.0, root = 1.0;
   float top = 0.f;
-  if (a.post) {
+  __syncthreads();   // (the stream as the other threads stored it)
+  if (a.post && !formed) {
 #pragma unroll 1
     for (int e = threadIdx.x; e < H; e += blockDim.x) s = fma((double)to_f32<T>(x[e]), (double)to_f32<T>(x[e]), s);
     root = root_of(sum_max(s, top));
@@ -266,23 +253,25 @@ __device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, double*
   s = 0.0;
 #pragma unroll 1
   for (int e = threadIdx.x; e < H; e += blockDim.x) {
-    double p = a.scale * root * to_f32<T>(x[e]);
-    if (a.post) p *= weight(a.post, a.post_f32, e);
-    if (a.gate) {
-      const long at = row_start(a.gs, m, a) + (a.gate_step ? e : 0);
-      p *= a.gate_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
+    if (!formed) {
+      double p = a.scale * root * to_f32<T>(x[e]);
+      if (a.post) p *= weight(a.post, a.post_f32, e);
+      if (a.gate) {
+        const long at = row_start(a.gs, m, a) + (a.gate_step ? e : 0);
+        p *= a.gate_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
+      }
+      if (a.residual) p = fma(a.residual_scale, (double)to_f32<R>((static_cast<const R*>(a.residual) + row_start(a.rs, m, a))[e]), p);
+      h[e] = rounded<R>(p);
     }
-    if (a.residual) p = fma(a.residual_scale, (double)to_f32<R>((static_cast<const R*>(a.residual) + row_start(a.rs, m, a))[e]), p);
-    h[e] = rounded<R>(p);
-    const float v = to_f32<R>(h[e]), t = a.weight ? v * weight(a.weight, a.weight_f32, e) : v;
+    const float v = to_f32<R>(row[e]), t = a.weight ? v * weight(a.weight, a.weight_f32, e) : v;
     s = fma((double)v, (double)v, s);
     top = max_abs_nan(top, t, t);
   }
   root = root_of(sum_max(s, top));
   if (QUANT && threadIdx.x == 0) a.q_scale[m] = (float)(top * root / 127.0);
 #pragma unroll 1
-  for (int e = threadIdx.x; e < H; e += blockDim.x) {   // (this thread's own elements of h)
-    const float v = to_f32<R>(h[e]), w = a.weight ? weight(a.weight, a.weight_f32, e) : 1.f;
+  for (int e = threadIdx.x; e < H; e += blockDim.x) {
+    const float v = to_f32<R>(row[e]), w = a.weight ? weight(a.weight, a.weight_f32, e) : 1.f;
     if constexpr (QUANT) a.q[(long)m * H + e] = (int8_t)code_exact(v * w, top);
     else static_cast<T*>(a.z)[(long)m * H + e] = rounded<T>(v * root * w);
   }
@@ -308,10 +297,10 @@ __device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, double*
 template <typename T, typename R, int NV, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(VEC ? 1024 : 512, VEC ? 1 : 2)
 block_norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ __align__(16) float red[2][3][64];
+  __shared__ __align__(16) float red[2][2][64];
   __shared__ double outlying[48];
   constexpr bool HOLD = VEC && NV == 1 && !QUANT;
-  for (int i = threadIdx.x; i < 2 * 3 * 64; i += blockDim.x) (&red[0][0][0])[i] = 0.f;
+  for (int i = threadIdx.x; i < 2 * 2 * 64; i += blockDim.x) (&red[0][0][0])[i] = 0.f;
   __syncthreads();
   allow_dependents();
   dependency_wait();
@@ -362,8 +351,8 @@ block_norm_kernel(const __grid_constant__ NormArgs a) {
       }
       // (every thread takes the same way: the sum has the same bits everywhere)
       const float ss = block_sum_max<false>(s.x + s.y, 0.f, red[parity][0]).x;
-      if (!(ss < 3e38f)) {   // (float32 may not hold such elements times a weight and a gate either)
-        outlying_row<T, R, QUANT>(a, m, outlying);
+      if (!holds(ss, __fmaf_rn(ss, inv_h, eps))) {   // (float32 may not hold the elements times a weight and a gate either)
+        outlying_row<T, R, QUANT>(a, m, false, outlying);
         continue;
       }
       by = split(exact_root(ss, a) * a.scale);
@@ -410,7 +399,6 @@ block_norm_kernel(const __grid_constant__ NormArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) ss2 = fma2(v[i][j], v[i][j], ss2);
     }
-    if (!a.h) row = const_cast<R*>(reinterpret_cast<const R*>(x));
     float2 w[HOLD ? NV : 1][4];   // the norm's weight, held where there are registers for it
     float top = 0.f;
     if constexpr (QUANT || HOLD) {
@@ -428,10 +416,13 @@ block_norm_kernel(const __grid_constant__ NormArgs a) {
       }
     }
     const float2 both_of = block_sum_max<QUANT>(ss2.x + ss2.y, top, red[parity][1]);
-    const bool large = !(both_of.x < 3e38f);
+    const float mean = __fmaf_rn(both_of.x, inv_h, eps);
+    if (!holds(both_of.x, mean)) {
+      outlying_row<T, R, QUANT>(a, m, true, outlying);
+      continue;
+    }
     float root = 0.f;
-    if (large) root = (float)root_of_large<R, NV, VEC>(row, H, a.inv_h, red[parity][2]);
-    else if (!QUANT || threadIdx.x == 0) root = __frsqrt_rn(__fmaf_rn(both_of.x, inv_h, eps));
+    if (!QUANT || threadIdx.x == 0) root = __frsqrt_rn(mean);
     if constexpr (!QUANT) {
       T* z = static_cast<T*>(a.z) + (long)m * H;
 #pragma unroll
@@ -440,9 +431,8 @@ block_norm_kernel(const __grid_constant__ NormArgs a) {
         if (!HOLD && a.weight) load_weight<T, VEC>(a.weight, a.weight_f32, a.offset, unit_at<VEC>(i), H, wi);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (large) v[i][j] = mul2(v[i][j], both(root));   // (products with the weights that float32 may not hold: by the root first)
           if (a.weight) v[i][j] = mul2(v[i][j], wi[j]);
-          if (!large) v[i][j] = mul2(v[i][j], both(root));
+          v[i][j] = mul2(v[i][j], both(root));
         }
         Rounded<T>(v[i]).template store<VEC>(z, unit_at<VEC>(i), H);
       }

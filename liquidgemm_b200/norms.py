@@ -153,7 +153,9 @@ def block_norm(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Option
     ``weight`` and ``post_weight`` are [H] in the type of ``x`` or float32, plus ``weight_offset`` each (1 where a checkpoint stores them
     around 0); ``weight`` None: no weights.  ``gate`` broadcasts to ``x``: one number for a channel, a row, a sequence ([B, 1, H]) or
     every element.  Everything is float32 in between; ``h`` is rounded to its type where it is stored, and ``z`` is the norm of
-    that.  Without ``residual``, ``post_weight``, ``gate`` and ``scale`` there is nothing to join: ``h`` is ``x`` itself."""
+    that.  Without ``residual``, ``post_weight``, ``gate`` and ``scale`` there is nothing to join: ``h`` is ``x`` itself.
+    Sums of squares that float32 does not hold, too large or (where ``eps`` does not stand above them) too small, are taken in 64 bits; a
+    row of zeros stays zeros, with ``eps`` 0 as well."""
     z, _, h = _call(x, weight, residual, post_weight, gate, eps, scale, residual_scale, weight_offset, False)
     return z, h
 
@@ -166,5 +168,5 @@ def block_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor], residual: 
 
     With ``t = h * (weight + weight_offset)`` in float32 the codes of a row are ``round(127 t / max|t|)``, exactly (ties to even): ``z`` is
     not rounded to 16 bits on the way and the root, a factor of the whole row, is in the scale alone.  A row of zeros has
-    scale 0; one that holds an infinity or a NaN has scale NaN."""
+    scale 0, whatever ``eps``; one that holds an infinity or a NaN has scale NaN."""
     return _call(x, weight, residual, post_weight, gate, eps, scale, residual_scale, weight_offset, True)
