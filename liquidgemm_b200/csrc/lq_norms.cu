@@ -218,7 +218,7 @@ __device__ __forceinline__ long row_start(const RowStrides& s, unsigned m, const
 // Whether float32 holds a row's sum of squares, and the `mean` of them and eps: each square may be off by 2^-150, 2^-30 of the least mean here.
 __device__ __forceinline__ bool holds(float ss, float mean) { return ss < 3e38f && mean >= 0x1p-120f; }
 
-// A row of which it does not, element by element in 64 bits: from its operands in memory, or, where that is `formed` already, from its
+// A row of which it does not, element by element in 64 bits: from its operands in memory, or, where that is `formed` for good, from its
 // stream.  A function of its own that ends the row: what hardly any row takes then costs the others no registers (the elements taken again
 // inside the kernel's own code: 7 to 24 % of all rows' time where 16-byte accesses do not go).  `sums`: 32 doubles, the maxima behind them.
 template <typename T, typename R, bool QUANT>
@@ -418,7 +418,8 @@ block_norm_kernel(const __grid_constant__ NormArgs a) {
     const float2 both_of = block_sum_max<QUANT>(ss2.x + ss2.y, top, red[parity][1]);
     const float mean = __fmaf_rn(both_of.x, inv_h, eps);
     if (!holds(both_of.x, mean)) {
-      outlying_row<T, R, QUANT>(a, m, true, outlying);
+      // (from the operands again: a product with the gate that float32 did not hold may have made it so; not where h took the place of one)
+      outlying_row<T, R, QUANT>(a, m, !a.h || a.h == a.x || a.h == a.residual, outlying);
       continue;
     }
     float root = 0.f;
