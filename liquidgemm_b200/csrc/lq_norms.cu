@@ -178,15 +178,15 @@ __device__ __forceinline__ float2 block_sum_max(float s, float m, float* red) {
   return make_float2(s, m);
 }
 
-// A factor of a whole row as the float32 number next to it on the side of zero and what that leaves of it, which is never quite 0: both
-// then take an infinity to the same one.
+// A factor of a whole row as the float32 number next to it on the side of zero and what that leaves of it.  The rest is never quite 0 (beside a
+// factor that dwarfs it: 2^-49), so that both take an infinity to the same one; factors smaller than that are what they are, 0 among them.
 struct Factor {
   float hi, lo;
 };
 __device__ __forceinline__ Factor split(double f) {
   const float hi = __double2float_rz(f);
   const float lo = fabsf(hi) < INFINITY ? (float)(f - (double)hi) : 0.f;
-  return {hi, lo == 0.f ? copysignf(1e-45f, hi) : lo};
+  return {hi, lo == 0.f && fabsf(hi) >= 0x1p-100f ? copysignf(0x1p-149f, hi) : lo};
 }
 
 // (mean of squares + eps)^-1/2 in 64 bits: a float32 root and one step of Newton's iteration.
