@@ -30,6 +30,8 @@ from ._lib import check, lib
 from .moe import _aligned, _plain_call, _refuse, _same_device
 from .ops import _DTYPE_CODES, _dev_ctx, _i8_gemm_scaled, _impl, _libdef, _linear, _quant_per_token, _req
 
+_is_alias_of = torch._C._is_alias_of
+
 MAX_SLOTS = 4096
 MAX_RANK = 256
 MAX_SLICES = 8
@@ -171,8 +173,9 @@ def make_stack(slots: int, rank: int, K: int, widths: Union[int, Sequence[int]],
 
 def load(stack: dict, slot: int, a, b, scale: float = 1.0) -> None:
     """Put an adapter into ``slot``: ``a`` [r, K] and ``b`` [N, r] (a list of such pairs' halves, one for each slice, for a fused
-    projection; ranks may differ, ``None`` for a slice without one), its part multiplied by ``scale`` (``alpha / r``).  Enqueued on the
-    current stream: work on other streams that reads the slot has to be ordered by the caller."""
+    projection; ranks may differ, ``None`` for a slice without one), its part multiplied by ``scale`` (``alpha / r``).  The
+    matrices may be the stack's own (copied aside first).  Enqueued on the current stream: work on other streams that reads the slot has
+    to be ordered by the caller."""
     widths = stack["widths"]
     a, b = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (a, b))
     _req(0 <= slot < stack["rank"].shape[0], f"slot must be 0..{stack['rank'].shape[0] - 1}")
@@ -187,6 +190,10 @@ def load(stack: dict, slot: int, a, b, scale: float = 1.0) -> None:
         _req(a[s].dim() == 2 and a[s].shape[1] == K and 1 <= a[s].shape[0] <= most, f"a must be [1..{most}, {K}]")
         _req(tuple(b[s].shape) == (w, a[s].shape[0]), f"b must be [{w}, {a[s].shape[0]}]")
         ranks.append(a[s].shape[0])
+    def aside(t):   # (the slot is cleared first)
+        return t.clone() if t is not None and (_is_alias_of(t, stack["a"]) or _is_alias_of(t, stack["b"])) else t
+
+    a, b = [aside(t) for t in a], [aside(t) for t in b]
     with torch.no_grad():
         stack["a"][slot].zero_()
         stack["b"][slot].zero_()
