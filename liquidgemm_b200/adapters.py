@@ -246,7 +246,8 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
         bias = bias.reshape(-1)
     code = _DTYPE_CODES[out_dtype]
     blob = layer.get("rs")
-    plain = _plain_call(x, blob if blob is not None else layer["w_i8"], layer["s1"], bias)
+    # (in place only where nothing transforms the call or asks for gradients, the stack's among them: y may be what is not batched)
+    plain = _plain_call(x, blob if blob is not None else layer["w_i8"], layer["s1"], bias, stack["a"], stack["b"], stack["scale"], ids)
     if blob is not None:
         run = _linear if plain else torch.ops.liquidgemm.w4a8_linear
         y = run(x, blob, layer["s_u8"], layer["offset_a"], layer["s1"], bias, layer["N"], layer["K"], 64, code)
@@ -257,4 +258,4 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
         y = product(rows, layer["w_i8"], scales, layer["s1"], code)
         if bias is not None:
             y = y.add_(bias) if plain else y + bias
-    return add(y, x, stack, ids, inplace=True)
+    return add(y, x, stack, ids, inplace=plain)
