@@ -30,7 +30,7 @@ from ._lib import check, lib
 from .moe import _aligned, _plain_call, _refuse, _same_device
 from .ops import _DTYPE_CODES, _dev_ctx, _i8_gemm_scaled, _impl, _libdef, _linear, _quant_per_token, _req
 
-_is_alias_of = torch._C._is_alias_of
+_is_alias_of, _increment_version = torch._C._is_alias_of, torch.autograd.graph.increment_version
 
 MAX_SLOTS = 4096
 MAX_RANK = 256
@@ -130,6 +130,8 @@ def _run(y, x, a, b, rank, scale, ids, widths, inplace):
                                    nbytes, torch._C._cuda_getCurrentRawStream(device.index))
     if code:
         check(code, "adapters_add")
+    if inplace:
+        _increment_version(y)   # autograd may have kept y
     return out
 
 
