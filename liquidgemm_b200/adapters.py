@@ -27,7 +27,7 @@ from typing import Optional, Sequence, Union
 import torch
 
 from ._lib import check, lib
-from .moe import _aligned, _plain_call, _refuse, _same_device
+from .moe import _aligned, _any_requires_grad, _plain_call, _refuse, _same_device
 from .ops import _DTYPE_CODES, _dev_ctx, _i8_gemm_scaled, _impl, _libdef, _linear, _quant_per_token, _req
 
 _is_alias_of, _increment_version = torch._C._is_alias_of, torch.autograd.graph.increment_version
@@ -140,6 +140,8 @@ def _add(y, x, a, b, rank, scale, ids, widths):
 
 
 def _add_(y, x, a, b, rank, scale, ids, widths):
+    torch.is_grad_enabled() and _any_requires_grad(y, x, a, b, scale) and \
+        _refuse("the adapters have no gradients to give: y cannot be changed in place where they are asked for (torch.no_grad, or out of place)")
     _run(y, x, a, b, rank, scale, ids, widths, True)
 
 
@@ -221,7 +223,7 @@ def add(y: torch.Tensor, x: torch.Tensor, stack: dict, ids: torch.Tensor, inplac
     float32): a new tensor, or ``y`` itself, changed, with ``inplace``.
 
     ``ids`` [T] (int32 or int64) names the slot of every row; an id outside the slots, or an empty slot, leaves its row as it is.
-    Both products are summed in float32 and the result is rounded once."""
+    Both products are summed in float32 and the result is rounded once.  In place is refused where gradients are asked for."""
     args = (y, x, stack["a"], stack["b"], stack["rank"], stack["scale"], ids)
     if inplace:
         (_add_ if _plain_call(*args) else torch.ops.liquidgemm.adapters_add_)(*args, stack["widths"])
