@@ -483,7 +483,8 @@ template <typename T, typename R, int NV, bool QUANT>
 static cudaError_t launch_norm(const NormArgs& a, int threads, bool vec, cudaStream_t st) {
   if constexpr (NV <= 4)
     if (vec) return launch_rows(block_norm_kernel<T, R, NV, true, QUANT>, a, threads, st);
-  return launch_rows(block_norm_kernel<T, R, NV, false, QUANT>, a, threads, st);
+  if constexpr (NV >= 2) return launch_rows(block_norm_kernel<T, R, NV, false, QUANT>, a, threads, st);
+  return cudaErrorInvalidValue;   // (none: launch_norm_nv takes NV 1 for 16-byte accesses, NV 8 for single elements alone)
 }
 
 template <typename T, typename R, int NV>
