@@ -251,7 +251,8 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
     code = _DTYPE_CODES[out_dtype]
     blob = layer.get("rs")
     # (in place only where nothing transforms the call or asks for gradients, the stack's among them: y may be what is not batched)
-    plain = _plain_call(x, blob if blob is not None else layer["w_i8"], layer["s1"], bias, stack["a"], stack["b"], stack["scale"], ids)
+    plain = _plain_call(x, blob if blob is not None else layer["w_i8"], layer["s1"], bias, stack["a"], stack["b"], stack["rank"], stack["scale"],
+                        ids)
     if blob is not None:
         run = _linear if plain else torch.ops.liquidgemm.w4a8_linear
         y = run(x, blob, layer["s_u8"], layer["offset_a"], layer["s1"], bias, layer["N"], layer["K"], 64, code)
@@ -262,4 +263,6 @@ def linear(x: torch.Tensor, layer: dict, stack: dict, ids: torch.Tensor, bias: O
         y = product(rows, layer["w_i8"], scales, layer["s1"], code)
         if bias is not None:
             y = y.add_(bias) if plain else y + bias
-    return add(y, x, stack, ids, inplace=plain)
+    if plain:
+        return _run(y, x, stack["a"], stack["b"], stack["rank"], stack["scale"], ids, stack["widths"], True)
+    return add(y, x, stack, ids)
