@@ -28,3 +28,21 @@ def test_large_rows_through_the_norm_of_the_output(T, H, dtype):
     _both(x, weight, residual=_randn(gen, T, H), post_weight=post.to(dtype), gate=4.0 * _randn(gen, H), scale=0.7, residual_scale=1.5)
     _both(x, None, residual=_randn(gen, T, H).to(dtype), post_weight=post, gate=4.0 * _randn(gen, T, H).to(dtype), weight_offset=1.0)
     _both(x, weight, post_weight=post, gate=_randn(gen, T, 1).to(dtype), scale=-3.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H", [8, 256, 1001])
+def test_rows_that_lie_apart(H, dtype):
+    """Two strides, gates of a sequence and of a row, more rows than CTAs: ordinary, large and small rows side by side."""
+    gen = torch.Generator(device="cuda").manual_seed(H)
+    B, S = 40, 60
+    wide = _randn(gen, B, S + 2, H + 24)
+    wide[:, 0::7] *= 1e30
+    wide[:, 3::7] *= 1e-30
+    wide = wide.to(dtype)
+    x, residual = wide[:, 1:S + 1, 8:H + 8], wide[:, 2:S + 2, 16:H + 16]
+    post = (1 + 0.2 * _randn(gen, H)).to(dtype)
+    _both(x, post, eps=0.0)
+    _both(x, None, post_weight=post, residual=residual, gate=_randn(gen, B, 1, H), eps=0.0)
+    _both(x, post, post_weight=post, residual=_randn(gen, B, S, H), gate=_randn(gen, B, S, 1).to(dtype), eps=1e-5)
+    _both(x, post, residual=residual, gate=_randn(gen, S, 1), scale=0.5, eps=1e-5)
