@@ -356,8 +356,8 @@ LQ_API int lq_experts_mlp(const void* x, int x_dtype, const float* weights, cons
  *
  * Low-rank adapters of many requests at once, added to a projection's output: for row t with slot l = ids[t]
  *   out[t, n] = (type of y)(y[t, n] + scales[l] * sum_j b[l, n, j] * (sum_k a[l, s, j, k] * x[t, k])),  j < ranks[l, s],
- * s the slice that column n belongs to; both sums in float32.  A row whose id is outside [0, L) is y's, and so is a slice with
- * ranks[l, s] == 0.  ranks [L, n_slices].
+ * s the slice that column n belongs to; both sums in float32, the inner one carried into the outer as two 16-bit numbers (16 bits of it in
+ * bf16, 22 in fp16).  A row whose id is outside [0, L) is y's, and so is a slice with ranks[l, s] == 0.  ranks [L, n_slices].
  * x [T, K] with rows `ldx` elements apart, a [L, n_slices, rank, K] and b [L, N, rank] in `dtype` (LQ_DT_BF16 or LQ_DT_F16); ranks beyond
  * a slice's own (ranks[l, s] <= rank) are zero in b.  y and out [T, N], rows `ldy` and `ldo` elements apart, in `dtype` or, with
  * y_f32, float32; out == y changes y in place, otherwise they must not overlap.  ids int32, or int64 with ids_64.  widths: a HOST
@@ -382,7 +382,8 @@ LQ_API int lq_adapters_add(const void* x, int dtype, long ldx, const void* a, co
  * (m / inner) * outer + (m % inner) * inner_stride elements behind the pointer (x_outer, x_inner, ...); gate_step 1: H gates a row, 0:
  * one.  z, q and h are contiguous.  H <= 32768; eps >= 0.  Any alignment; 16-byte aligned rows of a multiple of 8 elements are faster.
  * Rows with a sum of squares that float32 does not hold, too large or (beside eps) too small, are taken in 64 bits; rows of zeros stay zeros
- * with eps 0 as well (q_scale 0). */
+ * with eps 0 as well (q_scale 0).  h may be residual or x itself, where that is
+ * contiguous; a row of which a product with the gate exceeds float32 is then not formed anew. */
 LQ_API int lq_block_norm(const void* x, int x_dtype, long x_outer, long x_inner, const void* residual, int stream_dtype,
                          long r_outer, long r_inner, const void* gate, int gate_dtype, long g_outer, long g_inner,
                          int gate_step, const void* weight, int weight_dtype, const void* post, int post_dtype, void* z,
