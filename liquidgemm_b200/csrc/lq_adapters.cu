@@ -953,7 +953,10 @@ template <typename T>
 cudaError_t run_add(const Plan& p, const Call& c, int y_f32) {
   // One launch for few rows.  At 4096 -> 6144 and rank 16 (rows of one adapter / of as many as there are rows), against the three
   // kernels: 1 row 10 us (13), 32 rows 11 / 14 (17 / 26), 64 rows 14 / 16 (25 / 43), 128 rows 20 / 23 (25 / 44).  Every cluster goes over all
-  // columns, so with 28672 of them 64 rows take 29 / 33 (22 / 54) and 128 rows 52 / 57 (27 / 57).
+  // columns, so with 28672 of them 64 rows take 29 / 33 (22 / 54) and 128 rows 52 / 57 (27 / 57).  What the rule costs: the ids are not
+  // known here, nor does it ask for the rank, and every eight rows of one adapter read its matrices again.  64 (65) rows of one adapter /
+  // of their own, slices x rank, columns: 1 x 64, 28672: 58 / 71 us (32 / 118); 2 x 256, 28672: 197 / 265 (61 / 482); 128 (129) rows:
+  // 1 x 256, 8192: 130 / 170 (78 / 410); 2 x 256, 4096: 116 / 160 (80 / 388).  Rows of their own gain where those of one lose.
   long N = 0;
   for (int i = 0; i < c.n_slices; ++i) N += c.widths[i];
   if ((c.T <= 64 || (c.T <= 128 && N <= 8192)) && p.R <= kFewRanks) {

@@ -220,7 +220,8 @@ __device__ __forceinline__ bool holds(float ss, float mean) { return ss < 3e38f 
 
 // A row of which it does not, element by element in 64 bits: from its operands in memory, or, where that is `formed` for good, from its
 // stream.  A function of its own that ends the row: what hardly any row takes then costs the others no registers (the elements taken again
-// inside the kernel's own code: 7 to 24 % of all rows' time where 16-byte accesses do not go).  `sums`: 32 doubles, the maxima behind them.
+// inside the kernel's own code: 7 to 24 % of all rows' time where 16-byte accesses do not go).  Batches of nothing else take two to six
+// times as long (4096 x 4096 to INT8 92 us, 144 with a post-norm).  `sums`: 32 doubles, the maxima behind them.
 template <typename T, typename R, bool QUANT>
 __device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, bool formed, double* sums) {
   const int H = a.H, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -289,11 +290,13 @@ __device__ __noinline__ void outlying_row(const NormArgs& a, unsigned m, bool fo
 // bits, as two float32 numbers) last: h then hangs on two roundings only before its own, and half as many elements as in the
 // order of the formula fall on the other side of a border between two 16-bit numbers than in 64 bits.
 // Bound by the chain of launch, load, reduction(s) and store at few rows (one of 4096: 2.6 us, a launch takes 2.2), by memory at
-// many (16384 x 8192 bf16, stream added and stored: 187 us, 5.7 TB/s; with a float32 stream and gates 310 us, 6.1), and by instruction
-// issue where the rows are quantised as well (4096 x 4096: 27 us, 4.4 TB/s).  Vectors that all rows share stay in L1.  Measured beside
-// it: rows asked for ahead, into registers (fewer warps: 10 to 40 % slower) or through a ring in shared memory (cp.async, two and three
+// many (16384 x 8192 bf16, stream added and stored: 184 us, 5.8 TB/s; with a float32 stream and gates 310 us, 6.1), and by instruction
+// issue where the rows are quantised as well (4096 x 4096: 25 us, 4.6 TB/s), spilled registers among it: 64 a thread, which let an
+// SM hold 1024 threads, do not take all that a row carries (stack bytes a thread at one, two and four units: 0, 8 to 48 and 112 to 272 to
+// 16- and 32-bit rows, 24 to 48, 56 to 120 and 184 to 344 to INT8; single elements at two, four and eight: 56 to 128, 256 to 320, 648 to 744).
+// Vectors that all rows share stay in L1.  Measured beside it: rows asked for ahead, into registers (fewer warps: 10 to 40 % slower) or through a ring in shared memory (cp.async, two and three
 // rows; 170 us for the first of these, 5 to 15 % slower elsewhere); four units a thread on 128 threads (25 us for the last, but 89 instead
-// of 58 at 4096 x 8192).  Rows that 16-byte accesses cannot take (8192 x 5001: 114 us, 2.9 TB/s) are bound by instruction issue too.
+// of 58 at 4096 x 8192).  Rows that 16-byte accesses cannot take (8192 x 5001: 109 us, 3.0 TB/s) are bound by instruction issue too.
 template <typename T, typename R, int NV, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(VEC ? 1024 : 512, VEC ? 1 : 2)
 block_norm_kernel(const __grid_constant__ NormArgs a) {
